@@ -72,6 +72,11 @@ SIGNATURES: dict[str, list[Any]] = {
     "ayk_int8_scaled_mm_workspace_bytes": [_l, _l, _l],
     "ayk_kv_cache_write": [_p, _p, _i, _l, _l, _l, _p, _p, _i, _l, _p, _f, _f, _p],
     "ayk_kv_cache_gather": [_p, _i, _l, _l, _p, _l, _p, _i, _f, _i, _p],
+    "ayk_rms_norm_quant_fp8": [_p, _i, _l, _l, _l, _p, _l, _p, _i, _f, _l, _i, _p, _p, _l, _l, _p, _p],
+    "ayk_paged_decode_attention": [_p, _i, _l, _l, _p, _p, _i, _l, _l, _p, _l, _l, _p, _l, _l, _l, _l, _f, _f, _f, _l, _l,
+                                   _p, _p, _z, _p],
+    "ayk_paged_decode_attention_workspace_bytes": [_l, _l, _l, _l],
+    "ayk_varlen_attention": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _p, _p, _l, _l, _l, _l, _l, _l, _f, _i, _l, _l, _p, _p],
     "ayk_mxfp8_scaled_mm": [_p, _l, _p, _l, _p, _l, _p, _l, _l, _l, _l, _p, _i, _p, _i, _l, _p, _z, _p],
     "ayk_mxfp8_scaled_mm_workspace_bytes": [_l, _l, _l],
     "ayk_fp8_weight_only_gemv": [_p, _i, _p, _l, _l, _l, _p, _i, _l, _l, _l, _p, _p, _z, _p],
@@ -93,6 +98,7 @@ _RESTYPES: dict[str, Any] = {
     "ayk_int8_scaled_mm_workspace_bytes": _z,
     "ayk_mxfp8_scaled_mm_workspace_bytes": _z,
     "ayk_fp8_weight_only_gemm_workspace_bytes": _z,
+    "ayk_paged_decode_attention_workspace_bytes": _z,
     "ayk_fp8_weight_only_gemv_static_max_bytes": _z,
 }
 

@@ -209,5 +209,51 @@ __device__ inline float floor_amax(float amax) {
   return amax < 1e-10f ? 1e-10f : amax;
 }
 
+// MX rule (reference quant.py:47-55): e = clamp(ceil(log2(max(amax/448, 1e-38))),
+// -126, 127) with log2 evaluated in fp32. The fp32 log2 is formed as the fp32
+// rounding of a double-precision log2, i.e. the correctly rounded fp32 result; the
+// only inputs where rounding decides the ceiling are r just above a power of two,
+// where log2(r) lies within half an fp32 ulp of an integer.
+struct MxScale {
+  float inv;     // 2^-e (e <= 120 for every finite fp32 amax); NaN for a NaN group
+  uint8_t code;  // 0 for an all-zero group, else e + 127
+  bool zero;
+};
+// The ceiling read from the bits of ratio = 2^k (1 + M / 2^23): an exact power of two
+// (M == 0) gives k. For M >= 64, log2(1 + M / 2^23) >= 1.1e-5 exceeds half an fp32 ulp
+// of every integer |k| <= 127 (at most 2^-18), so the rounded log2 lies above k and the
+// ceiling is k + 1. A subnormal ratio (at least 1e-38, below 2^-126) has its log2 in
+// (-126.2, -126): the clamped result is -126. Only 1 <= M < 64, and NaN or infinity,
+// evaluate the rounded log2.
+__device__ inline float mx_ceil_log2(float ratio) {
+  const uint32_t b = f2u(ratio);
+  const uint32_t ef = (b >> 23) & 0xFFu, m = b & 0x7FFFFFu;
+  if (ef == 0u) return -126.0f;
+  if (ef != 0xFFu && (m == 0u || m >= 64u)) return (float)((int)ef - 127 + (m != 0u ? 1 : 0));
+  return ceilf((float)log2((double)ratio));
+}
+__device__ inline MxScale mx_scale(float amax) {
+  MxScale r;
+  if (amax != amax) {
+    // A NaN group: the reference's NaN exponent converts to code 0 and every quotient
+    // by its NaN scale is NaN.
+    r.zero = false;
+    r.code = 0;
+    r.inv = amax;
+    return r;
+  }
+  float ratio = amax / kE4M3Max;
+  ratio = ratio < 1e-38f ? 1e-38f : ratio;
+  float e = mx_ceil_log2(ratio);
+  e = e < -126.0f ? -126.0f : (e > 127.0f ? 127.0f : e);
+  const int ei = (int)e;
+  r.zero = (amax == 0.0f);
+  r.code = r.zero ? (uint8_t)0 : (uint8_t)(ei + 127);
+  // 2^-e; 2^-127 (e = 127, only for an infinite amax) is the subnormal 2^-127, so an
+  // infinite element still divides to infinity and clamps to 448 as in the reference.
+  r.inv = ei <= 126 ? u2f((uint32_t)(127 - ei) << 23) : u2f(0x00400000u);
+  return r;
+}
+
 }  // namespace
 }  // namespace ayk

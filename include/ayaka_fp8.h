@@ -288,6 +288,56 @@ int ayk_kv_cache_gather(const void* cache, int cache_dtype, int64_t num_slots, i
                         const int64_t* slots, int64_t n, void* dest, int dest_dtype, float scale,
                         int dequantize, ayk_stream_t stream);
 
+/* ------------------------------------------------------------------ norm
+ * No counterpart in the reference's FP8 path: h = x + residual (x without one), rounded to
+ * x's dtype into residual_out; y = h * weight / sqrt(mean(h^2) + eps) in fp32 from the
+ * unrounded h; then the quantizers' rules. residual and residual_out come together and
+ * must not overlap x or each other; residual_out and q are contiguous [rows, k].
+ *   group == 0: scale[m] = max(amax(y[m]), 1e-10) / 448                  (fp32)
+ *   group > 0:  one scale per (row, group), fp32 (scale_dtype AYK_F32) or UE8M0 codes
+ *               (AYK_U8), at scale[m * scale_row_stride + g * scale_group_stride], laid
+ *               out [rows, k/group] or [k/group, rows] as in the strided quantizer. */
+int ayk_rms_norm_quant_fp8(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t ldx,
+                           const void* residual, int64_t ldr, const void* weight, int weight_dtype,
+                           float eps, int64_t group, int scale_dtype, void* q, void* scale,
+                           int64_t scale_row_stride, int64_t scale_group_stride,
+                           void* residual_out, ayk_stream_t stream);
+
+/* ------------------------------------------------------------------ attention
+ * No counterpart in the reference's FP8 path. Query head h reads kv head h / (heads /
+ * kv_heads). Softmax statistics and sums are fp32; the weights p are rounded once to 16
+ * bits for the product with V. A query that sees nothing gives 0. With window > 0 a query
+ * at position p sees the positions j with p - window < j <= p and j < sinks (j <= p). */
+
+/* One new token per sequence over the paged cache of ayk_kv_cache_write: the query of row b
+ * is at position seq_lens[b] - 1 and sees positions below seq_lens[b], position j at page
+ * block_tables[b * table_stride + j / page_size], offset j % page_size. The caches are
+ * [num_pages, page_size, kv_heads, dim] contiguous, of the query's 16-bit dtype or fp8 with
+ * one scale per plane. A length past table_width * page_size is cut there, and positions of
+ * a page outside [0, num_pages) count as hidden: neither is read. out: [batch, heads, dim]
+ * contiguous, the query's dtype. A workspace smaller than the query's answer, or none,
+ * leaves the work of each sequence unsplit. */
+int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                               const void* key_cache, const void* value_cache, int cache_dtype,
+                               int64_t num_pages, int64_t page_size, const int32_t* block_tables,
+                               int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
+                               int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, float scale,
+                               float k_scale, float v_scale, int64_t window, int64_t sinks, void* out,
+                               void* workspace, size_t workspace_bytes, ayk_stream_t stream);
+size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
+
+/* Packed sequences: sequence b holds query rows [starts_q[b], starts_q[b + 1]) and key rows
+ * [starts_k[b], starts_k[b + 1]); its queries are the last positions of its keys (more
+ * queries than keys: the first ones see nothing when causal). Rows are [*, heads, dim] with
+ * the given strides in elements; out is contiguous [total_q, heads, dim]. Rows of no sequence give 0;
+ * bounds outside the packed rows are cut to them. */
+int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+                         int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
+                         int64_t v_head_stride, int dtype, const int32_t* starts_q, const int32_t* starts_k,
+                         int64_t batch, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
+                         int64_t dim, float scale, int causal, int64_t window, int64_t sinks, void* out,
+                         ayk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
