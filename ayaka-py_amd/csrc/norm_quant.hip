@@ -16,6 +16,178 @@ namespace {
 
 enum { kScaleRow = 0, kScaleGroup = 1, kScaleMx = 2 };
 
+// The sum over a workgroup of NT threads, in a fixed order.
+template <int NT>
+__device__ inline float block_sum(float v, float* red) {
+  v = wave_sum_dpp(v);
+  if constexpr (NT == kWave) return v;
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < NT / kWave; ++i) v += red[i];
+  return v;
+}
+template <int NT>
+__device__ inline uint32_t block_max_u32(uint32_t v, uint32_t* red) {
+  v = wave_max_u32<kWave>(v);
+  if constexpr (NT == kWave) return v;
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < NT / kWave; ++i) v = max(v, red[i]);
+  return v;
+}
+
+// Elements i .. i + V - 1 of the weight, in fp32 (V elements of x fill 16 bytes).
+template <int V>
+__device__ inline void load_weight(const void* w, int w_dtype, int64_t i, float* f) {
+  if (w_dtype == AYK_F32) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) unpack16<F32T>(*reinterpret_cast<const uint4*>(static_cast<const float*>(w) + i + j), f + j);
+    return;
+  }
+  uint4 a{};
+  if constexpr (V == 8) {
+    a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + i);
+  } else {
+    const uint2 half = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + i);
+    a = make_uint4(half.x, half.y, 0, 0);
+  }
+  float t[8];
+  if (w_dtype == AYK_BF16) unpack16<BF16T>(a, t); else unpack16<F16T>(a, t);
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = t[j];
+}
+
+template <typename T>
+__device__ inline void store_vec(typename T::storage* p, const float* f) {
+  if constexpr (T::id == AYK_F32) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = T::id == AYK_BF16 ? f32_to_bf16_bits(f[2 * j]) : f32_to_f16_bits(f[2 * j]);
+      const uint32_t hi = T::id == AYK_BF16 ? f32_to_bf16_bits(f[2 * j + 1]) : f32_to_f16_bits(f[2 * j + 1]);
+      w[j] = lo | hi << 16;
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// One workgroup of NT threads per row, the row's h in VPT 16-byte vectors' worth of fp32 a
+// thread: thread t holds vectors t, t + NT, ... The weight's vectors are asked for before
+// the sum of squares is joined, so that their latency runs beside it. 2^log_gl lanes, neighbours in
+// one wave, hold a group. Rows and groups whose
+// amax is finite take the quantizers' path without special cases.
+template <typename T, int MODE, int NT, int VPT>
+__global__ __launch_bounds__(NT) void rms_quant_vec_kernel(
+    const typename T::storage* __restrict__ x, int64_t ldx, const typename T::storage* __restrict__ res, int64_t ldr,
+    const void* __restrict__ w, int w_dtype, float eps, int64_t k, int log_gl, uint8_t* __restrict__ q,
+    void* __restrict__ scale_out, int64_t srs, int64_t sgs, typename T::storage* __restrict__ res_out) {
+  constexpr int V = Vec16<T>::N;
+  __shared__ float red[2][NT / kWave];
+  const int64_t row = blockIdx.x;
+  const int nvec = (int)(k / V), tid = (int)threadIdx.x;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
+  const uint4* rr = reinterpret_cast<const uint4*>(res + row * ldr);
+  uint4 raw[VPT], more[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * NT;
+    raw[i] = v < nvec ? xr[v] : uint4{};
+    more[i] = res && v < nvec ? rr[v] : uint4{};  // + 0 below, where there is none
+  }
+  float h[VPT][V], wv[VPT][V], ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * NT;
+    if (v < nvec) load_weight<V>(w, w_dtype, (int64_t)v * V, wv[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * NT;
+    unpack16<T>(raw[i], h[i]);
+    if (res) {
+      float r[V];
+      unpack16<T>(more[i], r);
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[i][j] += r[j];
+      if (v < nvec) store_vec<T>(res_out + row * k + (int64_t)v * V, h[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+  }
+  const float rstd = 1.0f / sqrtf(block_sum<NT>(ss, red[0]) / (float)k + eps);
+  uint8_t* qr = q + row * k;
+  uint32_t bits = 0;
+  if constexpr (MODE == kScaleRow) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (tid + i * NT >= nvec) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        h[i][j] = h[i][j] * rstd * wv[i][j];
+        bits = max(bits, f2u(h[i][j]) & 0x7FFFFFFFu);
+      }
+    }
+    bits = block_max_u32<NT>(bits, reinterpret_cast<uint32_t*>(red[1]));
+    const float s = floor_amax(u2f(bits)) / kE4M3Max;
+    if (tid == 0) static_cast<float*>(scale_out)[row] = s;
+    if (bits < kInfBits) {  // workgroup-uniform
+      const float r = 1.0f / s;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (tid + i * NT < nvec) store_quant_finite<V>(qr + (int64_t)(tid + i * NT) * V, h[i], s, r);
+    } else {
+      const Divisor dv{s, 0.0f, false};
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (tid + i * NT < nvec) store_quant<V>(qr + (int64_t)(tid + i * NT) * V, h[i], dv);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * NT;
+      const bool live = v < nvec;  // of a group's lanes all or none: k is a multiple of the group
+      bits = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (live) h[i][j] = h[i][j] * rstd * wv[i][j];
+        bits = max(bits, live ? f2u(h[i][j]) & 0x7FFFFFFFu : 0u);
+      }
+      for (int off = 1 << log_gl >> 1; off > 0; off >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, off, kWave));
+      if (!live) continue;
+      const int64_t at = row * srs + (v >> log_gl) * sgs;
+      uint8_t* dst = qr + (int64_t)v * V;
+      if constexpr (MODE == kScaleMx) {
+        const MxScale ms = mx_scale(u2f(bits));
+        if ((v & ((1 << log_gl) - 1)) == 0) static_cast<uint8_t*>(scale_out)[at] = ms.code;
+        if (bits < kInfBits && !ms.zero) {
+          store_mx_finite<V>(dst, h[i], ms.inv);
+        } else {
+          uint32_t c[V / 4] = {};
+          if (!ms.zero) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) h[i][j] = clamp_e4m3(h[i][j] * ms.inv);
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) c[j] = e4m3x4_encode(h[i][4 * j], h[i][4 * j + 1], h[i][4 * j + 2], h[i][4 * j + 3]);
+          }
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) reinterpret_cast<uint32_t*>(dst)[j] = c[j];
+        }
+      } else {
+        const float s = floor_amax(u2f(bits)) / kE4M3Max;
+        if ((v & ((1 << log_gl) - 1)) == 0) static_cast<float*>(scale_out)[at] = s;
+        if (bits < kInfBits) store_quant_finite<V>(dst, h[i], s, 1.0f / s);
+        else store_quant<V>(dst, h[i], Divisor{s, 0.0f, false});
+      }
+    }
+  }
+}
+
 // Any K, alignment and group size: one workgroup per row, the row walked once per step.
 template <typename T, int MODE>
 __global__ __launch_bounds__(kQuantThreads) void rms_quant_scalar_kernel(
@@ -70,15 +242,52 @@ int launch(const void* x, int64_t rows, int64_t k, int64_t ldx, const void* res,
            float eps, int mode, int64_t group, void* q, void* scale, int64_t srs, int64_t sgs, void* res_out,
            hipStream_t st) {
   using S = typename T::storage;
+  constexpr int V = Vec16<T>::N;
   const S* xs = static_cast<const S*>(x);
   const S* rs = static_cast<const S*>(res);
-#define AYK_RS(MODE)                                                                                            \
-  hipLaunchKernelGGL((rms_quant_scalar_kernel<T, MODE>), dim3((unsigned)rows), dim3(kQuantThreads), 0, st, xs, ldx, rs, \
-                     ldr, w, w_dtype, eps, k, group, static_cast<uint8_t*>(q), scale, srs, sgs, static_cast<S*>(res_out))
+  S* ro = static_cast<S*>(res_out);
+  uint8_t* qb = static_cast<uint8_t*>(q);
+  const int64_t nvec = k / V, gl = group / V;
+  const auto rows16 = [](const void* p, int64_t ld) { return aligned16(p) && ld * (int64_t)sizeof(S) % 16 == 0; };
+  const bool vec = k % V == 0 && nvec <= 4096 && rows16(x, ldx) && (!res || (rows16(res, ldr) && aligned16(ro))) &&
+                   aligned16(w) && (reinterpret_cast<uintptr_t>(q) & 7) == 0 &&
+                   (mode == kScaleRow || (group % V == 0 && gl <= kWave && (gl & (gl - 1)) == 0));
+  int log_gl = 0;
+  while ((int64_t)2 << log_gl <= gl) ++log_gl;
+  const dim3 grid((unsigned)rows);
+#define AYK_RV(MODE, NT, VPT)                                                                                             \
+  hipLaunchKernelGGL((rms_quant_vec_kernel<T, MODE, NT, VPT>), grid, dim3(NT), 0, st, xs, ldx, rs, ldr, w, w_dtype, eps, k, \
+                     log_gl, qb, scale, srs, sgs, ro)
+#define AYK_RM(NT, VPT)                                                                    \
+  do {                                                                                     \
+    if (mode == kScaleRow) AYK_RV(kScaleRow, NT, VPT);                                     \
+    else if (mode == kScaleGroup) AYK_RV(kScaleGroup, NT, VPT);                            \
+    else AYK_RV(kScaleMx, NT, VPT);                                                        \
+    note_plan("rms_quant vec " #NT "x" #VPT);                                              \
+    return check_launch("rms_norm_quant_fp8");                                             \
+  } while (0)
+  if (vec) {
+    // Few rows leave CUs idle, so a row takes one vector a thread; many rows keep up to four
+    // vectors a thread in flight and join fewer waves.
+    const bool few = rows <= 512;
+    if (nvec <= 64) AYK_RM(64, 1);
+    if (nvec <= 128 && !few) AYK_RM(64, 2);
+    if (nvec <= 256) { if (few) AYK_RM(256, 1); else AYK_RM(64, 4); }
+    if (nvec <= 512 && !few) AYK_RM(256, 2);
+    if (nvec <= 1024) { if (few) AYK_RM(1024, 1); else AYK_RM(256, 4); }
+    if (nvec <= 2048) { if (few) AYK_RM(1024, 2); else AYK_RM(512, 4); }
+    AYK_RM(1024, 4);
+  }
+#undef AYK_RM
+#undef AYK_RV
+#define AYK_RS(MODE)                                                                                                    \
+  hipLaunchKernelGGL((rms_quant_scalar_kernel<T, MODE>), grid, dim3(kQuantThreads), 0, st, xs, ldx, rs, ldr, w, w_dtype, eps, \
+                     k, group, qb, scale, srs, sgs, ro)
   if (mode == kScaleRow) AYK_RS(kScaleRow);
   else if (mode == kScaleGroup) AYK_RS(kScaleGroup);
   else AYK_RS(kScaleMx);
 #undef AYK_RS
+  note_plan("rms_quant scalar");
   return check_launch("rms_norm_quant_fp8");
 }
 
