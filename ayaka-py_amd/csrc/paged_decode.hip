@@ -6,6 +6,7 @@
 //
 // with g = h / (heads / kv_heads). HBM-bound: every visible K and V row is read once for all
 // the query heads that share it.
+#include "attn_frag.h"
 #include "attn_rows.h"
 
 namespace ayk {
@@ -47,7 +48,509 @@ __global__ __launch_bounds__(kRowThreads) void paged_decode_rows_kernel(
                      scale, v_scale, out + (b * heads + h) * dim);
 }
 
+// ---------------------------------------------------------------- matrix kernel
+// A wave takes 32 positions of one sequence and kv head at a time, for up to 16 of the query
+// heads that share it: S^T = K Q^T (16x16x32, K the first operand) leaves lane l the scores
+// of head l % 16 at positions 16 t + 4 (l / 16) + i, which is the order in which O^T = V^T P^T
+// wants its second operand if V's k slots are numbered alike. So the weights never cross
+// lanes and K and V go from HBM to registers without LDS: every lane loads 16 bytes of a K row,
+// and of V, for its eight positions, the dims that its column of V^T needs (the transposition
+// is byte permutes within the lane).
+constexpr int kBlock = 32;              // positions a wave takes at a time
+constexpr int kStep = 4 * kBlock;       // positions a workgroup takes at a time
+constexpr int kDecodeThreads = 256;
+constexpr int kHeadTile = 16;
+
+// The blocks of 32 positions that hold a sequence's visible ones: those of the first tokens,
+// then those from the window's first position to the end.
+struct Blocks {
+  int first_blocks, jump, count;  // block i lies at positions 32 (i < first_blocks ? i : i + jump)
+};
+__device__ inline Blocks blocks_of(const Visible& v) {
+  Blocks b;
+  const int end = (int)((v.end + kBlock - 1) / kBlock), from = (int)(v.first / kBlock);
+  const int64_t kept = v.sinks < v.first ? v.sinks : v.first;
+  b.first_blocks = (int)((kept + kBlock - 1) / kBlock);
+  const int second = from > b.first_blocks ? from : b.first_blocks;
+  b.jump = second - b.first_blocks;
+  b.count = b.first_blocks + (end > second ? end - second : 0);
+  return b;
+}
+__device__ inline int steps_of(const int32_t* lens, int64_t b, const PagedCache& c, int64_t window, int64_t sinks) {
+  const int64_t n = cached_length(lens, b, c);
+  return (blocks_of(visible_to(n - 1, n, true, window, sinks)).count + 3) / 4;
+}
+
+struct DecodeArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  PagedCache c;
+  const int32_t* lens;
+  int batch, heads, kv_heads, group, tiles, rows;  // tiles of 16 heads in a group, heads in a full one
+  float scale_log2, v_scale;
+  int64_t window, sinks;
+  uint16_t* out;
+  float* partial;  // split launches: two partial results a workgroup
+  int q_aligned, page_shift;  // page_shift: log2 of the page size, or -1
+};
+
+// What a wave holds of an item.
+template <int CT, int D>
+struct Shape {
+  static constexpr bool kFp8 = CT == AYK_E4M3 || CT == AYK_E5M2;
+  static constexpr int kElem = kFp8 ? 1 : 2;
+  static constexpr int kKWords = D * kElem / 16;    // dwords of a K row in each of its four lanes
+  static constexpr int kSteps = D / 32;             // 32-dim steps of the score product
+  static constexpr int kCols = D / 16;              // dims of a V row in each of its sixteen lanes
+  static constexpr int kVWords = (kCols * kElem + 3) / 4;
+  static constexpr int kPartial = D + 2;            // fp32 values of a partial result a head
+  static constexpr int kWavesPerSimd = D * kElem <= 64 ? 4 : D * kElem <= 128 ? 3 : D * kElem <= 256 ? 2 : 1;  // what its registers leave room for
+};
+
+// First dim of lane quad `quad`'s eight k slots at step s of the score product.
+template <int CT, int D>
+__device__ inline int k_dim(int s, int quad) {
+  if constexpr (Shape<CT, D>::kFp8) return s < 2 * (D / 64) ? 64 * (s / 2) + 16 * quad + 8 * (s % 2) : 64 * (D / 64) + 8 * quad;
+  else return 32 * s + 8 * quad;
+}
+template <int CT, int D>
+__device__ inline void load_k_row(const uint8_t* row, int quad, uint32_t* w) {
+  if constexpr (Shape<CT, D>::kFp8) {
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) *reinterpret_cast<v4u*>(w + 4 * j) = *reinterpret_cast<const v4u*>(row + 64 * j + 16 * quad);
+    if constexpr (D % 64) *reinterpret_cast<uint2*>(w + 4 * (D / 64)) = *reinterpret_cast<const uint2*>(row + 64 * (D / 64) + 8 * quad);
+  } else {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) *reinterpret_cast<v4u*>(w + 4 * s) = *reinterpret_cast<const v4u*>(row + 64 * s + 16 * quad);
+  }
+}
+template <int CT, int QT, int D>
+__device__ inline v4u k_frag(const uint32_t* w, int s) {
+  if constexpr (Shape<CT, D>::kFp8)
+    return v4u{widen2<CT, QT, false>(w[2 * s]), widen2<CT, QT, true>(w[2 * s]), widen2<CT, QT, false>(w[2 * s + 1]),
+               widen2<CT, QT, true>(w[2 * s + 1])};
+  else return v4u{w[4 * s], w[4 * s + 1], w[4 * s + 2], w[4 * s + 3]};
+}
+
+// A lane's dims of a V row: kCols of them in pieces of a power of two, piece by piece 16 lanes
+// side by side. Its t-th dim is v_dim(t, column).
+template <int CT, int D>
+constexpr int v_piece(int t) {  // size of the piece that holds the t-th dim
+  constexpr int most = Shape<CT, D>::kFp8 ? 16 : 8;
+  int at = 0, size = most;
+  while (true) {
+    while (size > D / 16 - at) size /= 2;
+    if (t < at + size) return size;
+    at += size;
+  }
+}
+template <int CT, int D>
+constexpr int v_piece_start(int t) {
+  int at = 0;
+  while (t >= at + v_piece<CT, D>(at)) at += v_piece<CT, D>(at);
+  return at;
+}
+template <int CT, int D>
+struct DimOrder {  // dim of column c: base[t] + c width[t]
+  int base[D / 16], width[D / 16];
+  constexpr DimOrder() : base{}, width{} {
+    for (int t = 0; t < D / 16; ++t) {
+      width[t] = v_piece<CT, D>(t);
+      base[t] = 16 * v_piece_start<CT, D>(t) + t - v_piece_start<CT, D>(t);
+    }
+  }
+};
+template <int CT, int D, int AT = 0>
+__device__ inline void load_v_row(const uint8_t* row, int col, uint32_t* w) {
+  if constexpr (AT < D / 16) {
+    constexpr int e = Shape<CT, D>::kElem, size = v_piece<CT, D>(AT), bytes = size * e;
+    const uint8_t* p = row + (16 * AT + col * size) * e;
+    uint32_t* d = w + AT * e / 4;
+    if constexpr (bytes == 16) *reinterpret_cast<v4u*>(d) = *reinterpret_cast<const v4u*>(p);
+    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(p);
+    else if constexpr (bytes == 4) *d = *reinterpret_cast<const uint32_t*>(p);
+    else *d = *reinterpret_cast<const uint16_t*>(p);
+    load_v_row<CT, D, AT + size>(row, col, w);
+  }
+}
+
+// The lane, as a value that the compiler cannot compute ahead: what depends on it would
+// otherwise be formed before the loop over a workgroup's items and spilled across it (175
+// registers at 128 dims).
+__device__ inline int item_lane() {
+  int lane = threadIdx.x % kWave;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// Registers of the running softmax: maximum (in log2 units), this lane's share of the sum,
+// and O^T, tile t element i at head l % 16, dim t of column 4 (l / 16) + i.
+template <int D>
+struct Running {
+  float m, l;
+  v4f acc[D / 16];
+};
+
+template <int QT, int CT, int D>
+__device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile, int from, int to, Running<D>& r) {
+  using S = Shape<CT, D>;
+  constexpr int PT = S::kFp8 ? AYK_F16 : QT;  // e4m3 and e5m2 are exact in fp16, whose weights round finer
+  const int lane = item_lane(), wave = threadIdx.x / kWave, col = lane % 16, quad = lane / 16;
+  const int64_t n = cached_length(a.lens, b, a.c);
+  const Visible vis = visible_to(n - 1, n, true, a.window, a.sinks);
+  const Blocks bl = blocks_of(vis);
+  r.m = -INFINITY;
+  r.l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) r.acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const int most = bl.count < 4 * to ? bl.count : 4 * to;
+  int i = __builtin_amdgcn_readfirstlane(4 * from + wave);
+  if (i >= most) return;
+
+  // Q of this lane's head in the order of the score product's k slots.
+  const int head = g * a.group + tile * kHeadTile + col;
+  const bool has_head = tile * kHeadTile + col < a.group;
+  v4u qf[S::kSteps];
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    qf[s] = v4u{0, 0, 0, 0};
+    if (has_head) {
+      const uint16_t* p = a.q + b * a.q_row + head * a.q_head + k_dim<CT, D>(s, quad);
+      if (a.q_aligned) {
+        qf[s] = *reinterpret_cast<const v4u*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[s][e] = (uint32_t)p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
+      }
+    }
+  }
+
+  const int32_t* table = a.c.table + b * a.c.table_stride;
+  const int64_t head_at = (int64_t)g * D * S::kElem;
+  const uint32_t page_size = (uint32_t)a.c.page_size, row_bytes = (uint32_t)a.c.row_bytes;
+  const int seen_end = (int)vis.end, seen_first = (int)vis.first, kept = (int)(vis.sinks < vis.first ? vis.sinks : vis.first);
+  auto page_index = [&](uint32_t j) { return a.page_shift >= 0 ? j >> a.page_shift : j / page_size; };
+  // Lane l looks up position l % 32 of a block: its page, a block ahead of the rows.
+  auto position = [&](int blk) { return kBlock * (blk < bl.first_blocks ? blk : blk + bl.jump) + lane % kBlock; };
+  auto page_of = [&](int blk) {
+    const int j = position(blk);
+    return j < seen_end ? table[page_index(j)] : -1;
+  };
+  auto slot_of = [&](int blk, int page) {  // -1: hidden
+    const int j = position(blk);
+    const bool on = j < seen_end && (j >= seen_first || j < kept) && (uint32_t)page < (uint32_t)a.c.num_pages;
+    return on ? (int)((uint32_t)page * page_size + j - page_index(j) * page_size) : -1;
+  };
+  uint32_t kw[2][S::kKWords], vw[8][S::kVWords];
+  auto issue_k = [&](int slot) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int at = __builtin_amdgcn_ds_bpermute(4 * col + 64 * t, slot);
+      load_k_row<CT, D>(a.c.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * row_bytes + head_at, quad, kw[t]);
+    }
+  };
+  auto issue_v = [&](int slot) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = __builtin_amdgcn_ds_bpermute(16 * quad + 64 * (j / 4) + 4 * (j % 4), slot);
+      load_v_row<CT, D>(a.c.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * row_bytes + head_at, col, vw[j]);
+    }
+  };
+  // The next block's K is asked for as soon as this block's is used up, and V likewise, so
+  // that loads are in flight throughout. The scheduling barriers keep them there: moved up,
+  // they would need registers of their own.
+  int slot = slot_of(i, page_of(i));
+  int page = i + 4 < most ? page_of(i + 4) : -1;
+  issue_k(slot);
+  issue_v(slot);
+  while (true) {
+    const bool more = i + 4 < most;
+    const uint32_t seen = (uint32_t)__ballot(slot >= 0);
+    v4f s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int d = 0; d < S::kSteps; ++d) s[t] = mfma16<QT>(k_frag<CT, QT, D>(kw[t], d), qf[d], s[t]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) {
+      slot = slot_of(i + 4, page);
+      if (i + 8 < most) page = page_of(i + 8);
+      issue_k(slot);
+    }
+    float x[8], top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = s[j / 4][j % 4] * a.scale_log2;
+    if (seen != 0xFFFFFFFFu) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int pos = 16 * (j / 4) + 4 * quad + j % 4;
+        const bool on = (seen >> pos) & 1;
+        x[j] = on ? x[j] : -INFINITY;
+#pragma unroll
+        for (int w = 0; w < S::kVWords; ++w) vw[j][w] = on ? vw[j][w] : 0u;  // a weight of 0 times a hidden NaN
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+    top = fmaxf(r.m, max_quads(top));
+    if (__ballot(top > r.m)) {  // wave-uniform: some head's maximum grew
+      const float keep = r.m == -INFINITY ? 0.0f : exp2_fast(r.m - top);
+      r.m = top;
+      r.l *= keep;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) r.acc[t] *= keep;
+    }
+    const float base = r.m == -INFINITY ? 0.0f : r.m;  // nothing visible so far weighs 0
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = exp2_fast(x[j] - base);
+      r.l += x[j];
+    }
+    const v4u p{pack2<PT>(x[0], x[1]), pack2<PT>(x[2], x[3]), pack2<PT>(x[4], x[5]), pack2<PT>(x[6], x[7])};
+    if constexpr (S::kFp8) {
+#pragma unroll
+      for (int w = 0; w < S::kVWords; ++w) {
+        v4u f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // bytes of positions 2j and 2j + 1 side by side
+          const uint32_t lo = __builtin_amdgcn_perm(vw[2 * j + 1][w], vw[2 * j][w], 0x05010400u);
+          f[0][j] = widen2<CT, PT, false>(lo);
+          f[1][j] = widen2<CT, PT, true>(lo);
+          if (4 * w + 2 < S::kCols) {
+            const uint32_t hi = __builtin_amdgcn_perm(vw[2 * j + 1][w], vw[2 * j][w], 0x07030602u);
+            f[2][j] = widen2<CT, PT, false>(hi);
+            f[3][j] = widen2<CT, PT, true>(hi);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * w + e < S::kCols) r.acc[4 * w + e] = mfma16<PT>(f[e], p, r.acc[4 * w + e]);
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < S::kVWords; ++w) {
+        v4u f[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[0][j] = __builtin_amdgcn_perm(vw[2 * j + 1][w], vw[2 * j][w], 0x05040100u);
+          f[1][j] = __builtin_amdgcn_perm(vw[2 * j + 1][w], vw[2 * j][w], 0x07060302u);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) r.acc[2 * w + e] = mfma16<PT>(f[e], p, r.acc[2 * w + e]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!more) break;
+    issue_v(slot);
+    i += 4;
+  }
+}
+
+// Scale a running softmax to a common maximum.
+template <int D>
+__device__ inline float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
+// Join the four waves' results in wave 0: 2 and 3 hand theirs to 0 and 1, then 1 to 0.
+template <int D>
+__device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave]) {
+  const int lane = item_lane(), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int half = 2; half >= 1; half /= 2) {
+    __syncthreads();  // the slots' last readers are done
+    if (wave >= half && wave < 2 * half) {
+      float(*to)[kWave] = lds[wave - half];
+      to[0][lane] = r.m;
+      to[1][lane] = r.l;
+#pragma unroll
+      for (int e = 0; e < D / 4; ++e) to[2 + e][lane] = r.acc[e / 4][e % 4];
+    }
+    __syncthreads();
+    if (wave < half) {
+      const float(*from)[kWave] = lds[wave];
+      const float om = from[0][lane], top = fmaxf(r.m, om);
+      const float mine = weight_of<D>(r.m, top), other = weight_of<D>(om, top);
+      r.m = top;
+      r.l = r.l * mine + from[1][lane] * other;
+#pragma unroll
+      for (int e = 0; e < D / 4; ++e) r.acc[e / 4][e % 4] = r.acc[e / 4][e % 4] * mine + from[2 + e][lane] * other;
+    }
+  }
+}
+
+// Wave 0 writes an item: rounded to the output, or as a partial result
+// (a row of D sums, the maximum and the sum for every head).
+template <int QT, int CT, int D>
+__device__ inline void write_item(const DecodeArgs& a, int b, int g, int tile, const Running<D>& r, float* partial) {
+  const int lane = item_lane(), col = lane % 16, quad = lane / 16;
+  const float l = sum_quads(r.l);
+  constexpr DimOrder<CT, D> order;
+  if (tile * kHeadTile + col >= a.group) return;
+  if (partial) {
+    float* p = partial + col * Shape<CT, D>::kPartial;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) p[order.base[t] + (4 * quad + i) * order.width[t]] = r.acc[t][i];
+    if (quad == 0) {
+      p[D] = r.m;
+      p[D + 1] = l;
+    }
+    return;
+  }
+  const int head = g * a.group + tile * kHeadTile + col;
+  uint16_t* o = a.out + ((int64_t)b * a.heads + head) * D;
+  const float f = l == 0.0f ? 0.0f : a.v_scale / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < D / 16; t += 2)
+      *reinterpret_cast<uint32_t*>(o + order.base[t] + (4 * quad + i) * order.width[t]) = pack2<QT>(r.acc[t][i] * f, r.acc[t + 1][i] * f);
+}
+
+// One workgroup per sequence, kv head and head tile: for calls whose longest possible
+// sequence is a few steps.
+template <int QT, int CT, int D>
+__global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_kernel(DecodeArgs a) {
+  __shared__ float lds[2][D / 4 + 2][kWave];
+  const int g = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads % a.tiles, b = blockIdx.x / a.kv_heads / a.tiles;
+  Running<D> r;
+  attend_blocks<QT, CT, D>(a, b, g, tile, 0, 0x1FFFFFF, r);
+  join_waves<D>(r, lds);
+  if (threadIdx.x < kWave) write_item<QT, CT, D>(a, b, g, tile, r, nullptr);
+}
+
+// The list of every item's steps, sequence by sequence, each with its (tile, kv head) items:
+// how many there are, and where sequence b's begin.
+__device__ inline int total_steps(const DecodeArgs& a) {
+  const int lane = threadIdx.x % kWave;
+  int sum = 0;
+  for (int b = lane; b < a.batch; b += kWave) sum += steps_of(a.lens, b, a.c, a.window, a.sinks);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+  return sum * a.tiles * a.kv_heads;
+}
+
+// Long sequences: the steps of all items are dealt out evenly, a run of `share` consecutive
+// ones to every workgroup, whatever the lengths. A run may end one item, hold some whole and
+// begin another; what it does not hold whole it leaves as a partial result, in slot 0 (the run
+// begins inside the item) or slot 1 (it ends inside).
+template <int QT, int CT, int D>
+__global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_split_kernel(DecodeArgs a) {
+  __shared__ float lds[2][D / 4 + 2][kWave];
+  const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_heads;
+  const int total = __builtin_amdgcn_readfirstlane(total_steps(a));
+  const int share = (total + gridDim.x - 1) / (int)gridDim.x;
+  int at = blockIdx.x * share;
+  const int end = at + share < total ? at + share : total;
+  int before = 0;  // steps of the sequences before chunk
+  for (int chunk = 0; chunk < a.batch && at < end; chunk += kWave) {
+    const int mine = chunk + lane < a.batch ? steps_of(a.lens, chunk + lane, a.c, a.window, a.sinks) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const int v = __shfl_up(upto, off, kWave);
+      if (lane >= off) upto += v;
+    }
+    while (at < end) {
+      // the first sequence whose items end past `at`
+      const uint64_t past = __ballot(before + upto * per > at);
+      if (!past) break;
+      const int k = __builtin_ctzll(past);
+      const int steps = __builtin_amdgcn_readlane(mine, k);
+      const int start = before + (__builtin_amdgcn_readlane(upto, k) - steps) * per;
+      const int item = (at - start) / steps, first = (at - start) - item * steps;
+      const int last = first + (end - at) < steps ? first + (end - at) : steps;
+      Running<D> r;
+      const int b = chunk + k, g = item % a.kv_heads, tile = item / a.kv_heads;
+      attend_blocks<QT, CT, D>(a, b, g, tile, first, last, r);
+      join_waves<D>(r, lds);
+      float* partial = nullptr;
+      if (first > 0 || last < steps)
+        partial = a.partial + ((int64_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * a.rows * Shape<CT, D>::kPartial;
+      if (threadIdx.x < kWave) write_item<QT, CT, D>(a, b, g, tile, r, partial);
+      at += last - first;
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1) * per;
+  }
+}
+
+// Joins the partial results of one (sequence, head) in the order of the runs, and writes the
+// zeros of empty sequences. A workgroup of D threads.
+template <int QT, int D>
+__global__ void paged_decode_join_kernel(DecodeArgs a, int runs) {
+  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x % kWave, per = a.tiles * a.kv_heads;
+  const int g = h / a.group, tile = h % a.group / kHeadTile, col = h % a.group % kHeadTile;
+  int sum = 0, early = 0;  // steps of all sequences, and of those before b
+  for (int s = lane; s < a.batch; s += kWave) {
+    const int n = steps_of(a.lens, s, a.c, a.window, a.sinks);
+    sum += n;
+    early += s < b ? n : 0;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    sum += __shfl_xor(sum, off, kWave);
+    early += __shfl_xor(early, off, kWave);
+  }
+  const int steps = steps_of(a.lens, b, a.c, a.window, a.sinks);
+  const int share = (sum * per + runs - 1) / runs;
+  uint16_t* o = a.out + ((int64_t)b * a.heads + h) * D;
+  const int d = threadIdx.x;
+  if (steps == 0) {
+    if (d < D) o[d] = 0;
+    return;
+  }
+  const int start = early * per + (tile * a.kv_heads + g) * steps;
+  const int w0 = start / share, w1 = (start + steps - 1) / share;
+  if (w0 == w1) return;  // whole in one run, already written
+  const int stride = a.rows * (D + 2);
+  const float* p = a.partial + (int64_t)col * (D + 2);
+  auto slot = [&](int w) { return p + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * stride; };
+  float top = -INFINITY;
+  for (int w = w0; w <= w1; ++w) top = fmaxf(top, slot(w)[D]);
+  float l = 0.0f, acc = 0.0f;
+  for (int w = w0; w <= w1; ++w) {
+    const float* s = slot(w);
+    const float f = weight_of<D>(s[D], top);
+    l += s[D + 1] * f;
+    acc += (d < D ? s[d] : 0.0f) * f;
+  }
+  if (d < D) store_f32(o, QT, d, l == 0.0f ? 0.0f : acc * a.v_scale / l);
+}
+
 bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AYK_E4M3 || dt == AYK_E5M2; }
+
+
+constexpr int kMostRuns = 1024;  // workgroups of a split launch that the chip holds at once, at most
+
+template <int QT, int CT, int D>
+int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
+  if (!split) {
+    hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D>), dim3((unsigned)(a.batch * a.tiles * a.kv_heads)), dim3(kDecodeThreads), 0,
+                       st, a);
+    note_plan("paged_decode whole");
+  } else {
+    constexpr int runs = 256 * Shape<CT, D>::kWavesPerSimd;
+    hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_decode_join_kernel<QT, D>), dim3((unsigned)a.batch, (unsigned)a.heads), dim3(D < kWave ? kWave : D), 0,
+                       st, a, runs);
+    note_plan("paged_decode split");
+  }
+  return check_launch("paged_decode_attention");
+}
+
+template <int QT, int CT>
+int launch_dim(const DecodeArgs& a, int64_t dim, bool split, hipStream_t st) {
+  switch (dim) {
+    case 64: return launch_matrix<QT, CT, 64>(a, split, st);
+    case 96: return launch_matrix<QT, CT, 96>(a, split, st);
+    case 128: return launch_matrix<QT, CT, 128>(a, split, st);
+    case 192: return launch_matrix<QT, CT, 192>(a, split, st);
+    default: return launch_matrix<QT, CT, 256>(a, split, st);
+  }
+}
+bool matrix_dim(int64_t dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256; }
 
 }  // namespace
 }  // namespace ayk
@@ -57,7 +560,9 @@ using namespace ayk;
 extern "C" {
 
 size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
-  return 0;
+  if (!matrix_dim(dim) || kv_heads < 1 || heads < kv_heads || batch < 1) return 0;
+  const int64_t group = heads / kv_heads;
+  return (size_t)(2 * kMostRuns * (group < kHeadTile ? group : kHeadTile) * (dim + 2)) * sizeof(float);
 }
 
 int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -89,12 +594,49 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
   hipStream_t st = static_cast<hipStream_t>(stream);
   const PagedCache c{static_cast<const uint8_t*>(key_cache), static_cast<const uint8_t*>(value_cache), num_pages, page_size,
                      kv_heads * dim * elem_size(cache_dtype), block_tables, table_stride, table_width};
+  const bool bf = q_dtype == AYK_BF16;
+  // The matrix kernels count positions, slots and items in 32 bits and load 16 bytes at a time.
+  const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
+  const int64_t items = batch * tiles * kv_heads;
+  if (matrix_dim(dim) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
+      num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && items < 0x7FFFFFFF) {
+    DecodeArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_row = q_row_stride;
+    a.q_head = q_head_stride;
+    a.c = c;
+    a.lens = seq_lens;
+    a.batch = (int)batch;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)group;
+    a.tiles = (int)tiles;
+    a.rows = (int)(group < kHeadTile ? group : kHeadTile);
+    a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctzll((uint64_t)page_size);
+    a.scale_log2 = scale * k_scale * kLog2e;
+    a.v_scale = v_scale;
+    a.window = window;
+    a.sinks = sinks;
+    a.out = static_cast<uint16_t*>(out);
+    a.partial = static_cast<float*>(workspace);
+    a.q_aligned = aligned16(q) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0;
+    // A sequence of at most four steps stays with one workgroup: a second launch would cost
+    // more than the steps.
+    const int64_t longest = window > 0 && window + sinks < most ? window + sinks + 2 * kBlock : most;
+    const int64_t steps = cdiv(longest, kStep) + 1;
+    const bool split = longest > 4 * kStep && items * steps < 0x40000000 && workspace != nullptr && aligned16(workspace) &&
+                       workspace_bytes >= ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
+    if (cache_dtype == AYK_E4M3)
+      return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, split, st);
+    if (cache_dtype == AYK_E5M2)
+      return bf ? launch_dim<AYK_BF16, AYK_E5M2>(a, dim, split, st) : launch_dim<AYK_F16, AYK_E5M2>(a, dim, split, st);
+    return bf ? launch_dim<AYK_BF16, AYK_BF16>(a, dim, split, st) : launch_dim<AYK_F16, AYK_F16>(a, dim, split, st);
+  }
   const dim3 grid((unsigned)batch, (unsigned)heads);
 #define AYK_PDR(Q, C)                                                                                                  \
   hipLaunchKernelGGL((paged_decode_rows_kernel<Q, C>), grid, dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(q), \
                      q_row_stride, q_head_stride, c, seq_lens, heads, heads / kv_heads, dim, scale * k_scale, v_scale,  \
                      window, sinks, static_cast<uint16_t*>(out))
-  const bool bf = q_dtype == AYK_BF16;
   if (cache_dtype == AYK_E4M3) { if (bf) AYK_PDR(AYK_BF16, AYK_E4M3); else AYK_PDR(AYK_F16, AYK_E4M3); }
   else if (cache_dtype == AYK_E5M2) { if (bf) AYK_PDR(AYK_BF16, AYK_E5M2); else AYK_PDR(AYK_F16, AYK_E5M2); }
   else if (bf) AYK_PDR(AYK_BF16, AYK_BF16);
