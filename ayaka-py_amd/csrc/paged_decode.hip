@@ -86,7 +86,7 @@ struct DecodeArgs {
   int64_t q_row, q_head;
   PagedCache c;
   const int32_t* lens;
-  int batch, heads, kv_heads, group, tiles, rows;  // tiles of 16 heads in a group, heads in a full one
+  int batch, heads, kv_items, group, tiles, rows;  // kv heads or pairs, tiles of 16 heads in a group, columns in use
   float scale_log2, v_scale;
   int64_t window, sinks;
   uint16_t* out;
@@ -103,7 +103,6 @@ struct Shape {
   static constexpr int kSteps = D / 32;             // 32-dim steps of the score product
   static constexpr int kCols = D / 16;              // dims of a V row in each of its sixteen lanes
   static constexpr int kVWords = (kCols * kElem + 3) / 4;
-  static constexpr int kPartial = D + 2;            // fp32 values of a partial result a head
   static constexpr int kWavesPerSimd = D * kElem <= 64 ? 4 : D * kElem <= 128 ? 3 : D * kElem <= 256 ? 2 : 1;  // what its registers leave room for
 };
 
@@ -191,7 +190,21 @@ struct Running {
   v4f acc[D / 16];
 };
 
-template <int QT, int CT, int D>
+// Kv heads of 64 dims are taken two at a time where both groups fit the 16 columns: one 64-dim
+// row fills half a cache line, whose other half, the neighbouring head's, another workgroup
+// would fetch again. K and V rows are then 128 dims, a column's Q is zero on the other head's
+// dims, and the half of O^T that mixes the heads is not written. PACK is 2 then, and the
+// columns of a head are:
+template <int PACK>
+struct Column {
+  static constexpr int kSpan = kHeadTile / PACK;
+  int sub, at;  // kv head within the pair, query head within the tile's share of its group
+  __device__ explicit Column(int col) : sub(col / kSpan), at(col % kSpan) {}
+  __device__ bool used(const DecodeArgs& a, int tile) const { return tile * kHeadTile + at < a.group; }
+  __device__ int head(const DecodeArgs& a, int g, int tile) const { return (g * PACK + sub) * a.group + tile * kHeadTile + at; }
+};
+
+template <int QT, int CT, int D, int PACK>
 __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile, int from, int to, Running<D>& r) {
   using S = Shape<CT, D>;
   constexpr int PT = S::kFp8 ? AYK_F16 : QT;  // e4m3 and e5m2 are exact in fp16, whose weights round finer
@@ -208,14 +221,16 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
   if (i >= most) return;
 
   // Q of this lane's head in the order of the score product's k slots.
-  const int head = g * a.group + tile * kHeadTile + col;
-  const bool has_head = tile * kHeadTile + col < a.group;
+  const Column<PACK> column(col);
+  const int head = column.head(a, g, tile);
+  const bool has_head = column.used(a, tile);
   v4u qf[S::kSteps];
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) {
     qf[s] = v4u{0, 0, 0, 0};
-    if (has_head) {
-      const uint16_t* p = a.q + b * a.q_row + head * a.q_head + k_dim<CT, D>(s, quad);
+    const int dim = k_dim<CT, D>(s, quad);
+    if (has_head && dim / (D / PACK) == column.sub) {
+      const uint16_t* p = a.q + b * a.q_row + head * a.q_head + dim % (D / PACK);
       if (a.q_aligned) {
         qf[s] = *reinterpret_cast<const v4u*>(p);
       } else {
@@ -348,8 +363,7 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
   }
 }
 
-// Scale a running softmax to a common maximum.
-template <int D>
+// What a result under maximum m counts under a common one.
 __device__ inline float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
 
 // Join the four waves' results in wave 0: 2 and 3 hand theirs to 0 and 1, then 1 to 0.
@@ -370,7 +384,7 @@ __device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave])
     if (wave < half) {
       const float(*from)[kWave] = lds[wave];
       const float om = from[0][lane], top = fmaxf(r.m, om);
-      const float mine = weight_of<D>(r.m, top), other = weight_of<D>(om, top);
+      const float mine = weight_of(r.m, top), other = weight_of(om, top);
       r.m = top;
       r.l = r.l * mine + from[1][lane] * other;
 #pragma unroll
@@ -381,44 +395,51 @@ __device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave])
 
 // Wave 0 writes an item: rounded to the output, or as a partial result
 // (a row of D sums, the maximum and the sum for every head).
-template <int QT, int CT, int D>
+template <int QT, int CT, int D, int PACK>
 __device__ inline void write_item(const DecodeArgs& a, int b, int g, int tile, const Running<D>& r, float* partial) {
   const int lane = item_lane(), col = lane % 16, quad = lane / 16;
   const float l = sum_quads(r.l);
   constexpr DimOrder<CT, D> order;
-  if (tile * kHeadTile + col >= a.group) return;
+  const Column<PACK> column(col);
+  if (!column.used(a, tile)) return;
+  constexpr int HD = D / PACK;
   if (partial) {
-    float* p = partial + col * Shape<CT, D>::kPartial;
+    float* p = partial + col * (HD + 2);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) p[order.base[t] + (4 * quad + i) * order.width[t]] = r.acc[t][i];
+      for (int t = 0; t < D / 16; ++t) {
+        const int dim = order.base[t] + (4 * quad + i) * order.width[t];
+        if (PACK == 1 || dim / HD == column.sub) p[dim % HD] = r.acc[t][i];
+      }
     if (quad == 0) {
-      p[D] = r.m;
-      p[D + 1] = l;
+      p[HD] = r.m;
+      p[HD + 1] = l;
     }
     return;
   }
-  const int head = g * a.group + tile * kHeadTile + col;
-  uint16_t* o = a.out + ((int64_t)b * a.heads + head) * D;
+  uint16_t* o = a.out + ((int64_t)b * a.heads + column.head(a, g, tile)) * HD;
   const float f = l == 0.0f ? 0.0f : a.v_scale / l;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int t = 0; t < D / 16; t += 2)
-      *reinterpret_cast<uint32_t*>(o + order.base[t] + (4 * quad + i) * order.width[t]) = pack2<QT>(r.acc[t][i] * f, r.acc[t + 1][i] * f);
+    for (int t = 0; t < D / 16; t += 2) {
+      const int dim = order.base[t] + (4 * quad + i) * order.width[t];
+      if (PACK == 1 || dim / HD == column.sub)
+        *reinterpret_cast<uint32_t*>(o + dim % HD) = pack2<QT>(r.acc[t][i] * f, r.acc[t + 1][i] * f);
+    }
 }
 
 // One workgroup per sequence, kv head and head tile: for calls whose longest possible
 // sequence is a few steps.
-template <int QT, int CT, int D>
+template <int QT, int CT, int D, int PACK>
 __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_kernel(DecodeArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
-  const int g = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads % a.tiles, b = blockIdx.x / a.kv_heads / a.tiles;
+  const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_blocks<QT, CT, D>(a, b, g, tile, 0, 0x1FFFFFF, r);
+  attend_blocks<QT, CT, D, PACK>(a, b, g, tile, 0, 0x1FFFFFF, r);
   join_waves<D>(r, lds);
-  if (threadIdx.x < kWave) write_item<QT, CT, D>(a, b, g, tile, r, nullptr);
+  if (threadIdx.x < kWave) write_item<QT, CT, D, PACK>(a, b, g, tile, r, nullptr);
 }
 
 // The list of every item's steps, sequence by sequence, each with its (tile, kv head) items:
@@ -429,20 +450,21 @@ __device__ inline int total_steps(const DecodeArgs& a) {
   for (int b = lane; b < a.batch; b += kWave) sum += steps_of(a.lens, b, a.c, a.window, a.sinks);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-  return sum * a.tiles * a.kv_heads;
+  return sum * a.tiles * a.kv_items;
 }
 
 // Long sequences: the steps of all items are dealt out evenly, a run of `share` consecutive
 // ones to every workgroup, whatever the lengths. A run may end one item, hold some whole and
 // begin another; what it does not hold whole it leaves as a partial result, in slot 0 (the run
 // begins inside the item) or slot 1 (it ends inside).
-template <int QT, int CT, int D>
+template <int QT, int CT, int D, int PACK>
 __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_split_kernel(DecodeArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
-  const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_heads;
+  const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
   const int total = __builtin_amdgcn_readfirstlane(total_steps(a));
   const int share = (total + gridDim.x - 1) / (int)gridDim.x;
-  int at = blockIdx.x * share;
+  const int run = blockIdx.x;
+  int at = run * share;
   const int end = at + share < total ? at + share : total;
   int before = 0;  // steps of the sequences before chunk
   for (int chunk = 0; chunk < a.batch && at < end; chunk += kWave) {
@@ -463,60 +485,91 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
       const int item = (at - start) / steps, first = (at - start) - item * steps;
       const int last = first + (end - at) < steps ? first + (end - at) : steps;
       Running<D> r;
-      const int b = chunk + k, g = item % a.kv_heads, tile = item / a.kv_heads;
-      attend_blocks<QT, CT, D>(a, b, g, tile, first, last, r);
+      const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
+      attend_blocks<QT, CT, D, PACK>(a, b, g, tile, first, last, r);
       join_waves<D>(r, lds);
       float* partial = nullptr;
       if (first > 0 || last < steps)
-        partial = a.partial + ((int64_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * a.rows * Shape<CT, D>::kPartial;
-      if (threadIdx.x < kWave) write_item<QT, CT, D>(a, b, g, tile, r, partial);
+        partial = a.partial + ((int64_t)run * 2 + (first > 0 ? 0 : 1)) * a.rows * (D / PACK + 2);
+      if (threadIdx.x < kWave) write_item<QT, CT, D, PACK>(a, b, g, tile, r, partial);
       at += last - first;
     }
     before += __builtin_amdgcn_readlane(upto, kWave - 1) * per;
   }
 }
 
-// Joins the partial results of one (sequence, head) in the order of the runs, and writes the
-// zeros of empty sequences. A workgroup of D threads.
-template <int QT, int D>
-__global__ void paged_decode_join_kernel(DecodeArgs a, int runs) {
-  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x % kWave, per = a.tiles * a.kv_heads;
-  const int g = h / a.group, tile = h % a.group / kHeadTile, col = h % a.group % kHeadTile;
+// Joins the partial results of one (sequence, head) and writes the zeros of empty sequences:
+// one wave a head, or four that take the partial results in turn (HEADS = 4 or 1), lane l the
+// dims l, l + 64, ..., summed in order. One long sequence alone has hundreds of partial
+// results: one after the other they took 63 us of 121, by four waves 8 us. Where heads and
+// sequences are many, one wave a head is what the chip holds: 96 sequences of 64 heads took
+// 14 us with four.
+template <int QT, int D, int PACK, int HEADS>
+__global__ __launch_bounds__(kDecodeThreads) void paged_decode_join_kernel(DecodeArgs a, int runs) {
+  constexpr int kPer = (D + kWave - 1) / kWave, kShare = 4 / HEADS;  // waves a head
+  __shared__ float part[4][D + 1];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, per = a.tiles * a.kv_items;
+  const int b = blockIdx.x, h = blockIdx.y * HEADS + wave / kShare;
+  if (h >= a.heads) return;  // whole waves, and no barrier with HEADS > 1
+  const int kv = h / a.group, tile = h % a.group / kHeadTile;
+  const int col = kv % PACK * (kHeadTile / PACK) + h % a.group % kHeadTile;
   int sum = 0, early = 0;  // steps of all sequences, and of those before b
   for (int s = lane; s < a.batch; s += kWave) {
     const int n = steps_of(a.lens, s, a.c, a.window, a.sinks);
     sum += n;
     early += s < b ? n : 0;
   }
+  const int steps = steps_of(a.lens, b, a.c, a.window, a.sinks);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
     sum += __shfl_xor(sum, off, kWave);
     early += __shfl_xor(early, off, kWave);
   }
-  const int steps = steps_of(a.lens, b, a.c, a.window, a.sinks);
   const int share = (sum * per + runs - 1) / runs;
   uint16_t* o = a.out + ((int64_t)b * a.heads + h) * D;
-  const int d = threadIdx.x;
   if (steps == 0) {
-    if (d < D) o[d] = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane + i * kWave < D && wave % kShare == 0) o[lane + i * kWave] = 0;
     return;
   }
-  const int start = early * per + (tile * a.kv_heads + g) * steps;
+  const int start = early * per + (tile * a.kv_items + kv / PACK) * steps;
   const int w0 = start / share, w1 = (start + steps - 1) / share;
   if (w0 == w1) return;  // whole in one run, already written
-  const int stride = a.rows * (D + 2);
+  const int64_t stride = (int64_t)a.rows * (D + 2);
   const float* p = a.partial + (int64_t)col * (D + 2);
   auto slot = [&](int w) { return p + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * stride; };
   float top = -INFINITY;
-  for (int w = w0; w <= w1; ++w) top = fmaxf(top, slot(w)[D]);
-  float l = 0.0f, acc = 0.0f;
-  for (int w = w0; w <= w1; ++w) {
+  for (int w = w0 + lane; w <= w1; w += kWave) top = fmaxf(top, slot(w)[D]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+  float l = 0.0f, acc[kPer] = {};
+#pragma unroll 4
+  for (int w = w0 + wave % kShare; w <= w1; w += kShare) {
     const float* s = slot(w);
-    const float f = weight_of<D>(s[D], top);
+    const float f = weight_of(s[D], top);
     l += s[D + 1] * f;
-    acc += (d < D ? s[d] : 0.0f) * f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane + i * kWave < D) acc[i] += s[lane + i * kWave] * f;
   }
-  if (d < D) store_f32(o, QT, d, l == 0.0f ? 0.0f : acc * a.v_scale / l);
+  if constexpr (kShare > 1) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane + i * kWave < D) part[wave][lane + i * kWave] = acc[i];
+    if (lane == 0) part[wave][D] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    l = part[0][D] + part[1][D] + part[2][D] + part[3][D];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int d = lane + i * kWave;
+      if (d < D) acc[i] = part[0][d] + part[1][d] + part[2][d] + part[3][d];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (lane + i * kWave < D) store_f32(o, QT, lane + i * kWave, l == 0.0f ? 0.0f : acc[i] * a.v_scale / l);
 }
 
 bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AYK_E4M3 || dt == AYK_E5M2; }
@@ -524,26 +577,30 @@ bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AY
 
 constexpr int kMostRuns = 1024;  // workgroups of a split launch that the chip holds at once, at most
 
-template <int QT, int CT, int D>
+template <int QT, int CT, int D, int PACK = 1>
 int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
   if (!split) {
-    hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D>), dim3((unsigned)(a.batch * a.tiles * a.kv_heads)), dim3(kDecodeThreads), 0,
-                       st, a);
+    hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, PACK>), dim3((unsigned)(a.batch * a.tiles * a.kv_items)),
+                       dim3(kDecodeThreads), 0, st, a);
     note_plan("paged_decode whole");
   } else {
     constexpr int runs = 256 * Shape<CT, D>::kWavesPerSimd;
-    hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
-    hipLaunchKernelGGL((paged_decode_join_kernel<QT, D>), dim3((unsigned)a.batch, (unsigned)a.heads), dim3(D < kWave ? kWave : D), 0,
-                       st, a, runs);
+    hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    if ((int64_t)a.batch * a.heads < 1024)
+      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 1>), dim3((unsigned)a.batch, (unsigned)a.heads),
+                         dim3(kDecodeThreads), 0, st, a, runs);
+    else
+      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 4>), dim3((unsigned)a.batch, (unsigned)cdiv(a.heads, 4)),
+                         dim3(kDecodeThreads), 0, st, a, runs);
     note_plan("paged_decode split");
   }
   return check_launch("paged_decode_attention");
 }
 
 template <int QT, int CT>
-int launch_dim(const DecodeArgs& a, int64_t dim, bool split, hipStream_t st) {
+int launch_dim(const DecodeArgs& a, int64_t dim, int pack, bool split, hipStream_t st) {
   switch (dim) {
-    case 64: return launch_matrix<QT, CT, 64>(a, split, st);
+    case 64: return pack == 2 ? launch_matrix<QT, CT, 128, 2>(a, split, st) : launch_matrix<QT, CT, 64>(a, split, st);
     case 96: return launch_matrix<QT, CT, 96>(a, split, st);
     case 128: return launch_matrix<QT, CT, 128>(a, split, st);
     case 192: return launch_matrix<QT, CT, 192>(a, split, st);
@@ -561,8 +618,7 @@ extern "C" {
 
 size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
   if (!matrix_dim(dim) || kv_heads < 1 || heads < kv_heads || batch < 1) return 0;
-  const int64_t group = heads / kv_heads;
-  return (size_t)(2 * kMostRuns * (group < kHeadTile ? group : kHeadTile) * (dim + 2)) * sizeof(float);
+  return (size_t)(2 * kMostRuns * kHeadTile * (dim + 2)) * sizeof(float);
 }
 
 int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -597,7 +653,8 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
   const bool bf = q_dtype == AYK_BF16;
   // The matrix kernels count positions, slots and items in 32 bits and load 16 bytes at a time.
   const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
-  const int64_t items = batch * tiles * kv_heads;
+  const int pack = dim == 64 && group <= kHeadTile / 2 && kv_heads % 2 == 0 ? 2 : 1;
+  const int64_t items = batch * tiles * (kv_heads / pack);
   if (matrix_dim(dim) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
       num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && items < 0x7FFFFFFF) {
     DecodeArgs a{};
@@ -608,10 +665,10 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     a.lens = seq_lens;
     a.batch = (int)batch;
     a.heads = (int)heads;
-    a.kv_heads = (int)kv_heads;
+    a.kv_items = (int)(kv_heads / pack);
     a.group = (int)group;
     a.tiles = (int)tiles;
-    a.rows = (int)(group < kHeadTile ? group : kHeadTile);
+    a.rows = (int)(pack == 1 && group < kHeadTile ? group : kHeadTile);
     a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctzll((uint64_t)page_size);
     a.scale_log2 = scale * k_scale * kLog2e;
     a.v_scale = v_scale;
@@ -627,10 +684,10 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     const bool split = longest > 4 * kStep && items * steps < 0x40000000 && workspace != nullptr && aligned16(workspace) &&
                        workspace_bytes >= ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
     if (cache_dtype == AYK_E4M3)
-      return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, split, st);
+      return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, pack, split, st);
     if (cache_dtype == AYK_E5M2)
-      return bf ? launch_dim<AYK_BF16, AYK_E5M2>(a, dim, split, st) : launch_dim<AYK_F16, AYK_E5M2>(a, dim, split, st);
-    return bf ? launch_dim<AYK_BF16, AYK_BF16>(a, dim, split, st) : launch_dim<AYK_F16, AYK_F16>(a, dim, split, st);
+      return bf ? launch_dim<AYK_BF16, AYK_E5M2>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E5M2>(a, dim, pack, split, st);
+    return bf ? launch_dim<AYK_BF16, AYK_BF16>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_F16>(a, dim, pack, split, st);
   }
   const dim3 grid((unsigned)batch, (unsigned)heads);
 #define AYK_PDR(Q, C)                                                                                                  \
