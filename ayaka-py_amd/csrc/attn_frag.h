@@ -52,6 +52,13 @@ __device__ inline uint32_t widen2(uint32_t w) {
   }
 }
 
+// Four 16-bit elements of one column from LDS: of sixteen lanes that point at 8 bytes each,
+// lanes 4 r .. 4 r + 3 at row r of a 4 x 16 block, lane i gets column i.
+__device__ inline uint2 read_transposed(const uint8_t* lds) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)lds));
+}
+
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Maximum and sum over the lanes l, l ^ 32, and over l, l ^ 16, l ^ 32, l ^ 48.
