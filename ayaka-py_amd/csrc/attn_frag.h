@@ -61,6 +61,13 @@ __device__ inline uint2 read_transposed(const uint8_t* lds) {
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The largest of three, NaN losing to numbers (fmaxf alone costs a canonicalization an operand).
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Maximum and sum over the lanes l, l ^ 32, and over l, l ^ 16, l ^ 32, l ^ 48.
 __device__ inline float max_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);

@@ -148,9 +148,9 @@ struct RunningRows {
 // The weights of a tile, from its scores; s becomes exp2(scale (s - m)).
 template <int D>
 __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[2], float c) {
-  float top = -INFINITY;
+  float top = s[0][0];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+  for (int i = 0; i < 16; ++i) top = max3(top, s[0][i], s[1][i]);
   top = max_halves(top);
   // The maximum moves only when a score beats it by 2^8: until then weights may reach 256,
   // which no sum or 16-bit type minds, and O need not be rescaled.
@@ -172,9 +172,16 @@ __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[2], float c) {
     }
 }
 
-// 16 bytes a lane from offset `at` of a buffer to lds + 16 lane.
-__device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t* lds, uint32_t at) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)lds, 16, at, 0, 0, 0);
+// 16 bytes a lane from offset `at` of a buffer to lds + 16 lane, in assembly: the compiler
+// takes a transposed read of LDS to depend on every direct load in flight and would wait for
+// the next tile's before a tile's second product. The waits are the kernel's own (arrived()),
+// and there is no output register. The idle cycles are those that the write of m0, and of the
+// descriptor's registers by readfirstlane, need before a load reads them.
+__device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lds, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(at), "s"(from), "s"(lds) : "memory");
+}
+__device__ inline uint32_t lds_address(const uint8_t* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
 }
 
 template <int DT, int D, int WAVES>
@@ -186,7 +193,9 @@ __global__ __launch_bounds__(WAVES * kWave, (D <= 128 ? 2 : 1)) void varlen_tile
   // Sequences 1 .. batch, and two without keys: the rows before the first and after the last,
   // which give 0. Of all tiles together those of sequence b begin at its first row / kRows + b,
   // which leaves room for its last, partial one. The last tiles come first: they see most.
-  const int head = blockIdx.x % a.heads, tile = a.tiles - 1 - blockIdx.x / a.heads;
+  // Workgroups go to the eight XCDs in turn: neighbouring heads, which share K and V, to one.
+  const int slot = blockIdx.x % a.heads, head = a.heads % 8 == 0 ? slot % 8 * (a.heads / 8) + slot / 8 : slot;
+  const int tile = a.tiles - 1 - blockIdx.x / a.heads;
   auto first_row = [&](int b) { return b == 0 ? 0 : b == a.batch + 2 ? a.total_q : clamp_row(a.starts_q[b - 1], a.total_q); };
   int lo = 0, hi = a.batch + 2;
   while (hi - lo > 1) {
@@ -242,7 +251,8 @@ __global__ __launch_bounds__(WAVES * kWave, (D <= 128 ? 2 : 1)) void varlen_tile
   }
   const uint16_t* kp = a.k.p + sq.k0 * a.k.row + (head / a.group) * a.k.head;
   const uint16_t* vp = a.v.p + sq.k0 * a.v.row + (head / a.group) * a.v.head;
-  auto issue = [&](int i, uint8_t* kd, uint8_t* vd) {
+  auto issue = [&](int i, const uint8_t* kb, const uint8_t* vb) {
+    const uint32_t kd = lds_address(kb), vd = lds_address(vb);
     const int64_t key = (int64_t)tl.at(i) * kTileKeys;
     const int64_t left = len_k - key < kTileKeys ? len_k - key : kTileKeys;  // at least 1: the tile holds a visible key
     const auto kr = uniform_rsrc(kp + key * a.k.row, (int)(((left - 1) * a.k.row + a.dim) * 2));
