@@ -92,8 +92,13 @@ def varlen_attention(
     if batch == 0:
         return result.zero_()
     query, key, value = rows_of_heads(query), rows_of_heads(key), rows_of_heads(value)
-    _lib.call("ayk_varlen_attention", query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
+    # below 1024 keys a sequence on average no split is taken, and no workspace
+    long = key.shape[0] >= 1024 * batch
+    need = _lib.query("ayk_varlen_attention_split_workspace_bytes", batch, tokens, heads, dim) if long else 0
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    _lib.call("ayk_varlen_attention_split", query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
               key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), _lib.dtype_code(query.dtype),
               cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch, tokens, key.shape[0], heads, key.shape[1], dim,
-              softmax_scale, int(causal), window, sinks, result.data_ptr(), _lib.stream_of(query))
+              softmax_scale, int(causal), window, sinks, result.data_ptr(), _lib.ptr(workspace), need,
+              _lib.stream_of(query))
     return result

@@ -59,14 +59,14 @@ __global__ __launch_bounds__(kRowThreads) void varlen_rows_kernel(Packed q, Pack
 
 
 // ---------------------------------------------------------------- matrix kernel
-// A workgroup takes 32 query rows of one head a wave, and walks over the keys in tiles of 64,
-// K and V of a tile in LDS. S^T = K Q^T (32x32x16, K the first operand) leaves lane l the
+// A workgroup takes 32 query rows of one head a wave, and walks over the keys in tiles of
+// KEYS, K and V of a tile in LDS. S^T = K Q^T (32x32x16, K the first operand) leaves lane l the
 // scores of query l % 32 at keys 32 u + 8 (i / 4) + 4 (l / 32) + i % 4, the order in which
 // O^T = V^T P^T wants its second operand if V's k slots are numbered alike: the weights never
 // cross lanes, a row's maximum and sum are within a lane but for one swap of halves, and V is
 // read transposed from LDS (ds_read_b64_tr_b16).
-constexpr int kTileKeys = 64;
-constexpr int kWaveRows = 32;
+constexpr int kMostSplits = 16;
+constexpr int kWaveRows = 32, kTileWaves = 4, kTileRows = kTileWaves * kWaveRows, kTileThreads = kTileWaves * kWave;
 
 struct VarlenArgs {
   Packed q, k, v;
@@ -76,19 +76,51 @@ struct VarlenArgs {
   int batch, heads, group, dim, tiles, causal;
   float scale, scale_log2;  // scale_log2 is positive; the sign is folded into Q
   uint32_t q_flip, q_keep;  // xor and mask of Q's bits: the scale's sign, or a zero scale
+  int splits;               // parts of the keys, a workgroup each, joined from `partial`
+  float* partial;           // [total_q][heads][splits][dim + 4]: sums, maximum, sum of weights
 };
 
-// The tiles of 64 keys that a workgroup's rows see: those of the first tokens, then those
+// Sequences 1 .. batch, and two without keys, 0 and batch + 1: the rows before the first
+// sequence and after the last, which give 0. find_sequence gives the last one whose order
+// key, order(first row, index), is at most `target`: every lane asks for one of 64 first
+// rows, so that a search is one round trip up to 62 sequences and two up to 3900.
+template <typename Order>
+__device__ inline Sequence find_sequence(const VarlenArgs& a, int target, Order order, int* index) {
+  const int lane = threadIdx.x % kWave;
+  auto first_row = [&](int b) { return b == 0 ? 0 : b == a.batch + 2 ? (int)a.total_q : (int)clamp_row(a.starts_q[b - 1], a.total_q); };
+  int lo = 0, hi = a.batch + 2;
+  while (hi - lo > 63) {
+    const int step = (hi - lo + 63) / 64, b = lo + lane * step;
+    const uint64_t at_most = __ballot(lane == 0 || (b < hi && order(first_row(b < hi ? b : hi), b) <= target));
+    lo += (__builtin_popcountll(at_most) - 1) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  const int b = lo + lane < hi ? lo + lane : hi;
+  const int q = first_row(b), k = b > 0 && b < a.batch + 2 ? (int)clamp_row(a.starts_k[b - 1], a.total_k) : 0;
+  const int at = __builtin_popcountll(__ballot(lane == 0 || (b < hi && order(q, b) <= target))) - 1;
+  Sequence sq{__builtin_amdgcn_readlane(q, at), __builtin_amdgcn_readlane(q, at + 1), 0, 0};
+  *index = lo + at;
+  if (lo + at > 0 && lo + at <= a.batch) {
+    sq.k0 = __builtin_amdgcn_readlane(k, at);
+    sq.k1 = __builtin_amdgcn_readlane(k, at + 1);
+    if (sq.k1 < sq.k0) sq.k1 = sq.k0;
+  }
+  return sq;
+}
+
+// The tiles of KEYS keys that a workgroup's rows see: those of the first tokens, then those
 // from the first row's window to the last row's end.
+template <int KEYS>
 struct Tiles {
   int first_tiles, jump, count;
   __device__ int at(int i) const { return i < first_tiles ? i : i + jump; }
 };
-__device__ inline Tiles tiles_of(int64_t end, int64_t first, int64_t sinks) {
-  Tiles t;
-  const int last = (int)((end + kTileKeys - 1) / kTileKeys), from = (int)(first / kTileKeys);
+template <int KEYS>
+__device__ inline Tiles<KEYS> tiles_of(int64_t end, int64_t first, int64_t sinks) {
+  Tiles<KEYS> t;
+  const int last = (int)((end + KEYS - 1) / KEYS), from = (int)(first / KEYS);
   const int64_t kept = sinks < first ? sinks : first;
-  t.first_tiles = (int)((kept + kTileKeys - 1) / kTileKeys);
+  t.first_tiles = (int)((kept + KEYS - 1) / KEYS);
   const int second = from > t.first_tiles ? from : t.first_tiles;
   t.jump = second - t.first_tiles;
   t.count = t.first_tiles + (last > second ? last - second : 0);
@@ -102,9 +134,10 @@ __device__ inline int k_swizzle(int row) { return D % 128 == 0 ? row & 15 : (row
 template <int D>
 __device__ inline int v_swizzle(int row) { return D % 128 == 0 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
 
-// One query row by one wave, position by position: what is hidden is never touched. For the
-// rows of a wave that met values which are not finite beside positions that some row must not
-// see, where a product with a weight of 0 would spread them.
+// One query row by one wave, position by position: what is hidden is never touched. For rows
+// whose sums came out NaN though their weights did not: a value that is not finite stood at a
+// position that the row must not see, and a product with a weight of 0 spread it (or the row
+// does see one).
 template <int DT>
 __device__ void attend_row_wave(const uint16_t* q, int dim, const Visible& vis, const uint16_t* k, int64_t k_row, const uint16_t* v,
                                 int64_t v_row, float scale, uint16_t* out) {
@@ -137,6 +170,57 @@ __device__ void attend_row_wave(const uint16_t* q, int dim, const Visible& vis, 
     if (lane + i * kWave < dim) store_f32(out, DT, lane + i * kWave, l == 0.0f ? 0.0f : acc[i] / l);
 }
 
+// The tile that is number `rank` of all from the longest on: the tile of a sequence's rows
+// t R .. sees (ahead + (t + 1) R) / KEYS tiles of keys, so a packed batch in its own order would
+// end with some workgroups at the longest tiles and the chip idle (8 prompts of 350 to 1500:
+// 122 us). Lane b holds sequence b; the length at which the count of longer tiles passes `rank`
+// is found by bisection. Causal, at most 62 sequences; false past the last tile.
+template <int R, int KEYS>
+__device__ inline bool find_ranked(const VarlenArgs& a, int rank, Sequence* sq, int* tile) {
+  const int lane = threadIdx.x % kWave, b = lane < a.batch + 2 ? lane : a.batch + 2;
+  const int q = b == 0 ? 0 : b == a.batch + 2 ? (int)a.total_q : (int)clamp_row(a.starts_q[b - 1], a.total_q);
+  const int k = b > 0 && b < a.batch + 2 ? (int)clamp_row(a.starts_k[b - 1], a.total_k) : 0;
+  const int q1 = __shfl_down(q, 1, kWave), kn = __shfl_down(k, 1, kWave);
+  const bool real = lane > 0 && lane <= a.batch;
+  const int len_q = lane < a.batch + 2 && q1 > q ? q1 - q : 0, len_k = real && kn > k ? kn - k : 0;
+  // keys of tile t: reach + t (R / 64), in tiles of KEYS; a sequence without keys counts 0 for all
+  const int tiles = (len_q + R - 1) / R, reach = len_k == 0 ? 0 : (len_k - len_q + R) / KEYS, step = len_k == 0 ? 0 : R / KEYS;
+  auto at_least = [&](int len) {  // this sequence's tiles of at least `len` tiles of keys
+    if (step == 0) return len <= 0 ? tiles : 0;
+    const int t = len <= reach ? 0 : (len - reach + step - 1) / step;
+    return t < tiles ? tiles - t : 0;
+  };
+  auto sum = [](int v) { return (int)wave_sum_dpp((float)v); };  // below 2^24
+  if (rank >= sum(tiles)) return false;
+  int low = reach < 0 ? reach : 0, high = reach + tiles * step + 1;  // more than `rank` tiles reach `low`, none `high`
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    low = min(low, __shfl_xor(low, off, kWave));
+    high = max(high, __shfl_xor(high, off, kWave));
+  }
+  while (high - low > 1) {
+    const int mid = low + (high - low) / 2;
+    if (sum(at_least(mid)) > rank) low = mid; else high = mid;
+  }
+  const int longer = at_least(high), these = at_least(low) - longer;
+  int before = these;  // tiles of this length in the sequences up to this one
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int v = __shfl_up(before, off, kWave);
+    if (lane >= off) before += v;
+  }
+  const int left = rank - sum(longer), at = __builtin_ctzll(__ballot(before > left));
+  *tile = __builtin_amdgcn_readlane(tiles - longer - 1, at) - (left - (__builtin_amdgcn_readlane(before, at) - __builtin_amdgcn_readlane(these, at)));
+  sq->q0 = __builtin_amdgcn_readlane(q, at);
+  sq->q1 = __builtin_amdgcn_readlane(q, at + 1);
+  sq->k0 = sq->k1 = 0;
+  if (at > 0 && at <= a.batch) {
+    sq->k0 = __builtin_amdgcn_readlane(k, at);
+    sq->k1 = __builtin_amdgcn_readlane(kn > k ? kn : k, at);
+  }
+  return true;
+}
+
 // A wave's running softmax over its 32 rows: lane l holds query l % 32, and of O^T tile t the
 // dims 32 t + 8 (i / 4) + 4 (l / 32) + i % 4.
 template <int D>
@@ -146,11 +230,11 @@ struct RunningRows {
 };
 
 // The weights of a tile, from its scores; s becomes exp2(scale (s - m)).
-template <int D>
-__device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[2], float c) {
+template <int D, int U>
+__device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
   float top = s[0][0];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max3(top, s[0][i], s[1][i]);
+  for (int i = 0; i < 16; i += 3 - U) top = max3(top, s[0][i], U == 2 ? s[U - 1][i] : s[0][i + 1]);
   top = max_halves(top);
   // The maximum moves only when a score beats it by 2^8: until then weights may reach 256,
   // which no sum or 16-bit type minds, and O need not be rescaled.
@@ -164,7 +248,7 @@ __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[2], float c) {
   }
   const float base = r.m == -INFINITY ? 0.0f : r.m * c;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[u][i] = exp2_fast(fmaf(s[u][i], c, -base));
@@ -172,47 +256,48 @@ __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[2], float c) {
     }
 }
 
+// This wave's direct loads have landed and its LDS reads are done; then the workgroup's barrier.
+__device__ inline void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+
 // 16 bytes a lane from offset `at` of a buffer to lds + 16 lane, in assembly: the compiler
 // takes a transposed read of LDS to depend on every direct load in flight and would wait for
-// the next tile's before a tile's second product. The waits are the kernel's own (arrived()),
+// the next tile's before a tile's second product. The waits are the kernel's own (tile_barrier),
 // and there is no output register. The idle cycles are those that the write of m0, and of the
 // descriptor's registers by readfirstlane, need before a load reads them.
 __device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lds, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(at), "s"(from), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(at), "s"(from), "s"(lds));
 }
 __device__ inline uint32_t lds_address(const uint8_t* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
 }
 
-template <int DT, int D, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, (D <= 128 ? 2 : 1)) void varlen_tile_kernel(VarlenArgs a) {
-  constexpr int kRows = WAVES * kWaveRows, kBytes = kTileKeys * D * 2, kChunks = D / 8, kDma = kBytes / 1024 / WAVES;
-  __shared__ __attribute__((aligned(16))) uint8_t k0[kBytes], k1[kBytes], v0[kBytes], v1[kBytes];
+template <int DT, int D, int KEYS>
+__global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs a) {
+  constexpr int WAVES = kTileWaves;
+  constexpr int kRows = kTileRows, kBytes = KEYS * D * 2, kChunks = D / 8, kDma = kBytes / 1024 / WAVES;
+  constexpr int kSub = KEYS / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kBytes];  // two stages of K, then V
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane / 32, row = lane % 32;
 
-  // Sequences 1 .. batch, and two without keys: the rows before the first and after the last,
-  // which give 0. Of all tiles together those of sequence b begin at its first row / kRows + b,
-  // which leaves room for its last, partial one. The last tiles come first: they see most.
-  // Workgroups go to the eight XCDs in turn: neighbouring heads, which share K and V, to one.
+  // Of all tiles together those of sequence b begin at its first row / kRows + b, which leaves
+  // room for its last, partial one. The tiles that see most come first. Workgroups go to
+  // the eight XCDs in turn: neighbouring heads, which share K and V, to one.
   const int slot = blockIdx.x % a.heads, head = a.heads % 8 == 0 ? slot % 8 * (a.heads / 8) + slot / 8 : slot;
-  const int tile = a.tiles - 1 - blockIdx.x / a.heads;
-  auto first_row = [&](int b) { return b == 0 ? 0 : b == a.batch + 2 ? a.total_q : clamp_row(a.starts_q[b - 1], a.total_q); };
-  int lo = 0, hi = a.batch + 2;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if ((int)(first_row(mid) / kRows) + mid <= tile) lo = mid; else hi = mid;
+  const int part = blockIdx.x / a.heads % a.splits, rank = blockIdx.x / a.heads / a.splits;
+  Sequence sq;
+  int tile;  // of the sequence
+  if (a.causal && a.batch > 1 && a.batch <= 61) {
+    if (!find_ranked<kRows, KEYS>(a, rank, &sq, &tile)) return;
+  } else {
+    int b;
+    sq = find_sequence(a, a.tiles - 1 - rank, [](int row, int b) { return row / kRows + b; }, &b);
+    tile = a.tiles - 1 - rank - ((int)sq.q0 / kRows + b);
   }
-  Sequence sq{first_row(lo), first_row(lo + 1), 0, 0};
-  if (lo > 0 && lo <= a.batch) {
-    sq.k0 = clamp_row(a.starts_k[lo - 1], a.total_k);
-    sq.k1 = clamp_row(a.starts_k[lo], a.total_k);
-    if (sq.k1 < sq.k0) sq.k1 = sq.k0;
-  }
-  const int64_t r0 = (int64_t)(tile - (int)(sq.q0 / kRows) - lo) * kRows, len_q = sq.q1 - sq.q0, len_k = sq.k1 - sq.k0;
+  const int64_t r0 = (int64_t)tile * kRows, len_q = sq.q1 - sq.q0, len_k = sq.k1 - sq.k0;
   if (r0 < 0 || r0 >= len_q) return;
   const int64_t ahead = len_k - len_q;  // row r sits at position r + ahead
   const int64_t last_row = (r0 + kRows < len_q ? r0 + kRows : len_q) - 1;
-  const Tiles tl = tiles_of(visible_to(last_row + ahead, len_k, a.causal, a.window, a.sinks).end,
+  const Tiles<KEYS> tl = tiles_of<KEYS>(visible_to(last_row + ahead, len_k, a.causal, a.window, a.sinks).end,
                             visible_to(r0 + ahead, len_k, a.causal, a.window, a.sinks).first, a.window > 0 ? a.sinks : 0);
   // This wave's rows, and this lane's.
   const int64_t w0 = r0 + wave * kWaveRows;
@@ -227,16 +312,7 @@ __global__ __launch_bounds__(WAVES * kWave, (D <= 128 ? 2 : 1)) void varlen_tile
   // but for the first tokens, before any_first.
   const int all_end = (int)top_row.end, all_first = (int)low_row.first, any_end = (int)low_row.end, any_first = (int)top_row.first;
   const int any_kept = (int)(low_row.sinks < low_row.first ? low_row.sinks : low_row.first);
-
-  v4u qf[D / 16];
-  {
-    const uint16_t* p = a.q.p + (sq.q0 + my_row) * a.q.row + head * a.q.head + 8 * half;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      qf[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const v4u*>(p + 16 * s) : v4u{0, 0, 0, 0};
-      qf[s] = (qf[s] ^ a.q_flip) & a.q_keep;
-    }
-  }
+  const int share = (tl.count + a.splits - 1) / a.splits, from = part * share, to = from + share < tl.count ? from + share : tl.count;
 
   // Direct loads into LDS: instruction n of a wave fills 1024 bytes, lane l the 16 at
   // 1024 (n WAVES + wave) + 16 l of the tile, from the chunk that the permutation puts there.
@@ -251,19 +327,29 @@ __global__ __launch_bounds__(WAVES * kWave, (D <= 128 ? 2 : 1)) void varlen_tile
   }
   const uint16_t* kp = a.k.p + sq.k0 * a.k.row + (head / a.group) * a.k.head;
   const uint16_t* vp = a.v.p + sq.k0 * a.v.row + (head / a.group) * a.v.head;
-  auto issue = [&](int i, const uint8_t* kb, const uint8_t* vb) {
-    const uint32_t kd = lds_address(kb), vd = lds_address(vb);
-    const int64_t key = (int64_t)tl.at(i) * kTileKeys;
-    const int64_t left = len_k - key < kTileKeys ? len_k - key : kTileKeys;  // at least 1: the tile holds a visible key
-    const auto kr = uniform_rsrc(kp + key * a.k.row, (int)(((left - 1) * a.k.row + a.dim) * 2));
-    const auto vr = uniform_rsrc(vp + key * a.v.row, (int)(((left - 1) * a.v.row + a.dim) * 2));
+  auto issue = [&](int i, int stage) {
+    const int64_t key = (int64_t)tl.at(i) * KEYS;
+    const int left = (int)(len_k - key < KEYS ? len_k - key : KEYS);  // at least 1: the tile holds a visible key
+    const auto kr = uniform_rsrc(kp + key * a.k.row, ((left - 1) * (int)a.k.row + a.dim) * 2);
+    const auto vr = uniform_rsrc(vp + key * a.v.row, ((left - 1) * (int)a.v.row + a.dim) * 2);
+    const uint32_t to = lds_address(lds + stage * 2 * kBytes + wave * 1024);
 #pragma unroll
-    for (int n = 0; n < kDma; ++n)
-      load_to_lds(kr, kd + (n * WAVES + wave) * 1024, k_off[n]);
+    for (int n = 0; n < kDma; ++n) load_to_lds(kr, to + n * WAVES * 1024, k_off[n]);
 #pragma unroll
-    for (int n = 0; n < kDma; ++n)
-      load_to_lds(vr, vd + (n * WAVES + wave) * 1024, v_off[n]);
+    for (int n = 0; n < kDma; ++n) load_to_lds(vr, to + kBytes + n * WAVES * 1024, v_off[n]);
   };
+
+  if (from < to) issue(from, 0);
+
+  v4u qf[D / 16];
+  {
+    const uint16_t* p = a.q.p + (sq.q0 + my_row) * a.q.row + head * a.q.head + 8 * half;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      qf[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const v4u*>(p + 16 * s) : v4u{0, 0, 0, 0};
+      qf[s] = (qf[s] ^ a.q_flip) & a.q_keep;
+    }
+  }
 
   RunningRows<D> r;
   r.m = -INFINITY;
@@ -287,100 +373,196 @@ __global__ __launch_bounds__(WAVES * kWave, (D <= 128 ? 2 : 1)) void varlen_tile
     return v4u{low.x, low.y, high.x, high.y};
   };
 
-  float odd = 0.0f;  // NaN once a tile that some row sees in part held a value that is not finite
-  auto compute = [&](int i, const uint8_t* kb, const uint8_t* vb) {
-    const int key = tl.at(i) * kTileKeys;
-    if (!has_rows || key >= any_end || (key + kTileKeys <= any_first && key >= any_kept)) return;
-    v16f s[2];
+  auto compute = [&](int i, const uint8_t* kb) {
+    const uint8_t* vb = kb + kBytes;
+    const int key = tl.at(i) * KEYS;
+    if (!has_rows || key >= any_end || (key + KEYS <= any_first && key >= any_kept))  return;
+    v16f s[kSub];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) s[u] = mfma32<DT>(key_frag(kb, u, d), qf[d], s[u]);
     }
-    const bool whole = key >= all_first && key + kTileKeys <= all_end;
-    if (!whole) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) s[u] = mfma32<DT>(key_frag(kb, u, d), qf[d], s[u]);
+    const bool whole = key >= all_first && key + KEYS <= all_end;
+    if (!whole) {
+      // Key j of this lane's slot e is at + n with n known at compile time: without a window one
+      // comparison an element, with one an unsigned one and the first tokens'.
+      const int at = key + 4 * half, below = end - at;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int j = key + 32 * u + 8 * (e / 4) + 4 * half + e % 4;
-          s[u][e] = j < end && (j >= first || j < kept) ? s[u][e] : -INFINITY;
+          const int n = 32 * u + 8 * (e / 4) + e % 4;
+          if (a.window == 0) s[u][e] = n < below ? s[u][e] : -INFINITY;
+          else if (key >= any_kept) s[u][e] = (uint32_t)(at - first + n) < (uint32_t)(end - first) ? s[u][e] : -INFINITY;
+          else s[u][e] = at + n < end && (at + n >= first || at + n < kept) ? s[u][e] : -INFINITY;
         }
     }
-    softmax_tile<D>(r, s, a.scale_log2);
-    v4u p[4];
+    softmax_tile<D, kSub>(r, s, a.scale_log2);
+    v4u p[KEYS / 16];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < KEYS / 16; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) p[k][e] = pack2<DT>(s[k / 2][8 * (k % 2) + 2 * e], s[k / 2][8 * (k % 2) + 2 * e + 1]);
-    if (!whole) {
-      // A hidden value times a weight of 0 must not reach the sum: does the tile hold one that
-      // is not finite? V^T 0 is 0 if not, NaN if so.
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
-        v16f z;
+    for (int k = 0; k < KEYS / 16; ++k)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z[e] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) z = mfma32<DT>(value_frag(vb, t, k), v4u{0, 0, 0, 0}, z);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) odd += z[e];
-      }
+      for (int t = 0; t < D / 32; ++t) r.acc[t] = mfma32<DT>(value_frag(vb, t, k), p[k], r.acc[t]);
+  };
+
+  // Two stages: a tile is on its way while the one before is used. One barrier a tile says
+  // that it has arrived for every wave and that the other stage, which the next loads fill, is
+  // no longer read.
+  auto turn = [&](int i, int stage) {
+    tile_barrier();
+    if (i + 1 < to) issue(i + 1, 1 - stage);
+    compute(i, lds + stage * 2 * kBytes);
+  };
+  for (int i = from; i < to; i += 2) {
+    turn(i, 0);
+    if (i + 1 < to) turn(i + 1, 1);
+  }
+
+  const float l = sum_halves(r.l);
+  if (a.splits > 1) {
+    if (w0 + row >= len_q) return;
+    float* p = a.partial + (((sq.q0 + w0 + row) * a.heads + head) * a.splits + part) * (a.dim + 4);
+    if (half == 0) {
+      p[a.dim] = r.m;
+      p[a.dim + 1] = l;
     }
+    if (r.m == -INFINITY) return;  // nothing seen: the join reads no sums
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r.acc[t] = mfma32<DT>(value_frag(vb, t, k), p[k], r.acc[t]);
-  };
-
-  // Two tile buffers: the next tile's loads run beside a tile's products, and one barrier a
-  // tile says that they have arrived and that the old tile is no longer read.
-  auto arrived = [&] {
-    wait_vmcnt<0>();
-    __syncthreads();
-  };
-  if (tl.count > 0) {
-    issue(0, k0, v0);
-    arrived();
-  }
-  for (int i = 0; i < tl.count; i += 2) {
-    if (i + 1 < tl.count) issue(i + 1, k1, v1);
-    compute(i, k0, v0);
-    arrived();
-    if (i + 1 >= tl.count) break;
-    if (i + 2 < tl.count) issue(i + 2, k0, v0);
-    compute(i + 1, k1, v1);
-    arrived();
-  }
-
-  if (__ballot(odd != odd)) {
-    for (int64_t i = w0; i <= w1; ++i)
-      attend_row_wave<DT>(a.q.p + (sq.q0 + i) * a.q.row + head * a.q.head, a.dim, visible_to(i + ahead, len_k, a.causal, a.window, a.sinks),
-                          kp, a.k.row, vp, a.v.row, a.scale, a.out + ((sq.q0 + i) * a.heads + head) * a.dim);
+      for (int e = 0; e < 4; ++e)
+        if (32 * t + 8 * e < a.dim)
+          *reinterpret_cast<v4f*>(p + 32 * t + 8 * e + 4 * half) = v4f{r.acc[t][4 * e], r.acc[t][4 * e + 1], r.acc[t][4 * e + 2], r.acc[t][4 * e + 3]};
     return;
   }
-  const float l = sum_halves(r.l);
-  if (w0 + row >= len_q) return;
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* o = a.out + ((sq.q0 + w0 + row) * a.heads + head) * a.dim + 4 * half;
+  float odd = 0.0f;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (32 * t + 8 * e < a.dim)
-        *reinterpret_cast<uint2*>(o + 32 * t + 8 * e) = make_uint2(pack2<DT>(r.acc[t][4 * e] * f, r.acc[t][4 * e + 1] * f),
-                                                                   pack2<DT>(r.acc[t][4 * e + 2] * f, r.acc[t][4 * e + 3] * f));
+    for (int e = 0; e < 16; ++e) odd = r.acc[t][e] != r.acc[t][e] ? NAN : odd;
+  uint64_t again = __ballot(odd != odd && l == l && w0 + row < len_q);
+  if (w0 + row < len_q) {
+    uint16_t* o = a.out + ((sq.q0 + w0 + row) * a.heads + head) * a.dim + 4 * half;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (32 * t + 8 * e < a.dim)
+          *reinterpret_cast<uint2*>(o + 32 * t + 8 * e) = make_uint2(pack2<DT>(r.acc[t][4 * e] * f, r.acc[t][4 * e + 1] * f),
+                                                                     pack2<DT>(r.acc[t][4 * e + 2] * f, r.acc[t][4 * e + 3] * f));
+  }
+  again |= again >> 32;
+  for (again &= 0xFFFFFFFFull; again; again &= again - 1) {
+    const int64_t i = w0 + __builtin_ctzll(again);
+    attend_row_wave<DT>(a.q.p + (sq.q0 + i) * a.q.row + head * a.q.head, a.dim, visible_to(i + ahead, len_k, a.causal, a.window, a.sinks),
+                        kp, a.k.row, vp, a.v.row, a.scale, a.out + ((sq.q0 + i) * a.heads + head) * a.dim);
+  }
 }
 
-template <int DT, int D>
+// Joins the parts of one row and head: 32 lanes each, four dims a lane at a time.
+template <int DT>
+__global__ __launch_bounds__(kRowThreads) void varlen_join_kernel(VarlenArgs a) {
+  const int lane = threadIdx.x % 32;
+  const int64_t all = a.total_q * a.heads, mine = (int64_t)blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32;
+  const int64_t at = mine < all ? mine : all - 1;  // no lane leaves: the wave may search below
+  const int width = a.dim + 4;
+  const float* p = a.partial + at * a.splits * width;
+  const float mine_m = lane < a.splits ? p[lane * width + a.dim] : -INFINITY;  // kMostSplits <= 32
+  const float mine_l = lane < a.splits ? p[lane * width + a.dim + 1] : 0.0f;
+  float top = mine_m, l;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 32));
+  const float mine_f = mine_m == -INFINITY ? 0.0f : exp2_fast((mine_m - top) * a.scale_log2);
+  l = mine_m == -INFINITY ? 0.0f : mine_l * mine_f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 32);
+  v4f acc[2] = {};
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) {
+    const float f = __shfl(mine_f, i, 32), m = __shfl(mine_m, i, 32);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const int dim = 128 * d + 4 * lane;
+      const v4f s = dim < a.dim && m != -INFINITY ? *reinterpret_cast<const v4f*>(p + i * width + dim) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      acc[d] += s * f;
+    }
+  }
+  uint16_t* o = a.out + at * a.dim;
+  const float r = l == 0.0f ? 0.0f : 1.0f / l;
+  float odd = 0.0f;
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd = acc[d][e] != acc[d][e] ? NAN : odd;
+    const int dim = 128 * d + 4 * lane;
+    if (dim < a.dim && mine < all)
+      *reinterpret_cast<uint2*>(o + dim) = make_uint2(pack2<DT>(acc[d][0] * r, acc[d][1] * r), pack2<DT>(acc[d][2] * r, acc[d][3] * r));
+  }
+  const uint64_t again = __ballot(odd != odd && l == l && mine < all);
+  for (int h = 0; h < 2; ++h) {
+    if (!(again >> (32 * h) & 0xFFFFFFFFu)) continue;
+    const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + threadIdx.x / kWave * 2 + h, row = item / a.heads;
+    const int head = (int)(item % a.heads);
+    int b;
+    const Sequence sq = find_sequence(a, (int)row, [](int first, int) { return first; }, &b);
+    const int64_t len_k = sq.k1 - sq.k0, position = row - sq.q0 + len_k - (sq.q1 - sq.q0);
+    attend_row_wave<DT>(a.q.p + row * a.q.row + head * a.q.head, a.dim, visible_to(position, len_k, a.causal, a.window, a.sinks),
+                        a.k.p + sq.k0 * a.k.row + head / a.group * a.k.head, a.k.row, a.v.p + sq.k0 * a.v.row + head / a.group * a.v.head,
+                        a.v.row, a.scale, a.out + item * a.dim);
+  }
+}
+
+// Workgroups of a launch whose keys are whole, about: what the chip holds at two a CU is 512.
+int64_t whole_groups(int64_t batch, int64_t total_q, int64_t heads) {
+  return (cdiv(total_q, kTileRows) > batch ? cdiv(total_q, kTileRows) : batch) * heads;
+}
+// How many workgroups share a tile's keys: with fewer tiles than the chip holds workgroups their
+// keys are split, down to 512 keys a part (by the mean length: what the sequences hold is known
+// on the device only). 512 rows of 32 heads behind 7000 keys: 160 us whole, 83 us split.
+int most_splits(int64_t batch, int64_t total_q, int64_t heads) {
+  if (batch < 1 || total_q < 1 || heads < 1) return 1;
+  const int64_t s = 512 / whole_groups(batch, total_q, heads);
+  return s < 2 ? 1 : s > kMostSplits ? kMostSplits : (int)s;
+}
+int splits_of(const VarlenArgs& a) {
+  int64_t keys = a.total_k / a.batch;
+  if (a.window > 0 && a.window + a.sinks + kTileRows < keys) keys = a.window + a.sinks + kTileRows;
+  const int most = most_splits(a.batch, a.total_q, a.heads);
+  return keys < 1024 ? 1 : keys / 512 < most ? (int)(keys / 512) : most;
+}
+
+template <int DT, int D, int KEYS>
 int launch_tiles(VarlenArgs a, hipStream_t st) {
-  constexpr int kWaves = 4;
-  a.tiles = (int)(a.total_q / (kWaves * kWaveRows)) + a.batch + 2;
-  hipLaunchKernelGGL((varlen_tile_kernel<DT, D, kWaves>), dim3((unsigned)(a.tiles * a.heads)), dim3(kWaves * kWave), 0, st, a);
-  note_plan("varlen tiles of %d", D);
+  a.tiles = (int)(a.total_q / kTileRows) + a.batch + 2;
+  hipLaunchKernelGGL((varlen_tile_kernel<DT, D, KEYS>), dim3((unsigned)(a.tiles * a.splits * a.heads)), dim3(kTileThreads), 0, st, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((varlen_join_kernel<DT>), dim3((unsigned)cdiv(a.total_q * a.heads, kRowThreads / 32)), dim3(kRowThreads), 0, st, a);
+  note_plan("varlen tiles of %d x %d, %d splits", KEYS, D, a.splits);
   return check_launch("varlen_attention");
+}
+
+// Keys of a tile. At 128 dims 32 keys leave a wave with 164 registers (64: 187), so that three
+// workgroups share a CU: with more than two for each, eight prompts of 350 to 1500 took
+// 109 us, with 64 keys 114; with two, which then pay only for more barriers, 512 rows behind
+// 7000 keys took 87, with 64 keys 83. Four workgroups of 64 dims fit either way (a window of
+// 1024 in 16000 rows: 112 and 109 us). From 192 on two fit with 32 keys and one with 64
+// (4096 rows, 32 heads: 218 and 360 us).
+template <int DT>
+int launch_dims(const VarlenArgs& a, hipStream_t st) {
+  if (a.dim <= 64) return launch_tiles<DT, 64, 64>(a, st);
+  if (a.dim <= 128)
+    return whole_groups(a.batch, a.total_q, a.heads) * a.splits > 512 ? launch_tiles<DT, 128, 32>(a, st) : launch_tiles<DT, 128, 64>(a, st);
+  return a.dim <= 192 ? launch_tiles<DT, 192, 32>(a, st) : launch_tiles<DT, 256, 32>(a, st);
 }
 
 }  // namespace
@@ -388,12 +570,18 @@ int launch_tiles(VarlenArgs a, hipStream_t st) {
 
 using namespace ayk;
 
-extern "C" int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+extern "C" size_t ayk_varlen_attention_split_workspace_bytes(int64_t batch, int64_t total_q, int64_t heads, int64_t dim) {
+  if (dim < 1 || dim > kMaxDim) return 0;
+  const int splits = most_splits(batch, total_q, heads);
+  return splits == 1 ? 0 : (size_t)splits * total_q * heads * (dim + 4) * sizeof(float);
+}
+
+extern "C" int ayk_varlen_attention_split(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
                                     int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
                                     int64_t v_head_stride, int dtype, const int32_t* starts_q, const int32_t* starts_k,
                                     int64_t batch, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
                                     int64_t dim, float scale, int causal, int64_t window, int64_t sinks, void* out,
-                                    ayk_stream_t stream) {
+                                    void* workspace, size_t workspace_bytes, ayk_stream_t stream) {
   const char* op = "varlen_attention";
   if (dtype != AYK_F16 && dtype != AYK_BF16) return fail(AYK_EINVAL, "%s: operands must be float16 or bfloat16", op);
   if (batch < 0 || total_q < 0 || total_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > kMaxDim)
@@ -421,7 +609,7 @@ extern "C" int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t
   };
   if (dim % 8 == 0 && rows16(q, q_row_stride, q_head_stride) && rows16(k, k_row_stride, k_head_stride) &&
       rows16(v, v_row_stride, v_head_stride) && aligned16(out) && batch < 0x1000000 &&
-      (total_q / kWaveRows + batch + 2) * heads < 0x7FFFFFFF) {
+      (total_q / kTileRows + batch + 2) * heads < 0x3FFFFFF) {
     VarlenArgs a{};
     a.q = qp;
     a.k = kp;
@@ -442,11 +630,11 @@ extern "C" int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t
     a.scale_log2 = scale == 0.0f ? 1.0f : fabsf(scale) * kLog2e;
     a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
     a.q_keep = scale == 0.0f ? 0u : 0xFFFFFFFFu;
-    const bool bf = dtype == AYK_BF16;
-    if (dim <= 64) return bf ? launch_tiles<AYK_BF16, 64>(a, st) : launch_tiles<AYK_F16, 64>(a, st);
-    if (dim <= 128) return bf ? launch_tiles<AYK_BF16, 128>(a, st) : launch_tiles<AYK_F16, 128>(a, st);
-    if (dim <= 192) return bf ? launch_tiles<AYK_BF16, 192>(a, st) : launch_tiles<AYK_F16, 192>(a, st);
-    return bf ? launch_tiles<AYK_BF16, 256>(a, st) : launch_tiles<AYK_F16, 256>(a, st);
+    a.partial = static_cast<float*>(workspace);
+    a.splits = workspace != nullptr && aligned16(workspace) &&
+                       workspace_bytes >= ayk_varlen_attention_split_workspace_bytes(batch, total_q, heads, dim)
+                   ? splits_of(a) : 1;
+    return dtype == AYK_BF16 ? launch_dims<AYK_BF16>(a, st) : launch_dims<AYK_F16>(a, st);
   }
   const dim3 grid((unsigned)total_q, (unsigned)heads);
 #define AYK_VAR(Q)                                                                                                     \
@@ -457,4 +645,15 @@ extern "C" int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t
 #undef AYK_VAR
   note_plan("varlen rows");
   return check_launch(op);
+}
+
+extern "C" int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+                                    int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
+                                    int64_t v_head_stride, int dtype, const int32_t* starts_q, const int32_t* starts_k,
+                                    int64_t batch, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
+                                    int64_t dim, float scale, int causal, int64_t window, int64_t sinks, void* out,
+                                    ayk_stream_t stream) {
+  return ayk_varlen_attention_split(q, q_row_stride, q_head_stride, k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride,
+                                    dtype, starts_q, starts_k, batch, total_q, total_k, heads, kv_heads, dim, scale, causal, window,
+                                    sinks, out, nullptr, 0, stream);
 }

@@ -337,6 +337,16 @@ int ayk_varlen_attention(const void* q, int64_t q_row_stride, int64_t q_head_str
                          int64_t batch, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
                          int64_t dim, float scale, int causal, int64_t window, int64_t sinks, void* out,
                          ayk_stream_t stream);
+/* The same with a workspace, in which the keys of few rows (a chunk behind a long prompt) are
+ * split over the chip and joined; sequences of less than 1024 keys on average are not. One
+ * smaller than the query's answer, or none, leaves them whole. */
+int ayk_varlen_attention_split(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+                               int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
+                               int64_t v_head_stride, int dtype, const int32_t* starts_q, const int32_t* starts_k,
+                               int64_t batch, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
+                               int64_t dim, float scale, int causal, int64_t window, int64_t sinks, void* out,
+                               void* workspace, size_t workspace_bytes, ayk_stream_t stream);
+size_t ayk_varlen_attention_split_workspace_bytes(int64_t batch, int64_t total_q, int64_t heads, int64_t dim);
 
 #ifdef __cplusplus
 }
