@@ -15,7 +15,15 @@ import torch
 
 from ayaka.kernel.hip import _lib
 from ayaka.kernel.hip._host import prepare_output, require_cuda, require_dtype, require_same_device
-from ayaka.kernel.hip.attention._checks import ATTENTION_DTYPES, check_heads, check_scale, check_window, rows_of_heads
+from ayaka.kernel.hip.attention._checks import (
+    ATTENTION_DTYPES,
+    check_heads,
+    check_scale,
+    check_window,
+    new_output,
+    on_device_of,
+    rows_of_heads,
+)
 from ayaka.kernel.ops import custom_op
 
 __all__ = ["paged_decode_attention"]
@@ -29,26 +37,30 @@ def _paged_decode_attention_fake(query, key_cache, value_cache, block_tables, se
 
 
 def _check(query, key_cache, value_cache, block_tables, seq_lens) -> None:
-    for t, name in ((query, "query"), (key_cache, "key_cache"), (value_cache, "value_cache"),
-                    (block_tables, "block_tables"), (seq_lens, "seq_lens")):
-        require_cuda(t, name)
-        require_same_device(t, name, query, "query")
+    if not on_device_of(query, key_cache, value_cache, block_tables, seq_lens):
+        for t, name in ((query, "query"), (key_cache, "key_cache"), (value_cache, "value_cache"),
+                        (block_tables, "block_tables"), (seq_lens, "seq_lens")):
+            require_cuda(t, name)
+            require_same_device(t, name, query, "query")
     require_dtype(query, "query", ATTENTION_DTYPES)
     require_dtype(key_cache, "key_cache", (*_FP8_DTYPES, query.dtype))
-    if query.ndim != 3:
+    shape, cache = query.shape, key_cache.shape
+    if len(shape) != 3:
         raise ValueError("query must be [batch, heads, head_dim]")
-    if key_cache.ndim != 4 or key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
+    if len(cache) != 4 or cache != value_cache.shape or key_cache.dtype != value_cache.dtype:
         raise ValueError("key_cache and value_cache must be [pages, page_size, kv_heads, head_dim] of one shape and dtype")
     if not key_cache.is_contiguous() or not value_cache.is_contiguous():
         raise ValueError("KV cache pages must be contiguous")
-    if key_cache.shape[1] < 1 or key_cache.shape[3] != query.shape[2]:
-        raise ValueError(f"cache {tuple(key_cache.shape)} does not match a query of head_dim {query.shape[2]}")
-    check_heads(query.shape[1], key_cache.shape[2], query.shape[2])
+    batch, heads, dim = shape
+    if cache[1] < 1 or cache[3] != dim:
+        raise ValueError(f"cache {tuple(cache)} does not match a query of head_dim {dim}")
+    check_heads(heads, cache[2], dim)
     require_dtype(block_tables, "block_tables", (torch.int32,))
     require_dtype(seq_lens, "seq_lens", (torch.int32,))
-    if block_tables.ndim != 2 or block_tables.shape[0] != query.shape[0] or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    table = block_tables.shape
+    if len(table) != 2 or table[0] != batch or (table[1] > 1 and block_tables.stride(1) != 1):
         raise ValueError("block_tables must be [batch, pages] with stride(1) == 1")
-    if seq_lens.ndim != 1 or seq_lens.shape[0] != query.shape[0] or not seq_lens.is_contiguous():
+    if seq_lens.shape != (batch,) or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous [batch] vector")
 
 
@@ -91,7 +103,7 @@ def paged_decode_attention(
     check_scale(softmax_scale)
     if not (math.isfinite(k_scale) and k_scale > 0 and math.isfinite(v_scale) and v_scale > 0):
         raise ValueError("KV scales must be finite and positive")
-    result = prepare_output(query, out, like_name="query")
+    result = new_output(query) if out is None else prepare_output(query, out, like_name="query")
     if not result.is_contiguous():
         raise ValueError("out must be contiguous")
     batch, heads, dim = query.shape

@@ -13,7 +13,15 @@ import torch
 
 from ayaka.kernel.hip import _lib
 from ayaka.kernel.hip._host import prepare_output, require_cuda, require_dtype, require_same_device
-from ayaka.kernel.hip.attention._checks import ATTENTION_DTYPES, check_heads, check_scale, check_window, rows_of_heads
+from ayaka.kernel.hip.attention._checks import (
+    ATTENTION_DTYPES,
+    check_heads,
+    check_scale,
+    check_window,
+    new_output,
+    on_device_of,
+    rows_of_heads,
+)
 from ayaka.kernel.ops import custom_op
 
 __all__ = ["varlen_attention"]
@@ -25,18 +33,20 @@ def _varlen_attention_fake(query, key, value, cu_seqlens_q, cu_seqlens_k, softma
 
 
 def _check(query, key, value, cu_seqlens_q, cu_seqlens_k) -> None:
-    for t, name in ((query, "query"), (key, "key"), (value, "value"), (cu_seqlens_q, "cu_seqlens_q"),
-                    (cu_seqlens_k, "cu_seqlens_k")):
-        require_cuda(t, name)
-        require_same_device(t, name, query, "query")
+    if not on_device_of(query, key, value, cu_seqlens_q, cu_seqlens_k):
+        for t, name in ((query, "query"), (key, "key"), (value, "value"), (cu_seqlens_q, "cu_seqlens_q"),
+                        (cu_seqlens_k, "cu_seqlens_k")):
+            require_cuda(t, name)
+            require_same_device(t, name, query, "query")
     require_dtype(query, "query", ATTENTION_DTYPES)
     require_dtype(key, "key", (query.dtype,))
     require_dtype(value, "value", (query.dtype,))
-    if query.ndim != 3:
+    shape, keys = query.shape, key.shape
+    if len(shape) != 3:
         raise ValueError("query must be [tokens, heads, head_dim]")
-    if key.ndim != 3 or key.shape != value.shape or key.shape[2] != query.shape[2]:
+    if len(keys) != 3 or keys != value.shape or keys[2] != shape[2]:
         raise ValueError("key and value must be [tokens, kv_heads, head_dim] of one shape, with the query's head_dim")
-    check_heads(query.shape[1], key.shape[1], query.shape[2])
+    check_heads(shape[1], keys[1], shape[2])
     for t, name in ((cu_seqlens_q, "cu_seqlens_q"), (cu_seqlens_k, "cu_seqlens_k")):
         require_dtype(t, name, (torch.int32,))
         if t.ndim != 1 or t.shape[0] < 1 or not t.is_contiguous():
@@ -82,7 +92,7 @@ def varlen_attention(
     check_scale(softmax_scale)
     if window and not causal:
         raise ValueError("a window needs causal attention")
-    result = prepare_output(query, out, like_name="query")
+    result = new_output(query) if out is None else prepare_output(query, out, like_name="query")
     if not result.is_contiguous():
         raise ValueError("out must be contiguous")
     tokens, heads, dim = query.shape

@@ -28,11 +28,10 @@ _SCALE_DTYPES = {"float32": torch.float32, "e8m0": torch.uint8}
 
 
 def _outputs(x, group_size, scale_dtype, scale_col_major):
-    k = int(x.shape[-1])
-    rows = math.prod(x.shape[:-1]) if x.ndim > 1 else 1
+    *lead, k = x.shape
+    rows = math.prod(lead)
     shape = (rows,) if group_size == 0 else (k // group_size, rows) if scale_col_major else (rows, k // group_size)
-    return (torch.empty((rows, k), dtype=FP8, device=x.device),
-            torch.empty(shape, dtype=_SCALE_DTYPES[scale_dtype], device=x.device))
+    return x.new_empty((rows, k), dtype=FP8), x.new_empty(shape, dtype=_SCALE_DTYPES[scale_dtype])
 
 
 def _rms_norm_quant_fake(x, weight, eps, group_size=0, scale_dtype="float32", scale_col_major=False):
@@ -69,7 +68,7 @@ def _check(x, weight, eps, group_size, scale_dtype, scale_col_major) -> None:
 def _launch(x, residual, weight, eps, group_size, scale_dtype, scale_col_major):
     q, scale = _outputs(x, group_size, scale_dtype, scale_col_major)
     rows, k = q.shape
-    residual_out = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    residual_out = None if residual is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     if rows:
         x2d = _rows_2d(x)
         r2d = None if residual is None else _rows_2d(residual)
