@@ -86,6 +86,21 @@ __device__ inline float sum_quads(float x) {
   return sum_halves(u2f(r[0]) + u2f(r[1]));
 }
 
+// Sum over the wave, for every lane, and the sum up to each lane, of integers (DPP moves:
+// within rows of 16, then across them).
+template <int CTRL, int ROWS>
+__device__ inline int dpp_int(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ inline int wave_scan(int v) {
+  v += dpp_int<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_int<0x112, 0xF>(v);
+  v += dpp_int<0x114, 0xF>(v);
+  v += dpp_int<0x118, 0xF>(v);
+  v += dpp_int<0x142, 0xA>(v);  // the end of rows 0 and 2 to rows 1 and 3, then of row 1 to 2 and 3
+  v += dpp_int<0x143, 0xC>(v);
+  return v;
+}
+__device__ inline int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1); }
+
 constexpr float kLog2e = 1.44269504088896340736f;
 
 }  // namespace

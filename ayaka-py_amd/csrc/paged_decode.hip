@@ -448,9 +448,7 @@ __device__ inline int total_steps(const DecodeArgs& a) {
   const int lane = threadIdx.x % kWave;
   int sum = 0;
   for (int b = lane; b < a.batch; b += kWave) sum += steps_of(a.lens, b, a.c, a.window, a.sinks);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-  return sum * a.tiles * a.kv_items;
+  return wave_total(sum) * a.tiles * a.kv_items;
 }
 
 // Long sequences: the steps of all items are dealt out evenly, a run of `share` consecutive
@@ -469,12 +467,7 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
   int before = 0;  // steps of the sequences before chunk
   for (int chunk = 0; chunk < a.batch && at < end; chunk += kWave) {
     const int mine = chunk + lane < a.batch ? steps_of(a.lens, chunk + lane, a.c, a.window, a.sinks) : 0;
-    int upto = mine;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int v = __shfl_up(upto, off, kWave);
-      if (lane >= off) upto += v;
-    }
+    const int upto = wave_scan(mine);
     while (at < end) {
       // the first sequence whose items end past `at`
       const uint64_t past = __ballot(before + upto * per > at);
@@ -499,15 +492,14 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
 }
 
 // Joins the partial results of one (sequence, head) and writes the zeros of empty sequences:
-// one wave a head, or four that take the partial results in turn (HEADS = 4 or 1), lane l the
-// dims l, l + 64, ..., summed in order. One long sequence alone has hundreds of partial
-// results: one after the other they took 63 us of 121, by four waves 8 us. Where heads and
-// sequences are many, one wave a head is what the chip holds: 96 sequences of 64 heads took
-// 14 us with four.
-template <int QT, int D, int PACK, int HEADS>
-__global__ __launch_bounds__(kDecodeThreads) void paged_decode_join_kernel(DecodeArgs a, int runs) {
-  constexpr int kPer = (D + kWave - 1) / kWave, kShare = 4 / HEADS;  // waves a head
-  __shared__ float part[4][D + 1];
+// one wave a head, or several that take the partial results in turn, lane l the dims l, l + 64,
+// ..., summed in order. One long sequence alone has hundreds of partial results: one after
+// the other they took 63 us of 121, by four waves 8 us. Where heads and sequences are many,
+// one wave a head is what the chip holds: 96 sequences of 64 heads took 14 us with four.
+template <int QT, int D, int PACK, int HEADS, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(DecodeArgs a, int runs) {
+  constexpr int kPer = (D + kWave - 1) / kWave, kShare = WAVES / HEADS;  // waves a head
+  __shared__ float part[WAVES][D + 1];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, per = a.tiles * a.kv_items;
   const int b = blockIdx.x, h = blockIdx.y * HEADS + wave / kShare;
   if (h >= a.heads) return;  // whole waves, and no barrier with HEADS > 1
@@ -520,11 +512,8 @@ __global__ __launch_bounds__(kDecodeThreads) void paged_decode_join_kernel(Decod
     early += s < b ? n : 0;
   }
   const int steps = steps_of(a.lens, b, a.c, a.window, a.sinks);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    sum += __shfl_xor(sum, off, kWave);
-    early += __shfl_xor(early, off, kWave);
-  }
+  sum = wave_total(sum);
+  early = wave_total(early);
   const int share = (sum * per + runs - 1) / runs;
   uint16_t* o = a.out + ((int64_t)b * a.heads + h) * D;
   if (steps == 0) {
@@ -560,11 +549,12 @@ __global__ __launch_bounds__(kDecodeThreads) void paged_decode_join_kernel(Decod
     if (lane == 0) part[wave][D] = l;
     __syncthreads();
     if (wave != 0) return;
-    l = part[0][D] + part[1][D] + part[2][D] + part[3][D];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + i * kWave;
-      if (d < D) acc[i] = part[0][d] + part[1][d] + part[2][d] + part[3][d];
+    for (int v = 1; v < WAVES; ++v) {
+      l += part[v][D];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (lane + i * kWave < D) acc[i] += part[v][lane + i * kWave];
     }
   }
 #pragma unroll
@@ -586,12 +576,16 @@ int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
   } else {
     constexpr int runs = 256 * Shape<CT, D>::kWavesPerSimd;
     hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
-    if ((int64_t)a.batch * a.heads < 1024)
-      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 1>), dim3((unsigned)a.batch, (unsigned)a.heads),
-                         dim3(kDecodeThreads), 0, st, a, runs);
+    const int64_t rows = (int64_t)a.batch * a.heads;
+    if (rows <= 256)
+      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 1, 16>), dim3((unsigned)a.batch, (unsigned)a.heads),
+                         dim3(16 * kWave), 0, st, a, runs);
+    else if (rows < 1024)
+      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 1, 4>), dim3((unsigned)a.batch, (unsigned)a.heads),
+                         dim3(4 * kWave), 0, st, a, runs);
     else
-      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 4>), dim3((unsigned)a.batch, (unsigned)cdiv(a.heads, 4)),
-                         dim3(kDecodeThreads), 0, st, a, runs);
+      hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 4, 4>), dim3((unsigned)a.batch, (unsigned)cdiv(a.heads, 4)),
+                         dim3(4 * kWave), 0, st, a, runs);
     note_plan("paged_decode split");
   }
   return check_launch("paged_decode_attention");
