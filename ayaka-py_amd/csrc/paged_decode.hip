@@ -61,38 +61,44 @@ constexpr int kStep = 4 * kBlock;       // positions a workgroup takes at a time
 constexpr int kDecodeThreads = 256;
 constexpr int kHeadTile = 16;
 
-// The blocks of 32 positions that hold a sequence's visible ones: those of the first tokens,
-// then those from the window's first position to the end.
-struct Blocks {
-  int first_blocks, jump, count;  // block i lies at positions 32 (i < first_blocks ? i : i + jump)
-};
-__device__ inline Blocks blocks_of(const Visible& v) {
-  Blocks b;
-  const int end = (int)((v.end + kBlock - 1) / kBlock), from = (int)(v.first / kBlock);
-  const int64_t kept = v.sinks < v.first ? v.sinks : v.first;
-  b.first_blocks = (int)((kept + kBlock - 1) / kBlock);
-  const int second = from > b.first_blocks ? from : b.first_blocks;
-  b.jump = second - b.first_blocks;
-  b.count = b.first_blocks + (end > second ? end - second : 0);
-  return b;
-}
-__device__ inline int steps_of(const int32_t* lens, int64_t b, const PagedCache& c, int64_t window, int64_t sinks) {
-  const int64_t n = cached_length(lens, b, c);
-  return (blocks_of(visible_to(n - 1, n, true, window, sinks)).count + 3) / 4;
-}
-
 struct DecodeArgs {
   const uint16_t* q;
   int64_t q_row, q_head;
-  PagedCache c;
+  const uint8_t *k, *v;
+  const int32_t* table;
+  int64_t table_stride;
   const int32_t* lens;
-  int batch, heads, kv_items, group, tiles, rows;  // kv heads or pairs, tiles of 16 heads in a group, columns in use
-  float scale_log2, v_scale;
-  int64_t window, sinks;
   uint16_t* out;
   float* partial;  // split launches: two partial results a workgroup
-  int q_aligned, page_shift;  // page_shift: log2 of the page size, or -1
+  // positions, pages and slots are counted in 32 bits (the host checks that they fit)
+  int num_pages, page_size, page_shift;  // page_shift: log2 of the page size, or -1
+  uint32_t row_bytes;
+  int longest, window, sinks;                       // longest: what a row of the table can name
+  int batch, heads, kv_items, group, tiles, rows;  // kv heads or pairs, tiles of 16 heads in a group, columns in use
+  int q_aligned;
+  float scale_log2, v_scale;
 };
+
+// The visible positions of a sequence, and the blocks of 32 that hold them: those of the first
+// tokens, then those from the window's first position to the end.
+struct Blocks {
+  int end, first, kept;           // visible: j < end and (j >= first or j < kept)
+  int first_blocks, jump, count;  // block i lies at positions 32 (i < first_blocks ? i : i + jump)
+};
+__device__ inline Blocks blocks_of(const DecodeArgs& a, int b) {
+  Blocks s;
+  const int n = a.lens[b];
+  s.end = n < 0 ? 0 : n < a.longest ? n : a.longest;
+  s.first = a.window > 0 && s.end > a.window ? s.end - a.window : 0;
+  s.kept = a.sinks < s.first ? a.sinks : s.first;
+  const int last = (s.end + kBlock - 1) / kBlock, from = s.first / kBlock;
+  s.first_blocks = (s.kept + kBlock - 1) / kBlock;
+  const int second = from > s.first_blocks ? from : s.first_blocks;
+  s.jump = second - s.first_blocks;
+  s.count = s.first_blocks + (last > second ? last - second : 0);
+  return s;
+}
+__device__ inline int steps_of(const DecodeArgs& a, int b) { return (blocks_of(a, b).count + 3) / 4; }
 
 // What a wave holds of an item.
 template <int CT, int D>
@@ -103,7 +109,10 @@ struct Shape {
   static constexpr int kSteps = D / 32;             // 32-dim steps of the score product
   static constexpr int kCols = D / 16;              // dims of a V row in each of its sixteen lanes
   static constexpr int kVWords = (kCols * kElem + 3) / 4;
-  static constexpr int kWavesPerSimd = D * kElem <= 64 ? 4 : D * kElem <= 128 ? 3 : D * kElem <= 256 ? 2 : 1;  // what its registers leave room for
+  // What leaves the registers of a split launch unspilled: 128 e4m3 dims with three waves
+  // spill two and read one long sequence in 68 us, with two waves in 63; 256 with two waves
+  // spill 26 (142 us against 112 with one).
+  static constexpr int kWavesPerSimd = D * kElem <= 64 ? 4 : (kFp8 ? D < 256 : D <= 128) ? 2 : 1;
 };
 
 // First dim of lane quad `quad`'s eight k slots at step s of the score product.
@@ -209,9 +218,7 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
   using S = Shape<CT, D>;
   constexpr int PT = S::kFp8 ? AYK_F16 : QT;  // e4m3 and e5m2 are exact in fp16, whose weights round finer
   const int lane = item_lane(), wave = threadIdx.x / kWave, col = lane % 16, quad = lane / 16;
-  const int64_t n = cached_length(a.lens, b, a.c);
-  const Visible vis = visible_to(n - 1, n, true, a.window, a.sinks);
-  const Blocks bl = blocks_of(vis);
+  const Blocks bl = blocks_of(a, b);
   r.m = -INFINITY;
   r.l = 0.0f;
 #pragma unroll
@@ -240,20 +247,19 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
     }
   }
 
-  const int32_t* table = a.c.table + b * a.c.table_stride;
+  const int32_t* table = a.table + b * a.table_stride;
   const int64_t head_at = (int64_t)g * D * S::kElem;
-  const uint32_t page_size = (uint32_t)a.c.page_size, row_bytes = (uint32_t)a.c.row_bytes;
-  const int seen_end = (int)vis.end, seen_first = (int)vis.first, kept = (int)(vis.sinks < vis.first ? vis.sinks : vis.first);
+  const uint32_t page_size = (uint32_t)a.page_size;
   auto page_index = [&](uint32_t j) { return a.page_shift >= 0 ? j >> a.page_shift : j / page_size; };
   // Lane l looks up position l % 32 of a block: its page, a block ahead of the rows.
   auto position = [&](int blk) { return kBlock * (blk < bl.first_blocks ? blk : blk + bl.jump) + lane % kBlock; };
   auto page_of = [&](int blk) {
     const int j = position(blk);
-    return j < seen_end ? table[page_index(j)] : -1;
+    return j < bl.end ? table[page_index(j)] : -1;
   };
   auto slot_of = [&](int blk, int page) {  // -1: hidden
     const int j = position(blk);
-    const bool on = j < seen_end && (j >= seen_first || j < kept) && (uint32_t)page < (uint32_t)a.c.num_pages;
+    const bool on = j < bl.end && (j >= bl.first || j < bl.kept) && (uint32_t)page < (uint32_t)a.num_pages;
     return on ? (int)((uint32_t)page * page_size + j - page_index(j) * page_size) : -1;
   };
   uint32_t kw[2][S::kKWords], vw[8][S::kVWords];
@@ -261,14 +267,14 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int at = __builtin_amdgcn_ds_bpermute(4 * col + 64 * t, slot);
-      load_k_row<CT, D>(a.c.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * row_bytes + head_at, quad, kw[t]);
+      load_k_row<CT, D>(a.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, quad, kw[t]);
     }
   };
   auto issue_v = [&](int slot) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int at = __builtin_amdgcn_ds_bpermute(16 * quad + 64 * (j / 4) + 4 * (j % 4), slot);
-      load_v_row<CT, D>(a.c.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * row_bytes + head_at, col, vw[j]);
+      load_v_row<CT, D>(a.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, col, vw[j]);
     }
   };
   // The next block's K is asked for as soon as this block's is used up, and V likewise, so
@@ -447,7 +453,7 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
 __device__ inline int total_steps(const DecodeArgs& a) {
   const int lane = threadIdx.x % kWave;
   int sum = 0;
-  for (int b = lane; b < a.batch; b += kWave) sum += steps_of(a.lens, b, a.c, a.window, a.sinks);
+  for (int b = lane; b < a.batch; b += kWave) sum += steps_of(a, b);
   return wave_total(sum) * a.tiles * a.kv_items;
 }
 
@@ -466,7 +472,7 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
   const int end = at + share < total ? at + share : total;
   int before = 0;  // steps of the sequences before chunk
   for (int chunk = 0; chunk < a.batch && at < end; chunk += kWave) {
-    const int mine = chunk + lane < a.batch ? steps_of(a.lens, chunk + lane, a.c, a.window, a.sinks) : 0;
+    const int mine = chunk + lane < a.batch ? steps_of(a, chunk + lane) : 0;
     const int upto = wave_scan(mine);
     while (at < end) {
       // the first sequence whose items end past `at`
@@ -507,11 +513,11 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(Decode
   const int col = kv % PACK * (kHeadTile / PACK) + h % a.group % kHeadTile;
   int sum = 0, early = 0;  // steps of all sequences, and of those before b
   for (int s = lane; s < a.batch; s += kWave) {
-    const int n = steps_of(a.lens, s, a.c, a.window, a.sinks);
+    const int n = steps_of(a, s);
     sum += n;
     early += s < b ? n : 0;
   }
-  const int steps = steps_of(a.lens, b, a.c, a.window, a.sinks);
+  const int steps = steps_of(a, b);
   sum = wave_total(sum);
   early = wave_total(early);
   const int share = (sum * per + runs - 1) / runs;
@@ -650,12 +656,20 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
   const int pack = dim == 64 && group <= kHeadTile / 2 && kv_heads % 2 == 0 ? 2 : 1;
   const int64_t items = batch * tiles * (kv_heads / pack);
   if (matrix_dim(dim) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
-      num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && items < 0x7FFFFFFF) {
+      num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && c.row_bytes < 0x7FFFFFFF &&
+      items < 0x7FFFFFFF) {
     DecodeArgs a{};
     a.q = static_cast<const uint16_t*>(q);
     a.q_row = q_row_stride;
     a.q_head = q_head_stride;
-    a.c = c;
+    a.k = c.k;
+    a.v = c.v;
+    a.table = block_tables;
+    a.table_stride = table_stride;
+    a.num_pages = (int)num_pages;
+    a.page_size = (int)page_size;
+    a.row_bytes = (uint32_t)c.row_bytes;
+    a.longest = (int)most;
     a.lens = seq_lens;
     a.batch = (int)batch;
     a.heads = (int)heads;
@@ -666,8 +680,8 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctzll((uint64_t)page_size);
     a.scale_log2 = scale * k_scale * kLog2e;
     a.v_scale = v_scale;
-    a.window = window;
-    a.sinks = sinks;
+    a.window = (int)(window < 0x7FFFFFFF ? window : 0x7FFFFFFF);
+    a.sinks = (int)(sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF);
     a.out = static_cast<uint16_t*>(out);
     a.partial = static_cast<float*>(workspace);
     a.q_aligned = aligned16(q) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0;
