@@ -75,7 +75,7 @@ struct DecodeArgs {
   uint32_t row_bytes;
   int longest, window, sinks;                       // longest: what a row of the table can name
   int batch, heads, kv_items, group, tiles, rows;  // kv heads or pairs, tiles of 16 heads in a group, columns in use
-  int q_aligned;
+  int q_aligned, dim;
   float scale_log2, v_scale;
 };
 
@@ -121,15 +121,25 @@ __device__ inline int k_dim(int s, int quad) {
   if constexpr (Shape<CT, D>::kFp8) return s < 2 * (D / 64) ? 64 * (s / 2) + 16 * quad + 8 * (s % 2) : 64 * (D / 64) + 8 * quad;
   else return 32 * s + 8 * quad;
 }
-template <int CT, int D>
-__device__ inline void load_k_row(const uint8_t* row, int quad, uint32_t* w) {
+// 16 or 8 bytes, or zeros for dims past the head's.
+template <typename T>
+__device__ inline T load_or_zero(const uint8_t* p, bool on) {
+  T v{};
+  if (on) v = *reinterpret_cast<const T*>(p);
+  return v;
+}
+template <int CT, int D, bool EXACT>
+__device__ inline void load_k_row(const uint8_t* row, int quad, int dim, uint32_t* w) {
   if constexpr (Shape<CT, D>::kFp8) {
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) *reinterpret_cast<v4u*>(w + 4 * j) = *reinterpret_cast<const v4u*>(row + 64 * j + 16 * quad);
-    if constexpr (D % 64) *reinterpret_cast<uint2*>(w + 4 * (D / 64)) = *reinterpret_cast<const uint2*>(row + 64 * (D / 64) + 8 * quad);
+    for (int j = 0; j < D / 64; ++j)
+      *reinterpret_cast<v4u*>(w + 4 * j) = load_or_zero<v4u>(row + 64 * j + 16 * quad, EXACT || 64 * j + 16 * quad < dim);
+    if constexpr (D % 64)
+      *reinterpret_cast<uint2*>(w + 4 * (D / 64)) = load_or_zero<uint2>(row + 64 * (D / 64) + 8 * quad, EXACT || 64 * (D / 64) + 8 * quad < dim);
   } else {
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) *reinterpret_cast<v4u*>(w + 4 * s) = *reinterpret_cast<const v4u*>(row + 64 * s + 16 * quad);
+    for (int s = 0; s < D / 32; ++s)
+      *reinterpret_cast<v4u*>(w + 4 * s) = load_or_zero<v4u>(row + 64 * s + 16 * quad, EXACT || 32 * s + 8 * quad < dim);
   }
 }
 template <int CT, int QT, int D>
@@ -168,17 +178,18 @@ struct DimOrder {  // dim of column c: base[t] + c width[t]
     }
   }
 };
-template <int CT, int D, int AT = 0>
-__device__ inline void load_v_row(const uint8_t* row, int col, uint32_t* w) {
+template <int CT, int D, bool EXACT, int AT = 0>
+__device__ inline void load_v_row(const uint8_t* row, int col, int dim, uint32_t* w) {
   if constexpr (AT < D / 16) {
     constexpr int e = Shape<CT, D>::kElem, size = v_piece<CT, D>(AT), bytes = size * e;
     const uint8_t* p = row + (16 * AT + col * size) * e;
+    const bool on = EXACT || 16 * AT + col * size < dim;
     uint32_t* d = w + AT * e / 4;
-    if constexpr (bytes == 16) *reinterpret_cast<v4u*>(d) = *reinterpret_cast<const v4u*>(p);
-    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(p);
-    else if constexpr (bytes == 4) *d = *reinterpret_cast<const uint32_t*>(p);
-    else *d = *reinterpret_cast<const uint16_t*>(p);
-    load_v_row<CT, D, AT + size>(row, col, w);
+    if constexpr (bytes == 16) *reinterpret_cast<v4u*>(d) = load_or_zero<v4u>(p, on);
+    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(d) = load_or_zero<uint2>(p, on);
+    else if constexpr (bytes == 4) *d = load_or_zero<uint32_t>(p, on);
+    else *d = load_or_zero<uint16_t>(p, on);
+    load_v_row<CT, D, EXACT, AT + size>(row, col, dim, w);
   }
 }
 
@@ -213,7 +224,7 @@ struct Column {
   __device__ int head(const DecodeArgs& a, int g, int tile) const { return (g * PACK + sub) * a.group + tile * kHeadTile + at; }
 };
 
-template <int QT, int CT, int D, int PACK>
+template <int QT, int CT, int D, int PACK, bool EXACT>
 __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile, int from, int to, Running<D>& r) {
   using S = Shape<CT, D>;
   constexpr int PT = S::kFp8 ? AYK_F16 : QT;  // e4m3 and e5m2 are exact in fp16, whose weights round finer
@@ -236,7 +247,7 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
   for (int s = 0; s < S::kSteps; ++s) {
     qf[s] = v4u{0, 0, 0, 0};
     const int dim = k_dim<CT, D>(s, quad);
-    if (has_head && dim / (D / PACK) == column.sub) {
+    if (has_head && dim / (D / PACK) == column.sub && (EXACT || dim < a.dim)) {
       const uint16_t* p = a.q + b * a.q_row + head * a.q_head + dim % (D / PACK);
       if (a.q_aligned) {
         qf[s] = *reinterpret_cast<const v4u*>(p);
@@ -248,7 +259,7 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
   }
 
   const int32_t* table = a.table + b * a.table_stride;
-  const int64_t head_at = (int64_t)g * D * S::kElem;
+  const int64_t head_at = (int64_t)g * (EXACT ? D : a.dim) * S::kElem;
   const uint32_t page_size = (uint32_t)a.page_size;
   auto page_index = [&](uint32_t j) { return a.page_shift >= 0 ? j >> a.page_shift : j / page_size; };
   // Lane l looks up position l % 32 of a block: its page, a block ahead of the rows.
@@ -267,14 +278,14 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int at = __builtin_amdgcn_ds_bpermute(4 * col + 64 * t, slot);
-      load_k_row<CT, D>(a.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, quad, kw[t]);
+      load_k_row<CT, D, EXACT>(a.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, quad, a.dim, kw[t]);
     }
   };
   auto issue_v = [&](int slot) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int at = __builtin_amdgcn_ds_bpermute(16 * quad + 64 * (j / 4) + 4 * (j % 4), slot);
-      load_v_row<CT, D>(a.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, col, vw[j]);
+      load_v_row<CT, D, EXACT>(a.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, col, a.dim, vw[j]);
     }
   };
   // The next block's K is asked for as soon as this block's is used up, and V likewise, so
@@ -401,7 +412,7 @@ __device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave])
 
 // Wave 0 writes an item: rounded to the output, or as a partial result
 // (a row of D sums, the maximum and the sum for every head).
-template <int QT, int CT, int D, int PACK>
+template <int QT, int CT, int D, int PACK, bool EXACT>
 __device__ inline void write_item(const DecodeArgs& a, int b, int g, int tile, const Running<D>& r, float* partial) {
   const int lane = item_lane(), col = lane % 16, quad = lane / 16;
   const float l = sum_quads(r.l);
@@ -424,28 +435,28 @@ __device__ inline void write_item(const DecodeArgs& a, int b, int g, int tile, c
     }
     return;
   }
-  uint16_t* o = a.out + ((int64_t)b * a.heads + column.head(a, g, tile)) * HD;
+  uint16_t* o = a.out + ((int64_t)b * a.heads + column.head(a, g, tile)) * (EXACT ? HD : a.dim);
   const float f = l == 0.0f ? 0.0f : a.v_scale / l;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int t = 0; t < D / 16; t += 2) {
       const int dim = order.base[t] + (4 * quad + i) * order.width[t];
-      if (PACK == 1 || dim / HD == column.sub)
+      if ((PACK == 1 || dim / HD == column.sub) && (EXACT || dim < a.dim))
         *reinterpret_cast<uint32_t*>(o + dim % HD) = pack2<QT>(r.acc[t][i] * f, r.acc[t + 1][i] * f);
     }
 }
 
 // One workgroup per sequence, kv head and head tile: for calls whose longest possible
 // sequence is a few steps.
-template <int QT, int CT, int D, int PACK>
+template <int QT, int CT, int D, int PACK, bool EXACT>
 __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_kernel(DecodeArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_blocks<QT, CT, D, PACK>(a, b, g, tile, 0, 0x1FFFFFF, r);
+  attend_blocks<QT, CT, D, PACK, EXACT>(a, b, g, tile, 0, 0x1FFFFFF, r);
   join_waves<D>(r, lds);
-  if (threadIdx.x < kWave) write_item<QT, CT, D, PACK>(a, b, g, tile, r, nullptr);
+  if (threadIdx.x < kWave) write_item<QT, CT, D, PACK, EXACT>(a, b, g, tile, r, nullptr);
 }
 
 // The list of every item's steps, sequence by sequence, each with its (tile, kv head) items:
@@ -461,7 +472,7 @@ __device__ inline int total_steps(const DecodeArgs& a) {
 // ones to every workgroup, whatever the lengths. A run may end one item, hold some whole and
 // begin another; what it does not hold whole it leaves as a partial result, in slot 0 (the run
 // begins inside the item) or slot 1 (it ends inside).
-template <int QT, int CT, int D, int PACK>
+template <int QT, int CT, int D, int PACK, bool EXACT>
 __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_split_kernel(DecodeArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
   const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
@@ -485,12 +496,12 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
       const int last = first + (end - at) < steps ? first + (end - at) : steps;
       Running<D> r;
       const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
-      attend_blocks<QT, CT, D, PACK>(a, b, g, tile, first, last, r);
+      attend_blocks<QT, CT, D, PACK, EXACT>(a, b, g, tile, first, last, r);
       join_waves<D>(r, lds);
       float* partial = nullptr;
       if (first > 0 || last < steps)
         partial = a.partial + ((int64_t)run * 2 + (first > 0 ? 0 : 1)) * a.rows * (D / PACK + 2);
-      if (threadIdx.x < kWave) write_item<QT, CT, D, PACK>(a, b, g, tile, r, partial);
+      if (threadIdx.x < kWave) write_item<QT, CT, D, PACK, EXACT>(a, b, g, tile, r, partial);
       at += last - first;
     }
     before += __builtin_amdgcn_readlane(upto, kWave - 1) * per;
@@ -521,11 +532,11 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(Decode
   sum = wave_total(sum);
   early = wave_total(early);
   const int share = (sum * per + runs - 1) / runs;
-  uint16_t* o = a.out + ((int64_t)b * a.heads + h) * D;
+  uint16_t* o = a.out + ((int64_t)b * a.heads + h) * a.dim;
   if (steps == 0) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (lane + i * kWave < D && wave % kShare == 0) o[lane + i * kWave] = 0;
+      if (lane + i * kWave < a.dim && wave % kShare == 0) o[lane + i * kWave] = 0;
     return;
   }
   const int start = early * per + (tile * a.kv_items + kv / PACK) * steps;
@@ -565,7 +576,7 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(Decode
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
-    if (lane + i * kWave < D) store_f32(o, QT, lane + i * kWave, l == 0.0f ? 0.0f : acc[i] * a.v_scale / l);
+    if (lane + i * kWave < a.dim) store_f32(o, QT, lane + i * kWave, l == 0.0f ? 0.0f : acc[i] * a.v_scale / l);
 }
 
 bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AYK_E4M3 || dt == AYK_E5M2; }
@@ -573,15 +584,15 @@ bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AY
 
 constexpr int kMostRuns = 1024;  // workgroups of a split launch that the chip holds at once, at most
 
-template <int QT, int CT, int D, int PACK = 1>
+template <int QT, int CT, int D, bool EXACT, int PACK = 1>
 int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
   if (!split) {
-    hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, PACK>), dim3((unsigned)(a.batch * a.tiles * a.kv_items)),
+    hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, PACK, EXACT>), dim3((unsigned)(a.batch * a.tiles * a.kv_items)),
                        dim3(kDecodeThreads), 0, st, a);
     note_plan("paged_decode whole");
   } else {
     constexpr int runs = 256 * Shape<CT, D>::kWavesPerSimd;
-    hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK, EXACT>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
     const int64_t rows = (int64_t)a.batch * a.heads;
     if (rows <= 256)
       hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 1, 16>), dim3((unsigned)a.batch, (unsigned)a.heads),
@@ -599,15 +610,19 @@ int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
 
 template <int QT, int CT>
 int launch_dim(const DecodeArgs& a, int64_t dim, int pack, bool split, hipStream_t st) {
-  switch (dim) {
-    case 64: return pack == 2 ? launch_matrix<QT, CT, 128, 2>(a, split, st) : launch_matrix<QT, CT, 64>(a, split, st);
-    case 96: return launch_matrix<QT, CT, 96>(a, split, st);
-    case 128: return launch_matrix<QT, CT, 128>(a, split, st);
-    case 192: return launch_matrix<QT, CT, 192>(a, split, st);
-    default: return launch_matrix<QT, CT, 256>(a, split, st);
-  }
+  if (pack == 2) return launch_matrix<QT, CT, 128, true, 2>(a, split, st);
+#define AYK_PD(D) \
+  if (dim <= D) return dim == D ? launch_matrix<QT, CT, D, true>(a, split, st) : launch_matrix<QT, CT, D, false>(a, split, st)
+  AYK_PD(64);
+  AYK_PD(96);
+  AYK_PD(128);
+  AYK_PD(192);
+  AYK_PD(256);
+#undef AYK_PD
+  return fail(AYK_EINVAL, "paged_decode_attention: dim=%lld", (long long)dim);
 }
-bool matrix_dim(int64_t dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256; }
+// A row of 16-byte pieces: dims in sixteens, or eights of 16 bits.
+bool matrix_dim(int64_t dim, int cache_dtype) { return dim % (elem_size(cache_dtype) == 1 ? 16 : 8) == 0; }
 
 }  // namespace
 }  // namespace ayk
@@ -617,8 +632,9 @@ using namespace ayk;
 extern "C" {
 
 size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
-  if (!matrix_dim(dim) || kv_heads < 1 || heads < kv_heads || batch < 1) return 0;
-  return (size_t)(2 * kMostRuns * kHeadTile * (dim + 2)) * sizeof(float);
+  if (dim < 1 || dim > kMaxDim || dim % 8 || kv_heads < 1 || heads < kv_heads || batch < 1) return 0;
+  const int64_t width = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;  // of the kernel
+  return (size_t)(2 * kMostRuns * kHeadTile * (width + 2)) * sizeof(float);
 }
 
 int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -655,7 +671,7 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
   const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
   const int pack = dim == 64 && group <= kHeadTile / 2 && kv_heads % 2 == 0 ? 2 : 1;
   const int64_t items = batch * tiles * (kv_heads / pack);
-  if (matrix_dim(dim) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
+  if (matrix_dim(dim, cache_dtype) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
       num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && c.row_bytes < 0x7FFFFFFF &&
       items < 0x7FFFFFFF) {
     DecodeArgs a{};
@@ -673,6 +689,7 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     a.lens = seq_lens;
     a.batch = (int)batch;
     a.heads = (int)heads;
+    a.dim = (int)dim;
     a.kv_items = (int)(kv_heads / pack);
     a.group = (int)group;
     a.tiles = (int)tiles;
