@@ -212,9 +212,9 @@ struct Running {
 
 // Kv heads of 64 dims are taken two at a time where both groups fit the 16 columns: one 64-dim
 // row fills half a cache line, whose other half, the neighbouring head's, another workgroup
-// would fetch again. K and V rows are then 128 dims, a column's Q is zero on the other head's
-// dims, and the half of O^T that mixes the heads is not written. PACK is 2 then, and the
-// columns of a head are:
+// would fetch again. K and V rows are then 128 dims, a column's scores are those of its own
+// head's half, and the half of O^T that mixes the heads is not written. PACK is 2 then, and
+// the columns of a head are:
 template <int PACK>
 struct Column {
   static constexpr int kSpan = kHeadTile / PACK;
@@ -301,9 +301,13 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
     v4f s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      v4f pair[PACK] = {};  // each head's own steps: a NaN of one must not reach the other through a zero of Q
 #pragma unroll
-      for (int d = 0; d < S::kSteps; ++d) s[t] = mfma16<QT>(k_frag<CT, QT, D>(kw[t], d), qf[d], s[t]);
+      for (int d = 0; d < S::kSteps; ++d) {
+        v4f& into = pair[d / (S::kSteps / PACK)];
+        into = mfma16<QT>(k_frag<CT, QT, D>(kw[t], d), qf[d], into);
+      }
+      s[t] = PACK == 2 && column.sub == 1 ? pair[PACK - 1] : pair[0];
     }
     __builtin_amdgcn_sched_barrier(0);
     if (more) {
