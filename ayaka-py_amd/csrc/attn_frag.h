@@ -101,6 +101,18 @@ __device__ inline int wave_scan(int v) {
 }
 __device__ inline int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1); }
 
+// The largest over the wave, and the next lane's value (lane 63: 0), of integers of at least 0.
+__device__ inline int wave_most(int v) {
+  v = max(v, dpp_int<0x111, 0xF>(v));
+  v = max(v, dpp_int<0x112, 0xF>(v));
+  v = max(v, dpp_int<0x114, 0xF>(v));
+  v = max(v, dpp_int<0x118, 0xF>(v));
+  v = max(v, dpp_int<0x142, 0xA>(v));
+  v = max(v, dpp_int<0x143, 0xC>(v));
+  return __builtin_amdgcn_readlane(v, kWave - 1);
+}
+__device__ inline int next_lane(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x130, 0xF, 0xF, false); }  // wave_shl 1
+
 constexpr float kLog2e = 1.44269504088896340736f;
 
 }  // namespace

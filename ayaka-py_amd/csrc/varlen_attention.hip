@@ -180,36 +180,26 @@ __device__ inline bool find_ranked(const VarlenArgs& a, int rank, Sequence* sq, 
   const int lane = threadIdx.x % kWave, b = lane < a.batch + 2 ? lane : a.batch + 2;
   const int q = b == 0 ? 0 : b == a.batch + 2 ? (int)a.total_q : (int)clamp_row(a.starts_q[b - 1], a.total_q);
   const int k = b > 0 && b < a.batch + 2 ? (int)clamp_row(a.starts_k[b - 1], a.total_k) : 0;
-  const int q1 = __shfl_down(q, 1, kWave), kn = __shfl_down(k, 1, kWave);
+  const int q1 = next_lane(q), kn = next_lane(k);
   const bool real = lane > 0 && lane <= a.batch;
   const int len_q = lane < a.batch + 2 && q1 > q ? q1 - q : 0, len_k = real && kn > k ? kn - k : 0;
   // keys of tile t: reach + t (R / 64), in tiles of KEYS; a sequence without keys counts 0 for all
   const int tiles = (len_q + R - 1) / R, reach = len_k == 0 ? 0 : (len_k - len_q + R) / KEYS, step = len_k == 0 ? 0 : R / KEYS;
-  auto at_least = [&](int len) {  // this sequence's tiles of at least `len` tiles of keys
-    if (step == 0) return len <= 0 ? tiles : 0;
+  auto at_least = [&](int len) {  // this sequence's tiles of at least `len` tiles of keys; all are of 0
+    if (len <= 0) return tiles;
+    if (step == 0) return 0;
     const int t = len <= reach ? 0 : (len - reach + step - 1) / step;
     return t < tiles ? tiles - t : 0;
   };
-  auto sum = [](int v) { return (int)wave_sum_dpp((float)v); };  // below 2^24
-  if (rank >= sum(tiles)) return false;
-  int low = reach < 0 ? reach : 0, high = reach + tiles * step + 1;  // more than `rank` tiles reach `low`, none `high`
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    low = min(low, __shfl_xor(low, off, kWave));
-    high = max(high, __shfl_xor(high, off, kWave));
-  }
+  if (rank >= wave_total(tiles)) return false;
+  int low = 0, high = wave_most(reach + tiles * step) + 1;  // more than `rank` tiles reach `low`, none `high`
   while (high - low > 1) {
     const int mid = low + (high - low) / 2;
-    if (sum(at_least(mid)) > rank) low = mid; else high = mid;
+    if (wave_total(at_least(mid)) > rank) low = mid; else high = mid;
   }
   const int longer = at_least(high), these = at_least(low) - longer;
-  int before = these;  // tiles of this length in the sequences up to this one
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const int v = __shfl_up(before, off, kWave);
-    if (lane >= off) before += v;
-  }
-  const int left = rank - sum(longer), at = __builtin_ctzll(__ballot(before > left));
+  const int before = wave_scan(these);  // tiles of this length in the sequences up to this one
+  const int left = rank - wave_total(longer), at = __builtin_ctzll(__ballot(before > left));
   *tile = __builtin_amdgcn_readlane(tiles - longer - 1, at) - (left - (__builtin_amdgcn_readlane(before, at) - __builtin_amdgcn_readlane(these, at)));
   sq->q0 = __builtin_amdgcn_readlane(q, at);
   sq->q1 = __builtin_amdgcn_readlane(q, at + 1);
@@ -339,17 +329,16 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
     for (int n = 0; n < kDma; ++n) load_to_lds(vr, to + kBytes + n * WAVES * 1024, v_off[n]);
   };
 
-  if (from < to) issue(from, 0);
-
+  // Q and the first tile are asked for together, and Q's sign or zero is put on afterwards.
   v4u qf[D / 16];
-  {
-    const uint16_t* p = a.q.p + (sq.q0 + my_row) * a.q.row + head * a.q.head + 8 * half;
+  const uint16_t* qp = a.q.p + (sq.q0 + my_row) * a.q.row + head * a.q.head + 8 * half;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      qf[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const v4u*>(p + 16 * s) : v4u{0, 0, 0, 0};
-      qf[s] = (qf[s] ^ a.q_flip) & a.q_keep;
-    }
-  }
+  for (int s = 0; s < D / 16; ++s) qf[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const v4u*>(qp + 16 * s) : v4u{0, 0, 0, 0};
+  __builtin_amdgcn_sched_barrier(0);
+  if (from < to) issue(from, 0);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) qf[s] = (qf[s] ^ a.q_flip) & a.q_keep;
 
   RunningRows<D> r;
   r.m = -INFINITY;
@@ -451,15 +440,23 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd = r.acc[t][e] != r.acc[t][e] ? NAN : odd;
   uint64_t again = __ballot(odd != odd && l == l && w0 + row < len_q);
-  if (w0 + row < len_q) {
-    uint16_t* o = a.out + ((sq.q0 + w0 + row) * a.heads + head) * a.dim + 4 * half;
+  {
+    // Runs of eight dims lie half in lane l and half in l + 32: of two runs each lane gets one.
+    uint16_t* o = a.out + ((sq.q0 + my_row) * a.heads + head) * a.dim + 8 * half;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (32 * t + 8 * e < a.dim)
-          *reinterpret_cast<uint2*>(o + 32 * t + 8 * e) = make_uint2(pack2<DT>(r.acc[t][4 * e] * f, r.acc[t][4 * e + 1] * f),
-                                                                     pack2<DT>(r.acc[t][4 * e + 2] * f, r.acc[t][4 * e + 3] * f));
+      for (int e = 0; e < 4; e += 2) {
+        v4u run;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const auto pair = __builtin_amdgcn_permlane32_swap(pack2<DT>(r.acc[t][4 * e + 2 * w] * f, r.acc[t][4 * e + 2 * w + 1] * f),
+                                                             pack2<DT>(r.acc[t][4 * e + 4 + 2 * w] * f, r.acc[t][4 * e + 5 + 2 * w] * f), false, false);
+          run[w] = pair[0];
+          run[2 + w] = pair[1];
+        }
+        if (w0 + row < len_q && 32 * t + 8 * e + 8 * half < a.dim) *reinterpret_cast<v4u*>(o + 32 * t + 8 * e) = run;
+      }
   }
   again |= again >> 32;
   for (again &= 0xFFFFFFFFull; again; again &= again - 1) {
