@@ -224,7 +224,7 @@ struct Column {
   __device__ int head(const DecodeArgs& a, int g, int tile) const { return (g * PACK + sub) * a.group + tile * kHeadTile + at; }
 };
 
-template <int QT, int CT, int D, int PACK, bool EXACT>
+template <int QT, int CT, int D, int PACK, bool EXACT, int WAVES>
 __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile, int from, int to, Running<D>& r) {
   using S = Shape<CT, D>;
   constexpr int PT = S::kFp8 ? AYK_F16 : QT;  // e4m3 and e5m2 are exact in fp16, whose weights round finer
@@ -292,11 +292,11 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
   // that loads are in flight throughout. The scheduling barriers keep them there: moved up,
   // they would need registers of their own.
   int slot = slot_of(i, page_of(i));
-  int page = i + 4 < most ? page_of(i + 4) : -1;
+  int page = i + WAVES < most ? page_of(i + WAVES) : -1;
   issue_k(slot);
   issue_v(slot);
   while (true) {
-    const bool more = i + 4 < most;
+    const bool more = i + WAVES < most;
     const uint32_t seen = (uint32_t)__ballot(slot >= 0);
     v4f s[2];
 #pragma unroll
@@ -311,8 +311,8 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
     }
     __builtin_amdgcn_sched_barrier(0);
     if (more) {
-      slot = slot_of(i + 4, page);
-      if (i + 8 < most) page = page_of(i + 8);
+      slot = slot_of(i + WAVES, page);
+      if (i + 2 * WAVES < most) page = page_of(i + 2 * WAVES);
       issue_k(slot);
     }
     float x[8], top = -INFINITY;
@@ -380,19 +380,19 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int g, int tile
     __builtin_amdgcn_sched_barrier(0);
     if (!more) break;
     issue_v(slot);
-    i += 4;
+    i += WAVES;
   }
 }
 
 // What a result under maximum m counts under a common one.
 __device__ inline float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
 
-// Join the four waves' results in wave 0: 2 and 3 hand theirs to 0 and 1, then 1 to 0.
-template <int D>
+// Join the waves' results in wave 0: the upper half hands theirs to the lower, and so on.
+template <int D, int WAVES>
 __device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave]) {
   const int lane = item_lane(), wave = threadIdx.x / kWave;
 #pragma unroll
-  for (int half = 2; half >= 1; half /= 2) {
+  for (int half = WAVES / 2; half >= 1; half /= 2) {
     __syncthreads();  // the slots' last readers are done
     if (wave >= half && wave < 2 * half) {
       float(*to)[kWave] = lds[wave - half];
@@ -451,15 +451,14 @@ __device__ inline void write_item(const DecodeArgs& a, int b, int g, int tile, c
     }
 }
 
-// One workgroup per sequence, kv head and head tile: for calls whose longest possible
-// sequence is a few steps.
-template <int QT, int CT, int D, int PACK, bool EXACT>
-__global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_kernel(DecodeArgs a) {
-  __shared__ float lds[2][D / 4 + 2][kWave];
+// One workgroup per sequence, kv head and head tile, whose waves take its blocks in turn.
+template <int QT, int CT, int D, int PACK, bool EXACT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_kernel(DecodeArgs a) {
+  __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_blocks<QT, CT, D, PACK, EXACT>(a, b, g, tile, 0, 0x1FFFFFF, r);
-  join_waves<D>(r, lds);
+  attend_blocks<QT, CT, D, PACK, EXACT, WAVES>(a, b, g, tile, 0, 0x1FFFFFF, r);
+  join_waves<D, WAVES>(r, lds);
   if (threadIdx.x < kWave) write_item<QT, CT, D, PACK, EXACT>(a, b, g, tile, r, nullptr);
 }
 
@@ -500,8 +499,8 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
       const int last = first + (end - at) < steps ? first + (end - at) : steps;
       Running<D> r;
       const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
-      attend_blocks<QT, CT, D, PACK, EXACT>(a, b, g, tile, first, last, r);
-      join_waves<D>(r, lds);
+      attend_blocks<QT, CT, D, PACK, EXACT, 4>(a, b, g, tile, first, last, r);
+      join_waves<D, 4>(r, lds);
       float* partial = nullptr;
       if (first > 0 || last < steps)
         partial = a.partial + ((int64_t)run * 2 + (first > 0 ? 0 : 1)) * a.rows * (D / PACK + 2);
@@ -591,8 +590,13 @@ constexpr int kMostRuns = 1024;  // workgroups of a split launch that the chip h
 template <int QT, int CT, int D, bool EXACT, int PACK = 1>
 int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
   if (!split) {
-    hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, PACK, EXACT>), dim3((unsigned)(a.batch * a.tiles * a.kv_items)),
-                       dim3(kDecodeThreads), 0, st, a);
+    const unsigned items = (unsigned)(a.batch * a.tiles * a.kv_items);
+    // Two waves a SIMD where a CU has one workgroup at most.
+    constexpr int kMostWaves = Shape<CT, D>::kWavesPerSimd >= 2 ? 8 : 4;
+    if (items <= 256)
+      hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, PACK, EXACT, kMostWaves>), dim3(items), dim3(kMostWaves * kWave), 0, st, a);
+    else
+      hipLaunchKernelGGL((paged_decode_kernel<QT, CT, D, PACK, EXACT, 4>), dim3(items), dim3(4 * kWave), 0, st, a);
     note_plan("paged_decode whole");
   } else {
     constexpr int runs = 256 * Shape<CT, D>::kWavesPerSimd;
@@ -625,6 +629,18 @@ int launch_dim(const DecodeArgs& a, int64_t dim, int pack, bool split, hipStream
 #undef AYK_PD
   return fail(AYK_EINVAL, "paged_decode_attention: dim=%lld", (long long)dim);
 }
+// The longest sequence (as far as the table's width says) whose items stay whole, a workgroup
+// each, in one launch: dealing out steps costs a second launch, partial results and a start
+// amid an item, a whole item the time of its blocks one after the other. 32 query heads over 8
+// of 128 e4m3 dims, whole and dealt out, us: 1 x 2000 18 / 20, 1 x 3000 23 / 21, 32 x 2000 33
+// / 38, 24 x 4000 41 / 33 (at most a workgroup a CU: eight waves, about 80 KB each); 48 x 1500
+// 40 / 43, 48 x 2000 39 / 35 (unequal; up to two a CU); 64 x 2000 44 / 46, 200 x 700 44 / 64,
+// 256 x 1500 104 / 111, 256 x 4000 261 / 231. 96 x 1024 in pairs of 64 e5m2 dims: 25 / 36.
+int64_t whole_limit(int64_t items, int64_t dim, int elem) {
+  const int64_t row = 2 * (dim < 64 ? 64 : dim) * elem, alone = dim * elem < 256 ? 640 : 320;
+  return (items <= 256 ? alone : items < 512 ? 400 : 560) * 1024 / row;
+}
+
 // A row of 16-byte pieces: dims in sixteens, or eights of 16 bits.
 bool matrix_dim(int64_t dim, int cache_dtype) { return dim % (elem_size(cache_dtype) == 1 ? 16 : 8) == 0; }
 
@@ -706,11 +722,9 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     a.out = static_cast<uint16_t*>(out);
     a.partial = static_cast<float*>(workspace);
     a.q_aligned = aligned16(q) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0;
-    // A sequence of at most four steps stays with one workgroup: a second launch would cost
-    // more than the steps.
     const int64_t longest = window > 0 && window + sinks < most ? window + sinks + 2 * kBlock : most;
     const int64_t steps = cdiv(longest, kStep) + 1;
-    const bool split = longest > 4 * kStep && items * steps < 0x40000000 && workspace != nullptr && aligned16(workspace) &&
+    const bool split = longest > whole_limit(items, dim * pack, elem_size(cache_dtype)) && items * steps < 0x40000000 && workspace != nullptr && aligned16(workspace) &&
                        workspace_bytes >= ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
     if (cache_dtype == AYK_E4M3)
       return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, pack, split, st);

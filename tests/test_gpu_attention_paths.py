@@ -34,7 +34,7 @@ def plan():
                                              (E5M2, F16, 208), (BF16, BF16, 8), (BF16, BF16, 72), (F16, F16, 120),
                                              (BF16, BF16, 168), (F16, F16, 248), (E4M3, BF16, 96), (E4M3, BF16, 192)])
 def test_head_sizes_split(gpu, cache, dtype, dim):
-    decode.check(decode.make_case([1300, 40, 0], 6, 2, dim, 16, cache, dtype, seed=dim), gpu, f"split dim={dim} {cache}")
+    decode.check(decode.make_case([5600, 40, 0], 6, 2, dim, 16, cache, dtype, seed=dim), gpu, f"split dim={dim} {cache}")
     assert plan() == "paged_decode split"
     decode.check(decode.make_case([90, 40, 0], 6, 2, dim, 16, cache, dtype, seed=dim), gpu, f"whole dim={dim} {cache}")
     assert plan() == "paged_decode whole"
@@ -69,7 +69,7 @@ def test_a_pair_keeps_its_heads_apart(gpu):
 @pytest.mark.parametrize("batch,heads,kv_heads,dim", [(1, 8, 8, 128), (40, 8, 2, 64), (70, 16, 1, 128), (130, 24, 2, 64)])
 def test_joins_of_few_and_many_heads(gpu, batch, heads, kv_heads, dim):
     """Sequence lengths from nothing to thousands in one call; every join width."""
-    lens = [0 if i % 9 == 4 else 1 + (i * 977) % 1500 for i in range(batch - 1)] + [2600]
+    lens = [0 if i % 9 == 4 else 1 + (i * 977) % 1500 for i in range(batch - 1)] + [5600]
     decode.check(decode.make_case(lens, heads, kv_heads, dim, 16, seed=batch), gpu, f"joins batch={batch}")
     assert plan() == "paged_decode split"
 
