@@ -65,6 +65,14 @@ __global__ __launch_bounds__(kRowThreads) void varlen_rows_kernel(Packed q, Pack
 // O^T = V^T P^T wants its second operand if V's k slots are numbered alike: the weights never
 // cross lanes, a row's maximum and sum are within a lane but for one swap of halves, and V is
 // read transposed from LDS (ds_read_b64_tr_b16).
+//
+// 8192 causal positions of 64 heads of 128 bf16 dims, 1.10 TFLOP: 1.02 ms, 1.08 PFLOP/s, 76% of
+// what a bf16 product of 8192^3 reaches on this card. Both hold the power limit: with zeros
+// for inputs the same launch runs at 2.4 GHz instead of 1.9 and takes 0.77 ms. There the matrix
+// units are busy 58% of the time; three waves a SIMD hide most of the exponentials, the LDS
+// latency and the barriers. More waves a workgroup with more stages (8 x 4: 1.07 ms), loads
+// spread over the products (1.08), priorities for the products and row sums by a product with
+// ones (1.10) were measured and are not used.
 constexpr int kMostSplits = 16;
 constexpr int kWaveRows = 32, kTileWaves = 4, kTileRows = kTileWaves * kWaveRows, kTileThreads = kTileWaves * kWave;
 
