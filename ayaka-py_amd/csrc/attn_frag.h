@@ -62,6 +62,9 @@ __device__ inline uint2 read_transposed(const uint8_t* lds) {
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The largest of three, NaN losing to numbers (fmaxf alone costs a canonicalization an operand).
+// The compiler does not count the wait that a read of a matrix product's result needs for an
+// assembly statement: at least one operand must come from another instruction that read the
+// same product's result.
 __device__ inline float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));

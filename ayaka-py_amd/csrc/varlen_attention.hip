@@ -230,7 +230,9 @@ struct RunningRows {
 // The weights of a tile, from its scores; s becomes exp2(scale (s - m)).
 template <int D, int U>
 __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
-  float top = s[0][0];
+  // The chain starts with an operation that the compiler knows to read the products' results:
+  // it waits for them, which it would not for the assembly of max3 alone.
+  float top = fmaxf(s[0][14], s[U - 1][15]);
 #pragma unroll
   for (int i = 0; i < 16; i += 3 - U) top = max3(top, s[0][i], U == 2 ? s[U - 1][i] : s[0][i + 1]);
   top = max_halves(top);

@@ -127,6 +127,32 @@ def test_split_hidden_and_visible_values_that_are_not_finite(gpu):
         assert torch.isfinite(out[10:][..., rest]).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("sequences", [1, 700])
+def test_steep_scores_in_fp16(gpu, dim, sequences):
+    """Scores that rise, fall or jump by 2^20 and more within a tile: a maximum that misses any of
+    them overflows an fp16 weight. Many short sequences take the other tile size at 128 dims."""
+    from ayaka.kernel.hip import varlen_attention
+
+    n = 333 if sequences == 1 else 70
+    gen = torch.Generator().manual_seed(dim)
+    jumps = torch.randperm(n, generator=gen).double() / n * 240 - 120
+    for name, score in (("rising", torch.linspace(-120, 120, n).double()), ("falling", torch.linspace(120, -120, n).double()),
+                        ("jumping", jumps)):
+        key = (score / 32)[:, None, None].expand(n, 1, dim).to(F16)
+        value = torch.randn(n, 1, dim, generator=gen).to(F16)
+        query = torch.ones(n, 2, dim, dtype=F16)
+        starts = torch.tensor([0, n], dtype=torch.int32)
+        scale = 32.0 / dim
+        ref, parts = ora.varlen_attention(query, key, value, starts, starts, scale)
+        many = lambda t: t.to(gpu).repeat(sequences, 1, 1)  # noqa: E731
+        all_starts = torch.arange(0, sequences * n + 1, n, dtype=torch.int32, device=gpu)
+        out = varlen_attention(many(query), many(key), many(value), all_starts, all_starts, scale).view(sequences, n, 2, dim)
+        for b in sorted({0, sequences // 2, sequences - 1}):
+            assert_attention_close(out[b], ref, parts, F16, f"{name} dim={dim} sequence {b}")
+        assert torch.equal(out, out[:1].expand_as(out))
+
+
 def test_nan_queries_stay_in_their_rows(gpu):
     c = varlen.make_case([150, 60], 4, 2, 128, seed=3)
     ref, parts = varlen.oracle(c)
