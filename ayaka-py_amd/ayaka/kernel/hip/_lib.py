@@ -76,6 +76,7 @@ SIGNATURES: dict[str, list[Any]] = {
     "ayk_paged_decode_attention": [_p, _i, _l, _l, _p, _p, _i, _l, _l, _p, _l, _l, _p, _l, _l, _l, _l, _f, _f, _f, _l, _l,
                                    _p, _p, _z, _p],
     "ayk_paged_decode_attention_workspace_bytes": [_l, _l, _l, _l],
+    "ayk_paged_decode_attention_split_bytes": [_l, _l, _l, _l, _i, _l, _l, _l],
     "ayk_varlen_attention": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _p, _p, _l, _l, _l, _l, _l, _l, _f, _i, _l, _l, _p, _p],
     "ayk_varlen_attention_split": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _p, _p, _l, _l, _l, _l, _l, _l, _f, _i, _l, _l, _p,
                                    _p, _z, _p],
@@ -103,6 +104,7 @@ _RESTYPES: dict[str, Any] = {
     "ayk_fp8_weight_only_gemm_workspace_bytes": _z,
     "ayk_paged_decode_attention_workspace_bytes": _z,
     "ayk_varlen_attention_split_workspace_bytes": _z,
+    "ayk_paged_decode_attention_split_bytes": _z,
     "ayk_fp8_weight_only_gemv_static_max_bytes": _z,
 }
 

@@ -42,8 +42,11 @@ def _check(query, key_cache, value_cache, block_tables, seq_lens) -> None:
                         (block_tables, "block_tables"), (seq_lens, "seq_lens")):
             require_cuda(t, name)
             require_same_device(t, name, query, "query")
-    require_dtype(query, "query", ATTENTION_DTYPES)
-    require_dtype(key_cache, "key_cache", (*_FP8_DTYPES, query.dtype))
+    dtype = query.dtype
+    if dtype not in ATTENTION_DTYPES:
+        require_dtype(query, "query", ATTENTION_DTYPES)
+    if key_cache.dtype not in _FP8_DTYPES and key_cache.dtype != dtype:
+        require_dtype(key_cache, "key_cache", (*_FP8_DTYPES, dtype))
     shape, cache = query.shape, key_cache.shape
     if len(shape) != 3:
         raise ValueError("query must be [batch, heads, head_dim]")
@@ -55,8 +58,9 @@ def _check(query, key_cache, value_cache, block_tables, seq_lens) -> None:
     if cache[1] < 1 or cache[3] != dim:
         raise ValueError(f"cache {tuple(cache)} does not match a query of head_dim {dim}")
     check_heads(heads, cache[2], dim)
-    require_dtype(block_tables, "block_tables", (torch.int32,))
-    require_dtype(seq_lens, "seq_lens", (torch.int32,))
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        require_dtype(block_tables, "block_tables", (torch.int32,))
+        require_dtype(seq_lens, "seq_lens", (torch.int32,))
     table = block_tables.shape
     if len(table) != 2 or table[0] != batch or (table[1] > 1 and block_tables.stride(1) != 1):
         raise ValueError("block_tables must be [batch, pages] with stride(1) == 1")
@@ -101,21 +105,26 @@ def paged_decode_attention(
     _check(query, key_cache, value_cache, block_tables, seq_lens)
     check_window(window, sinks)
     check_scale(softmax_scale)
-    if not (math.isfinite(k_scale) and k_scale > 0 and math.isfinite(v_scale) and v_scale > 0):
+    if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
         raise ValueError("KV scales must be finite and positive")
-    result = new_output(query) if out is None else prepare_output(query, out, like_name="query")
-    if not result.is_contiguous():
-        raise ValueError("out must be contiguous")
+    if out is None:
+        result = new_output(query)
+    else:
+        result = prepare_output(query, out, like_name="query")
+        if not result.is_contiguous():
+            raise ValueError("out must be contiguous")
     batch, heads, dim = query.shape
     if batch == 0:
         return result
     query = rows_of_heads(query)
     pages, page_size, kv_heads, _ = key_cache.shape
-    need = _lib.query("ayk_paged_decode_attention_workspace_bytes", batch, heads, kv_heads, dim)
+    width = block_tables.shape[1]
+    cache_code = _lib.dtype_code(key_cache.dtype)
+    need = _lib.query("ayk_paged_decode_attention_split_bytes", batch, heads, kv_heads, dim, cache_code, width * page_size,
+                      window, sinks)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     _lib.call("ayk_paged_decode_attention", query.data_ptr(), _lib.dtype_code(query.dtype), query.stride(0), query.stride(1),
-              key_cache.data_ptr(), value_cache.data_ptr(), _lib.dtype_code(key_cache.dtype), pages, page_size,
-              block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(), batch, heads,
-              kv_heads, dim, softmax_scale, k_scale, v_scale, window, sinks, result.data_ptr(), _lib.ptr(workspace), need,
-              _lib.stream_of(query))
+              key_cache.data_ptr(), value_cache.data_ptr(), cache_code, pages, page_size, block_tables.data_ptr(),
+              block_tables.stride(0), width, seq_lens.data_ptr(), batch, heads, kv_heads, dim, softmax_scale, k_scale, v_scale,
+              window, sinks, result.data_ptr(), _lib.ptr(workspace), need, _lib.stream_of(query))
     return result

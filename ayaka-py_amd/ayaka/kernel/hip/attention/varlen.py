@@ -38,9 +38,11 @@ def _check(query, key, value, cu_seqlens_q, cu_seqlens_k) -> None:
                         (cu_seqlens_k, "cu_seqlens_k")):
             require_cuda(t, name)
             require_same_device(t, name, query, "query")
-    require_dtype(query, "query", ATTENTION_DTYPES)
-    require_dtype(key, "key", (query.dtype,))
-    require_dtype(value, "value", (query.dtype,))
+    dtype = query.dtype
+    if dtype not in ATTENTION_DTYPES or key.dtype != dtype or value.dtype != dtype:
+        require_dtype(query, "query", ATTENTION_DTYPES)
+        require_dtype(key, "key", (dtype,))
+        require_dtype(value, "value", (dtype,))
     shape, keys = query.shape, key.shape
     if len(shape) != 3:
         raise ValueError("query must be [tokens, heads, head_dim]")
@@ -48,7 +50,8 @@ def _check(query, key, value, cu_seqlens_q, cu_seqlens_k) -> None:
         raise ValueError("key and value must be [tokens, kv_heads, head_dim] of one shape, with the query's head_dim")
     check_heads(shape[1], keys[1], shape[2])
     for t, name in ((cu_seqlens_q, "cu_seqlens_q"), (cu_seqlens_k, "cu_seqlens_k")):
-        require_dtype(t, name, (torch.int32,))
+        if t.dtype != torch.int32:
+            require_dtype(t, name, (torch.int32,))
         if t.ndim != 1 or t.shape[0] < 1 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous [sequences + 1] vector")
     if cu_seqlens_q.shape != cu_seqlens_k.shape:
@@ -92,9 +95,12 @@ def varlen_attention(
     check_scale(softmax_scale)
     if window and not causal:
         raise ValueError("a window needs causal attention")
-    result = new_output(query) if out is None else prepare_output(query, out, like_name="query")
-    if not result.is_contiguous():
-        raise ValueError("out must be contiguous")
+    if out is None:
+        result = new_output(query)
+    else:
+        result = prepare_output(query, out, like_name="query")
+        if not result.is_contiguous():
+            raise ValueError("out must be contiguous")
     tokens, heads, dim = query.shape
     batch = cu_seqlens_q.shape[0] - 1
     if tokens == 0:

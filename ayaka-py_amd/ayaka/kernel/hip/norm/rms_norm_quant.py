@@ -31,7 +31,9 @@ def _outputs(x, group_size, scale_dtype, scale_col_major):
     *lead, k = x.shape
     rows = math.prod(lead)
     shape = (rows,) if group_size == 0 else (k // group_size, rows) if scale_col_major else (rows, k // group_size)
-    return x.new_empty((rows, k), dtype=FP8), x.new_empty(shape, dtype=_SCALE_DTYPES[scale_dtype])
+    q = (torch.empty_like(x, dtype=FP8, memory_format=torch.contiguous_format) if len(lead) == 1
+         else x.new_empty((rows, k), dtype=FP8))
+    return q, x.new_empty(shape, dtype=_SCALE_DTYPES[scale_dtype])
 
 
 def _rms_norm_quant_fake(x, weight, eps, group_size=0, scale_dtype="float32", scale_col_major=False):

@@ -646,6 +646,20 @@ int64_t whole_limit(int64_t items, int64_t dim, int elem) {
   return (items <= 256 ? alone : items < 512 ? 400 : 560) * 1024 / row;
 }
 
+// Kv heads taken together (the kernels' PACK), the positions that a window leaves of `most`, and
+// whether the items of such a call are dealt out.
+int pack_of(int64_t heads, int64_t kv_heads, int64_t dim) {
+  return dim == 64 && heads / kv_heads <= kHeadTile / 2 && kv_heads % 2 == 0 ? 2 : 1;
+}
+int64_t longest_of(int64_t most, int64_t window, int64_t sinks) {
+  return window > 0 && sinks < most && window < most - sinks ? window + sinks + 2 * kBlock : most;
+}
+bool deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int elem, int64_t longest) {
+  const int pack = pack_of(heads, kv_heads, dim);
+  const int64_t items = batch * cdiv(heads / kv_heads, kHeadTile) * (kv_heads / pack);
+  return longest > whole_limit(items, dim * pack, elem) && items * (cdiv(longest, kStep) + 1) < 0x40000000;
+}
+
 // A row of 16-byte pieces: dims in sixteens, or eights of 16 bits.
 bool matrix_dim(int64_t dim, int cache_dtype) { return dim % (elem_size(cache_dtype) == 1 ? 16 : 8) == 0; }
 
@@ -660,6 +674,13 @@ size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, 
   if (dim < 1 || dim > kMaxDim || dim % 8 || kv_heads < 1 || heads < kv_heads || batch < 1) return 0;
   const int64_t width = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;  // of the kernel
   return (size_t)(2 * kMostRuns * kHeadTile * (width + 2)) * sizeof(float);
+}
+
+size_t ayk_paged_decode_attention_split_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int cache_dtype,
+                                              int64_t most, int64_t window, int64_t sinks) {
+  const size_t bytes = ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
+  if (bytes == 0 || !is_cache_dtype(cache_dtype) || most < 0 || window < 0 || sinks < 0) return 0;
+  return deals_out(batch, heads, kv_heads, dim, elem_size(cache_dtype), longest_of(most, window, sinks)) ? bytes : 0;
 }
 
 int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -694,7 +715,7 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
   const bool bf = q_dtype == AYK_BF16;
   // The matrix kernels count positions, slots and items in 32 bits and load 16 bytes at a time.
   const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
-  const int pack = dim == 64 && group <= kHeadTile / 2 && kv_heads % 2 == 0 ? 2 : 1;
+  const int pack = pack_of(heads, kv_heads, dim);
   const int64_t items = batch * tiles * (kv_heads / pack);
   if (matrix_dim(dim, cache_dtype) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
       num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && c.row_bytes < 0x7FFFFFFF &&
@@ -727,9 +748,8 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     a.out = static_cast<uint16_t*>(out);
     a.partial = static_cast<float*>(workspace);
     a.q_aligned = aligned16(q) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0;
-    const int64_t longest = window > 0 && window + sinks < most ? window + sinks + 2 * kBlock : most;
-    const int64_t steps = cdiv(longest, kStep) + 1;
-    const bool split = longest > whole_limit(items, dim * pack, elem_size(cache_dtype)) && items * steps < 0x40000000 && workspace != nullptr && aligned16(workspace) &&
+    const bool split = deals_out(batch, heads, kv_heads, dim, elem_size(cache_dtype), longest_of(most, window, sinks)) &&
+                       workspace != nullptr && aligned16(workspace) &&
                        workspace_bytes >= ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
     if (cache_dtype == AYK_E4M3)
       return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, pack, split, st);

@@ -325,6 +325,10 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
                                float k_scale, float v_scale, int64_t window, int64_t sinks, void* out,
                                void* workspace, size_t workspace_bytes, ayk_stream_t stream);
 size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
+/* The same for calls whose longest possible sequence is known, table_width * page_size positions:
+ * 0 where every sequence stays whole. */
+size_t ayk_paged_decode_attention_split_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int cache_dtype,
+                                              int64_t most, int64_t window, int64_t sinks);
 
 /* Packed sequences: sequence b holds query rows [starts_q[b], starts_q[b + 1]) and key rows
  * [starts_k[b], starts_k[b + 1]); its queries are the last positions of its keys (more

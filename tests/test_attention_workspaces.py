@@ -39,3 +39,13 @@ def test_workspaces_hold_what_the_kernels_write():
         assert paged(4, 32, 8, dim) == 2 * 1024 * 16 * (width + 2) * 4
     assert paged(4, 32, 8, 100) == 0  # the row kernel takes none
     assert paged(4, 4, 8, 128) == 0
+    # sequences that stay whole ask for none
+    split_bytes = lambda *a: _lib.query("ayk_paged_decode_attention_split_bytes", *a)  # noqa: E731
+    assert split_bytes(1, 32, 8, 128, _lib.AYK_E4M3, 1024, 0, 0) == 0
+    assert split_bytes(1, 32, 8, 128, _lib.AYK_E4M3, 100000, 0, 0) == paged(1, 32, 8, 128)
+    assert split_bytes(1, 32, 8, 128, _lib.AYK_E4M3, 100000, 1024, 4) == 0
+    assert split_bytes(1, 32, 8, 128, _lib.AYK_E4M3, 100000, 2**62, 2**62) == paged(1, 32, 8, 128)
+    assert split_bytes(1, 32, 8, 100, _lib.AYK_BF16, 100000, 0, 0) == 0
+    for bad in ((0, 32, 8, 128, 3, 9, 0, 0), (1, 0, 8, 128, 3, 9, 0, 0), (1, 32, 0, 128, 3, 9, 0, 0), (1, 32, 8, 128, 0, 9, 0, 0),
+                (1, 32, 8, 128, 3, -1, 0, 0), (1, 32, 8, 128, 3, 9, -1, 0)):
+        assert split_bytes(*bad) == 0
