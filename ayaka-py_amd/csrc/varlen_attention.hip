@@ -192,15 +192,16 @@ __device__ inline bool find_ranked(const VarlenArgs& a, int rank, Sequence* sq, 
   const bool real = lane > 0 && lane <= a.batch;
   const int len_q = lane < a.batch + 2 && q1 > q ? q1 - q : 0, len_k = real && kn > k ? kn - k : 0;
   // keys of tile t: reach + t (R / 64), in tiles of KEYS; a sequence without keys counts 0 for all
-  const int tiles = (len_q + R - 1) / R, reach = len_k == 0 ? 0 : (len_k - len_q + R) / KEYS, step = len_k == 0 ? 0 : R / KEYS;
+  constexpr int step = R / KEYS;
+  const int tiles = (len_q + R - 1) / R, reach = len_k == 0 ? 0 : (len_k - len_q + R) / KEYS;
   auto at_least = [&](int len) {  // this sequence's tiles of at least `len` tiles of keys; all are of 0
     if (len <= 0) return tiles;
-    if (step == 0) return 0;
-    const int t = len <= reach ? 0 : (len - reach + step - 1) / step;
+    if (len_k == 0) return 0;
+    const int t = len <= reach ? 0 : (int)((uint32_t)(len - reach + step - 1) / step);
     return t < tiles ? tiles - t : 0;
   };
   if (rank >= wave_total(tiles)) return false;
-  int low = 0, high = wave_most(reach + tiles * step) + 1;  // more than `rank` tiles reach `low`, none `high`
+  int low = 0, high = wave_most(len_k == 0 ? 0 : reach + tiles * step) + 1;  // more than `rank` tiles reach `low`, none `high`
   while (high - low > 1) {
     const int mid = low + (high - low) / 2;
     if (wave_total(at_least(mid)) > rank) low = mid; else high = mid;
