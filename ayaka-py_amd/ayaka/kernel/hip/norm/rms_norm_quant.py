@@ -45,14 +45,17 @@ def _add_rms_norm_quant_fake(x, residual, weight, eps, group_size=0, scale_dtype
 
 
 def _check(x, weight, eps, group_size, scale_dtype, scale_col_major) -> None:
-    _validate_input(x, "x")
-    k = int(x.shape[-1])
+    shape = x.shape
+    if x.dtype not in _FLOAT_DTYPES or not x.is_cuda or not shape:
+        _validate_input(x, "x")
+    k = shape[-1]
     if k < 1:
         raise ValueError("x must have a positive last dimension")
-    require_cuda(weight, "weight")
-    require_dtype(weight, "weight", _FLOAT_DTYPES)
-    require_same_device(weight, "weight", x, "x")
-    if weight.ndim != 1 or weight.shape[0] != k or not weight.is_contiguous():
+    if weight.dtype not in _FLOAT_DTYPES or weight.get_device() != x.get_device():
+        require_cuda(weight, "weight")
+        require_dtype(weight, "weight", _FLOAT_DTYPES)
+        require_same_device(weight, "weight", x, "x")
+    if weight.shape != (k,) or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous vector of shape [{k}]")
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative")
@@ -67,18 +70,25 @@ def _check(x, weight, eps, group_size, scale_dtype, scale_col_major) -> None:
         raise ValueError(f"K={k} must be divisible by group_size={group_size}")
 
 
+def _rows(x, rows, k):
+    """``x`` as ``[rows, k]`` with unit stride along ``k``, and the distance of its rows."""
+    if not x.is_contiguous():
+        x = _rows_2d(x)
+        return x, x.stride(0) if rows > 1 else k
+    return x, k
+
+
 def _launch(x, residual, weight, eps, group_size, scale_dtype, scale_col_major):
     q, scale = _outputs(x, group_size, scale_dtype, scale_col_major)
     rows, k = q.shape
     residual_out = None if residual is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     if rows:
-        x2d = _rows_2d(x)
-        r2d = None if residual is None else _rows_2d(residual)
-        strides = (1, rows) if scale_col_major else (k // group_size if group_size else 1, 1)
-        _lib.call("ayk_rms_norm_quant_fp8", x2d.data_ptr(), _lib.dtype_code(x.dtype), rows, k,
-                  x2d.stride(0) if rows > 1 else k, _lib.ptr(r2d), 0 if r2d is None else r2d.stride(0) if rows > 1 else k,
+        x2d, ldx = _rows(x, rows, k)
+        r2d, ldr = (None, 0) if residual is None else _rows(residual, rows, k)
+        scale_row, scale_group = (1, rows) if scale_col_major else (k // group_size if group_size else 1, 1)
+        _lib.call("ayk_rms_norm_quant_fp8", x2d.data_ptr(), _lib.dtype_code(x.dtype), rows, k, ldx, _lib.ptr(r2d), ldr,
                   weight.data_ptr(), _lib.dtype_code(weight.dtype), eps, group_size, _lib.dtype_code(scale.dtype),
-                  q.data_ptr(), scale.data_ptr(), *strides, _lib.ptr(residual_out), _lib.stream_of(x))
+                  q.data_ptr(), scale.data_ptr(), scale_row, scale_group, _lib.ptr(residual_out), _lib.stream_of(x))
     return q, scale, residual_out
 
 
@@ -124,8 +134,9 @@ def add_rms_norm_quant_fp8(
     dtype, as the next residual. ``residual`` has ``x``'s shape and dtype and is not changed.
     """
     _check(x, weight, eps, group_size, scale_dtype, scale_col_major)
-    require_cuda(residual, "residual")
-    require_same_device(residual, "residual", x, "x")
+    if residual.get_device() != x.get_device():
+        require_cuda(residual, "residual")
+        require_same_device(residual, "residual", x, "x")
     if residual.shape != x.shape or residual.dtype != x.dtype:
         raise ValueError("residual must have x's shape and dtype")
     return _launch(x, residual, weight, eps, group_size, scale_dtype, scale_col_major)
