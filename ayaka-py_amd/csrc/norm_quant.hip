@@ -97,13 +97,13 @@ __device__ inline bool short_way(float amax, float amax_y) {
   return amax >= 0x1p-100f && amax < INFINITY && amax_y >= 1e-10f && amax_y < INFINITY;
 }
 
-// 8192 rows of 8192 bf16 with a residual, 470 MB: 91 us, 5.2 TB/s, the rate of a large copy; 32
+// 8192 rows of 8192 bf16 with a residual, 470 MB: 83 us, 5.7 TB/s, above the rate of a large copy; 32
 // rows of 7168 with group scales: 4.6 us of the kernel, one row's chain of load, sum, amax.
 //
 // One workgroup of NT threads per row, the row's h in VPT 16-byte vectors' worth of fp32 a
 // thread: thread t holds vectors t, t + NT, ... 2^log_gl lanes, neighbours in one wave, hold a
-// group. Loads return in order, so the weight, which the caches hold, is asked for first: behind
-// the row it took 93 us, and 46.5 for 43 us at 16384 rows of 2048 with groups of 128.
+// group. Loads return in order, so the weight, which the caches hold, is asked for first: 16384
+// rows of 2048 with groups of 128 took 47.9 us with it behind the row, 43.1 so (four vectors a thread).
 //
 // 1 / rms is in y and in s alike, so codes by float scales are taken of h w: one rounding an
 // element (none for 16-bit inputs without a residual) where y has two, and the amax is joined
@@ -324,15 +324,16 @@ int launch(const void* x, int64_t rows, int64_t k, int64_t ldx, const void* res,
     return check_launch("rms_norm_quant_fp8");                                             \
   } while (0)
   if (vec) {
-    // Few rows leave CUs idle, so a row takes one vector a thread; many rows keep up to four
-    // vectors a thread in flight and join fewer waves.
+    // Few rows leave CUs idle, so a row takes one vector a thread. Many rows keep two a thread in
+    // flight: 8192 rows of 8192 take 83 us so, 91 with four and 86 with one in 1024 threads; 4096
+    // without a residual 20.2, 21.2 and 27.5.
     const bool few = rows <= 512;
     if (nvec <= 64) AYK_RM(64, 1);
     if (nvec <= 128 && !few) AYK_RM(64, 2);
-    if (nvec <= 256) { if (few) AYK_RM(256, 1); else AYK_RM(64, 4); }
+    if (nvec <= 256) { if (few) AYK_RM(256, 1); else AYK_RM(128, 2); }
     if (nvec <= 512 && !few) AYK_RM(256, 2);
-    if (nvec <= 1024) { if (few) AYK_RM(1024, 1); else AYK_RM(256, 4); }
-    if (nvec <= 2048) { if (few) AYK_RM(1024, 2); else AYK_RM(512, 4); }
+    if (nvec <= 1024) { if (few) AYK_RM(1024, 1); else AYK_RM(512, 2); }
+    if (nvec <= 2048) AYK_RM(1024, 2);
     AYK_RM(1024, 4);
   }
 #undef AYK_RM
