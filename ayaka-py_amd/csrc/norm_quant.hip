@@ -14,6 +14,8 @@
 namespace ayk {
 namespace {
 
+constexpr int64_t kLastLevelCache = 256ll << 20;  // bytes
+
 enum { kScaleRow = 0, kScaleGroup = 1, kScaleMx = 2 };
 
 // The sum and the largest over a workgroup of NT threads, in a fixed order, behind one barrier.
@@ -73,6 +75,15 @@ __device__ inline void store_vec(typename T::storage* p, const float* f) {
   }
 }
 
+// ONCE: past the caches.
+template <bool ONCE>
+__device__ inline uint4 load_vec(const uint4* p) {
+  if constexpr (!ONCE) return *p;
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  const v4u v = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // Vector v of y, from memory: the steps of the definition, for what the short way below leaves.
 template <typename T>
 __device__ inline void norm_vec(const uint4* xr, const uint4* rr, const void* w, int w_dtype, int v, float rstd, float* y) {
@@ -97,7 +108,7 @@ __device__ inline bool short_way(float amax, float amax_y) {
   return amax >= 0x1p-100f && amax < INFINITY && amax_y >= 1e-10f && amax_y < INFINITY;
 }
 
-// 8192 rows of 8192 bf16 with a residual, 470 MB: 83 us, 5.7 TB/s, above the rate of a large copy; 32
+// 8192 rows of 8192 bf16 with a residual, 470 MB: 75 us, 6.3 TB/s, above the rate of a large copy; 32
 // rows of 7168 with group scales: 4.6 us of the kernel, one row's chain of load, sum, amax.
 //
 // One workgroup of NT threads per row, the row's h in VPT 16-byte vectors' worth of fp32 a
@@ -109,7 +120,12 @@ __device__ inline bool short_way(float amax, float amax_y) {
 // element (none for 16-bit inputs without a residual) where y has two, and the amax is joined
 // behind the same barrier as the sum of squares. Scales are s = rstd amax / 448. Of the 67
 // million codes above 91 are not those of exact arithmetic, 1234 by way of y.
-template <typename T, int MODE, int NT, int VPT>
+//
+// Where a call's operands pass what the last-level cache holds, the row is read past the caches
+// (ONCE), which then keep the outputs that the next kernel reads: 83 us become 75. Below that x
+// may still lie in the cache of the kernel that wrote it: 4096 rows of 8192 without a residual
+// take 20 us, 24 past the caches.
+template <typename T, int MODE, int NT, int VPT, bool ONCE>
 __global__ __launch_bounds__(NT) void rms_quant_vec_kernel(
     const typename T::storage* __restrict__ x, int64_t ldx, const typename T::storage* __restrict__ res, int64_t ldr,
     const void* __restrict__ w, int w_dtype, float eps, int64_t k, int log_gl, uint8_t* __restrict__ q,
@@ -126,12 +142,12 @@ __global__ __launch_bounds__(NT) void rms_quant_vec_kernel(
     const int v = tid + i * NT;
     if (v < nvec) load_weight<V>(w, w_dtype, (int64_t)v * V, wv[i]);
   }
-  uint4 raw[VPT], more[VPT];
+  uint4 raw[VPT], more[VPT];  // + 0 below, where there is no residual
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = tid + i * NT;
-    raw[i] = v < nvec ? xr[v] : uint4{};
-    more[i] = res && v < nvec ? rr[v] : uint4{};  // + 0 below, where there is none
+    raw[i] = v < nvec ? load_vec<ONCE>(xr + v) : uint4{};
+    more[i] = res && v < nvec ? load_vec<ONCE>(rr + v) : uint4{};
   }
   uint32_t bits[VPT] = {};
 #pragma unroll
@@ -312,30 +328,40 @@ int launch(const void* x, int64_t rows, int64_t k, int64_t ldx, const void* res,
   int log_gl = 0;
   while ((int64_t)2 << log_gl <= gl) ++log_gl;
   const dim3 grid((unsigned)rows);
-#define AYK_RV(MODE, NT, VPT)                                                                                             \
-  hipLaunchKernelGGL((rms_quant_vec_kernel<T, MODE, NT, VPT>), grid, dim3(NT), 0, st, xs, ldx, rs, ldr, w, w_dtype, eps, k, \
-                     log_gl, qb, scale, srs, sgs, ro)
-#define AYK_RM(NT, VPT)                                                                    \
+  const bool once = rows * k * (int64_t)((res ? 3 : 1) * sizeof(S) + 1) > kLastLevelCache;
+#define AYK_RV(MODE, NT, VPT, ONCE)                                                                                      \
+  hipLaunchKernelGGL((rms_quant_vec_kernel<T, MODE, NT, VPT, ONCE>), grid, dim3(NT), 0, st, xs, ldx, rs, ldr, w, w_dtype, \
+                     eps, k, log_gl, qb, scale, srs, sgs, ro)
+#define AYK_RO(NT, VPT, ONCE)                                                              \
   do {                                                                                     \
-    if (mode == kScaleRow) AYK_RV(kScaleRow, NT, VPT);                                     \
-    else if (mode == kScaleGroup) AYK_RV(kScaleGroup, NT, VPT);                            \
-    else AYK_RV(kScaleMx, NT, VPT);                                                        \
+    if (mode == kScaleRow) AYK_RV(kScaleRow, NT, VPT, ONCE);                               \
+    else if (mode == kScaleGroup) AYK_RV(kScaleGroup, NT, VPT, ONCE);                      \
+    else AYK_RV(kScaleMx, NT, VPT, ONCE);                                                  \
     note_plan("rms_quant vec " #NT "x" #VPT);                                              \
     return check_launch("rms_norm_quant_fp8");                                             \
   } while (0)
+#define AYK_RF(NT, VPT) AYK_RO(NT, VPT, false)  // few rows
+#define AYK_RM(NT, VPT) do { if (once) AYK_RO(NT, VPT, true); AYK_RO(NT, VPT, false); } while (0)
   if (vec) {
     // Few rows leave CUs idle, so a row takes one vector a thread. Many rows keep two a thread in
-    // flight: 8192 rows of 8192 take 83 us so, 91 with four and 86 with one in 1024 threads; 4096
-    // without a residual 20.2, 21.2 and 27.5.
+    // flight: through the caches 8192 rows of 8192 take 83 us so, 91 with four
+    // and 86 with one in 1024 threads; 4096 without a residual 20.2, 21.2 and 27.5.
     const bool few = rows <= 512;
+    if (few) {
+      if (nvec <= 64) AYK_RF(64, 1);
+      if (nvec <= 256) AYK_RF(256, 1);
+      if (nvec <= 1024) AYK_RF(1024, 1);
+    }
     if (nvec <= 64) AYK_RM(64, 1);
-    if (nvec <= 128 && !few) AYK_RM(64, 2);
-    if (nvec <= 256) { if (few) AYK_RM(256, 1); else AYK_RM(128, 2); }
-    if (nvec <= 512 && !few) AYK_RM(256, 2);
-    if (nvec <= 1024) { if (few) AYK_RM(1024, 1); else AYK_RM(512, 2); }
+    if (nvec <= 128) AYK_RM(64, 2);
+    if (nvec <= 256) AYK_RM(128, 2);
+    if (nvec <= 512) AYK_RM(256, 2);
+    if (nvec <= 1024) AYK_RM(512, 2);
     if (nvec <= 2048) AYK_RM(1024, 2);
     AYK_RM(1024, 4);
   }
+#undef AYK_RF
+#undef AYK_RO
 #undef AYK_RM
 #undef AYK_RV
 #define AYK_RS(MODE)                                                                                                    \

@@ -63,3 +63,20 @@ def test_infinite_products_of_finite_rows(gpu):
     rest = [0, 2, 3, 4, 5, 6, 7]
     assert torch.equal(s[:, rest], s2.cpu()[:, rest])
     assert torch.equal(q.float().view(4, 8, 64)[:, rest], q2.cpu().float().view(4, 8, 64)[:, rest])
+
+
+@pytest.mark.parametrize("rows,k,dtype,group", [(8192, 8192, BF16, 0), (20000, 2048, BF16, 128), (4500, 8192, F32, 32), (45000, 1000, F16, 0)])
+def test_large_calls_row_by_row(gpu, rows, k, dtype, group):
+    """Operands larger than the caches: a row's results are those of a smaller call, bit for bit."""
+    from ayaka.kernel.hip import add_rms_norm_quant_fp8
+
+    _say(f"large {rows}x{k} {dtype} group={group}")
+    g = torch.Generator(device=gpu).manual_seed(15)
+    x, res = (torch.randn(rows, k, generator=g, device=gpu).to(dtype) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(k, generator=g, device=gpu)).to(dtype)
+    full = add_rms_norm_quant_fp8(x, res, w, EPS, group_size=group)
+    pick = torch.arange(0, rows, max(1, rows // 601), device=gpu)
+    assert pick.numel() > 512
+    part = add_rms_norm_quant_fp8(x[pick], res[pick], w, EPS, group_size=group)
+    for a, b in zip(full, part):
+        assert torch.equal(a[pick].view(torch.uint8), b.view(torch.uint8))
