@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kRowThreads) void varlen_rows_kernel(Packed q, Pack
 // cross lanes, a row's maximum and sum are within a lane but for one swap of halves, and V is
 // read transposed from LDS (ds_read_b64_tr_b16).
 //
-// 8192 causal positions of 64 heads of 128 bf16 dims, 1.10 TFLOP: 1.02 ms, 1.08 PFLOP/s, 76% of
+// 8192 causal positions of 64 heads of 128 bf16 dims, 1.10 TFLOP: 1.03 ms, 1.07 PFLOP/s, 75% of
 // what a bf16 product of 8192^3 reaches on this card. Both hold the power limit: with zeros
 // for inputs the same launch runs at 2.4 GHz instead of 1.9 and takes 0.77 ms. There the matrix
 // units are busy 58% of the time; three waves a SIMD hide most of the exponentials, the LDS
