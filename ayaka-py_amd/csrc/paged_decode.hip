@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_decode_rows_kernel(
 // is byte permutes within the lane).
 //
 // Bound by HBM where the cache read is long (64 sequences of 8192, 4 kv heads of 128 bf16 dims:
-// 1.07 GB in 199 us, 5.4 TB/s, the rate of a large read on this card); 131072 e4m3 positions of
+// 1.07 GB in 197 us, 5.5 TB/s, the rate of a large read on this card); 131072 e4m3 positions of
 // 8 kv heads, 268 MB, take 63 us: 50 of the read and the rest of the second launch and the
 // start. A wave has one block's K and V in flight (8 KB at 128 e4m3 dims), asked for as soon as
 // the registers of the block before are free.
@@ -81,7 +81,7 @@ struct DecodeArgs {
   uint32_t row_bytes;
   int longest, window, sinks;                       // longest: what a row of the table can name
   int batch, heads, kv_items, group, tiles, rows;  // kv heads or pairs, tiles of 16 heads in a group, columns in use
-  int q_aligned, dim;
+  int q_aligned, dim, once;
   float scale_log2, v_scale;
 };
 
@@ -126,25 +126,30 @@ __device__ inline int k_dim(int s, int quad) {
   if constexpr (Shape<CT, D>::kFp8) return s < 2 * (D / 64) ? 64 * (s / 2) + 16 * quad + 8 * (s % 2) : 64 * (D / 64) + 8 * quad;
   else return 32 * s + 8 * quad;
 }
-// 16 or 8 bytes, or zeros for dims past the head's.
-template <typename T>
+// 16 or 8 bytes, or zeros for dims past the head's. ONCE: past the caches.
+template <bool ONCE, typename T>
 __device__ inline T load_or_zero(const uint8_t* p, bool on) {
   T v{};
-  if (on) v = *reinterpret_cast<const T*>(p);
+  if constexpr (ONCE && sizeof(T) >= 8) {
+    typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) / 4)));
+    if (on) v = __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+  } else {
+    if (on) v = *reinterpret_cast<const T*>(p);
+  }
   return v;
 }
-template <int CT, int D, bool EXACT>
+template <int CT, int D, bool EXACT, bool ONCE>
 __device__ inline void load_k_row(const uint8_t* row, int quad, int dim, uint32_t* w) {
   if constexpr (Shape<CT, D>::kFp8) {
 #pragma unroll
     for (int j = 0; j < D / 64; ++j)
-      *reinterpret_cast<v4u*>(w + 4 * j) = load_or_zero<v4u>(row + 64 * j + 16 * quad, EXACT || 64 * j + 16 * quad < dim);
+      *reinterpret_cast<v4u*>(w + 4 * j) = load_or_zero<ONCE, v4u>(row + 64 * j + 16 * quad, EXACT || 64 * j + 16 * quad < dim);
     if constexpr (D % 64)
-      *reinterpret_cast<uint2*>(w + 4 * (D / 64)) = load_or_zero<uint2>(row + 64 * (D / 64) + 8 * quad, EXACT || 64 * (D / 64) + 8 * quad < dim);
+      *reinterpret_cast<uint2*>(w + 4 * (D / 64)) = load_or_zero<ONCE, uint2>(row + 64 * (D / 64) + 8 * quad, EXACT || 64 * (D / 64) + 8 * quad < dim);
   } else {
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
-      *reinterpret_cast<v4u*>(w + 4 * s) = load_or_zero<v4u>(row + 64 * s + 16 * quad, EXACT || 32 * s + 8 * quad < dim);
+      *reinterpret_cast<v4u*>(w + 4 * s) = load_or_zero<ONCE, v4u>(row + 64 * s + 16 * quad, EXACT || 32 * s + 8 * quad < dim);
   }
 }
 template <int CT, int QT, int D>
@@ -183,18 +188,18 @@ struct DimOrder {  // dim of column c: base[t] + c width[t]
     }
   }
 };
-template <int CT, int D, bool EXACT, int AT = 0>
+template <int CT, int D, bool EXACT, bool ONCE, int AT = 0>
 __device__ inline void load_v_row(const uint8_t* row, int col, int dim, uint32_t* w) {
   if constexpr (AT < D / 16) {
     constexpr int e = Shape<CT, D>::kElem, size = v_piece<CT, D>(AT), bytes = size * e;
     const uint8_t* p = row + (16 * AT + col * size) * e;
     const bool on = EXACT || 16 * AT + col * size < dim;
     uint32_t* d = w + AT * e / 4;
-    if constexpr (bytes == 16) *reinterpret_cast<v4u*>(d) = load_or_zero<v4u>(p, on);
-    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(d) = load_or_zero<uint2>(p, on);
-    else if constexpr (bytes == 4) *d = load_or_zero<uint32_t>(p, on);
-    else *d = load_or_zero<uint16_t>(p, on);
-    load_v_row<CT, D, EXACT, AT + size>(row, col, dim, w);
+    if constexpr (bytes == 16) *reinterpret_cast<v4u*>(d) = load_or_zero<ONCE, v4u>(p, on);
+    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(d) = load_or_zero<ONCE, uint2>(p, on);
+    else if constexpr (bytes == 4) *d = load_or_zero<ONCE, uint32_t>(p, on);
+    else *d = load_or_zero<ONCE, uint16_t>(p, on);
+    load_v_row<CT, D, EXACT, ONCE, AT + size>(row, col, dim, w);
   }
 }
 
@@ -229,7 +234,7 @@ struct Column {
   __device__ int head(const DecodeArgs& a, int g, int tile) const { return (g * PACK + sub) * a.group + tile * kHeadTile + at; }
 };
 
-template <int QT, int CT, int D, int PACK, bool EXACT, int WAVES>
+template <int QT, int CT, int D, int PACK, bool EXACT, int WAVES, bool ONCE>
 __device__ inline void attend_blocks(const DecodeArgs& a, int b, int len, int g, int tile, int from, int to, Running<D>& r) {
   using S = Shape<CT, D>;
   constexpr int PT = S::kFp8 ? AYK_F16 : QT;  // e4m3 and e5m2 are exact in fp16, whose weights round finer
@@ -283,14 +288,14 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int len, int g,
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int at = __builtin_amdgcn_ds_bpermute(4 * col + 64 * t, slot);
-      load_k_row<CT, D, EXACT>(a.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, quad, a.dim, kw[t]);
+      load_k_row<CT, D, EXACT, ONCE>(a.k + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, quad, a.dim, kw[t]);
     }
   };
   auto issue_v = [&](int slot) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int at = __builtin_amdgcn_ds_bpermute(16 * quad + 64 * (j / 4) + 4 * (j % 4), slot);
-      load_v_row<CT, D, EXACT>(a.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, col, a.dim, vw[j]);
+      load_v_row<CT, D, EXACT, ONCE>(a.v + (uint64_t)(uint32_t)(at < 0 ? 0 : at) * a.row_bytes + head_at, col, a.dim, vw[j]);
     }
   };
   // The next block's K is asked for as soon as this block's is used up, and V likewise, so
@@ -462,7 +467,7 @@ __global__ __launch_bounds__(WAVES * kWave, (Shape<CT, D>::kWavesPerSimd)) void 
   __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_blocks<QT, CT, D, PACK, EXACT, WAVES>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
+  attend_blocks<QT, CT, D, PACK, EXACT, WAVES, false>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
   join_waves<D, WAVES>(r, lds);
   if (threadIdx.x < kWave) write_item<QT, CT, D, PACK, EXACT>(a, b, g, tile, r, nullptr);
 }
@@ -480,7 +485,7 @@ __device__ inline int total_steps(const DecodeArgs& a) {
 // ones to every workgroup, whatever the lengths. A run may end one item, hold some whole and
 // begin another; what it does not hold whole it leaves as a partial result, in slot 0 (the run
 // begins inside the item) or slot 1 (it ends inside).
-template <int QT, int CT, int D, int PACK, bool EXACT>
+template <int QT, int CT, int D, int PACK, bool EXACT, bool ONCE>
 __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void paged_decode_split_kernel(DecodeArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
   const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
@@ -504,7 +509,7 @@ __global__ __launch_bounds__(kDecodeThreads, (Shape<CT, D>::kWavesPerSimd)) void
       const int last = first + (end - at) < steps ? first + (end - at) : steps;
       Running<D> r;
       const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
-      attend_blocks<QT, CT, D, PACK, EXACT, 4>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
+      attend_blocks<QT, CT, D, PACK, EXACT, 4, ONCE>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
       join_waves<D, 4>(r, lds);
       float* partial = nullptr;
       if (first > 0 || last < steps)
@@ -590,6 +595,12 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(Decode
 bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AYK_E4M3 || dt == AYK_E5M2; }
 
 
+// A call whose table can name as much as the last-level cache holds finds little of it there and
+// reads K and V past the caches, which they would fill for nothing. Through them and past them,
+// us: 48 x 6000 of 4 kv heads of 256 bf16 dims 217 / 196, 160 x 4000 of 128 e4m3 dims (unequal)
+// 89 / 83; below, 4 x 8000 of 8 heads (67 MB) 23.4 / 25.5.
+constexpr int64_t kLastLevelCache = 256ll << 20;  // bytes
+
 constexpr int kMostRuns = 1024;  // workgroups of a split launch that the chip holds at once, at most
 
 template <int QT, int CT, int D, bool EXACT, int PACK = 1>
@@ -605,7 +616,13 @@ int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
     note_plan("paged_decode whole");
   } else {
     constexpr int runs = 256 * Shape<CT, D>::kWavesPerSimd;
-    hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK, EXACT>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    // Whole lines only: of others the two loads that share a line would both fetch it (1 x
+    // 100000 of 192 e4m3 dims 77 / 81 us, 32 x 4000 of 96 46 / 55).
+    constexpr bool kLines = EXACT && D * Shape<CT, D>::kElem % 128 == 0;
+    if (kLines && a.once)
+      hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK, EXACT, kLines>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    else
+      hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK, EXACT, false>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
     const int64_t rows = (int64_t)a.batch * a.heads;
     if (rows <= 256)
       hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 1, 16>), dim3((unsigned)a.batch, (unsigned)a.heads),
@@ -751,6 +768,7 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     const bool split = deals_out(batch, heads, kv_heads, dim, elem_size(cache_dtype), longest_of(most, window, sinks)) &&
                        workspace != nullptr && aligned16(workspace) &&
                        workspace_bytes >= ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
+    a.once = longest_of(most, window, sinks) >= kLastLevelCache / (2 * c.row_bytes) / batch;
     if (cache_dtype == AYK_E4M3)
       return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, pack, split, st);
     if (cache_dtype == AYK_E5M2)
