@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
       p[a.dim] = r.m;
       p[a.dim + 1] = l;
     }
-    if (r.m == -INFINITY) return;  // nothing seen: the join reads no sums
+    if (r.m == -INFINITY) return;  // nothing seen, or nothing but NaN (then l is NaN): the join reads no sums
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(kRowThreads) void varlen_join_kernel(VarlenArgs a) 
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 32));
   const float mine_f = mine_m == -INFINITY ? 0.0f : exp2_fast((mine_m - top) * a.scale_log2);
-  l = mine_m == -INFINITY ? 0.0f : mine_l * mine_f;
+  l = mine_l * mine_f;  // of a part that saw nothing 0; of one whose scores were all NaN, which leave no maximum, NaN
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 32);
   v4f acc[2] = {};
