@@ -89,9 +89,8 @@ __device__ inline void attend_row(const void* q, int64_t dim, const Visible& vis
   for (int w = 1; w < kRowWaves; ++w) top = fmaxf(top, stat[w][0]);
   float sum = 0.0f, o = 0.0f;
   for (int w = 0; w < kRowWaves; ++w) {
-    // a wave that saw nothing counts nothing, and a NaN maximum stays visible in sum
+    // a wave that saw nothing holds zeros; what is NaN stays so under a weight of 0
     const float f = stat[w][0] == -INFINITY ? 0.0f : expf(stat[w][0] - top);
-    if (f == 0.0f) continue;
     sum += f * stat[w][1];
     if ((int)threadIdx.x < dim) o += f * part[w][threadIdx.x];
   }
