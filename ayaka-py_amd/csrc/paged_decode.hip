@@ -348,7 +348,10 @@ __device__ inline void attend_blocks(const DecodeArgs& a, int b, int len, int g,
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) r.acc[t] *= keep;
     }
-    const float base = r.m == -INFINITY ? 0.0f : r.m;  // nothing visible so far weighs 0
+    // Weights are at most 1, which fp16 would hold down to 2^-25: scaled up by 2^15, with their sum,
+    // they keep 15 bits more (a first token may take nearly all weight, and hold little).
+    constexpr float kShift = PT == AYK_F16 ? 15.0f : 0.0f;
+    const float base = r.m == -INFINITY ? 0.0f : r.m - kShift;  // nothing visible so far weighs 0
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       x[j] = exp2_fast(x[j] - base);

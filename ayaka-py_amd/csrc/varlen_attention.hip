@@ -228,8 +228,13 @@ struct RunningRows {
   v16f acc[D / 32];
 };
 
-// The weights of a tile, from its scores; s becomes exp2(scale (s - m)).
-template <int D, int U>
+// The weights of a tile, from its scores; s becomes exp2(scale (s - m) + shift).
+//
+// fp16 holds 2^-24 to 2^15 and weights reach 2^8 before the maximum moves, so they are scaled up
+// by 2^7 (the sum of weights with them): what is 2^-25 of the largest weight and less rounded
+// to nothing while the sum counted it, which left a row whose first token takes nearly all
+// weight, and holds little, without the others' part. bf16 has the exponents of fp32.
+template <int DT, int D, int U>
 __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
   // The chain starts with an operation that the compiler knows to read the products' results:
   // it waits for them, which it would not for the assembly of max3 alone.
@@ -247,7 +252,12 @@ __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) r.acc[t] *= keep;
   }
-  const float base = r.m == -INFINITY ? 0.0f : r.m * c;
+  constexpr float shift = DT == AYK_F16 ? 7.0f : 0.0f;
+  float base = 0.0f;
+  {
+#pragma clang fp contract(off)  // a fused form would hold the shift in a register: 129, three waves a SIMD instead of four
+    if (r.m != -INFINITY) base = r.m * c - shift;
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -402,7 +412,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
           else s[u][e] = at + n < end && (at + n >= first || at + n < kept) ? s[u][e] : -INFINITY;
         }
     }
-    softmax_tile<D, kSub>(r, s, a.scale_log2);
+    softmax_tile<DT, D, kSub>(r, s, a.scale_log2);
     v4u p[KEYS / 16];
 #pragma unroll
     for (int k = 0; k < KEYS / 16; ++k)
