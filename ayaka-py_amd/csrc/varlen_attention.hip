@@ -82,7 +82,7 @@ struct VarlenArgs {
   int64_t total_q, total_k, window, sinks;
   uint16_t* out;
   int batch, heads, group, dim, tiles, causal;
-  float scale, scale_log2;  // scale_log2 is positive; the sign is folded into Q
+  float scale_log2;         // positive; the sign is folded into Q
   uint32_t q_flip, q_keep;  // xor and mask of Q's bits: the scale's sign, or a zero scale
   int splits;               // parts of the keys, a workgroup each, joined from `partial`
   float* partial;           // [total_q][heads][splits][dim + 4]: sums, maximum, sum of weights
@@ -142,42 +142,6 @@ __device__ inline int k_swizzle(int row) { return D % 128 == 0 ? row & 15 : (row
 template <int D>
 __device__ inline int v_swizzle(int row) { return D % 128 == 0 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
 
-// One query row by one wave, position by position: what is hidden is never touched. For rows
-// whose sums came out NaN though their weights did not: a value that is not finite stood at a
-// position that the row must not see, and a product with a weight of 0 spread it (or the row
-// does see one).
-template <int DT>
-__device__ void attend_row_wave(const uint16_t* q, int dim, const Visible& vis, const uint16_t* k, int64_t k_row, const uint16_t* v,
-                                int64_t v_row, float scale, uint16_t* out) {
-  constexpr int kPer = kMaxDim / kWave;
-  const int lane = threadIdx.x % kWave;
-  float qv[kPer], acc[kPer], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    qv[i] = lane + i * kWave < dim ? load_elem<DT>(q, lane + i * kWave) * scale : 0.0f;
-    acc[i] = 0.0f;
-  }
-  for (int64_t j = 0; j < vis.end; ++j) {
-    if (j >= vis.sinks && j < vis.first) j = vis.first;
-    if (!vis(j)) break;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane + i * kWave < dim) s += qv[i] * load_elem<DT>(k, j * k_row + lane + i * kWave);
-    s = wave_sum_dpp(s);
-    if (s == -INFINITY) continue;
-    const float top = s != s ? s : fmaxf(m, s), keep = expf(m - top), p = expf(s - top);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane + i * kWave < dim) acc[i] = acc[i] * keep + p * load_elem<DT>(v, j * v_row + lane + i * kWave);
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (lane + i * kWave < dim) store_f32(out, DT, lane + i * kWave, l == 0.0f ? 0.0f : acc[i] / l);
-}
-
 // The tile that is number `rank` of all from the longest on: the tile of a sequence's rows
 // t R .. sees (ahead + (t + 1) R) / KEYS tiles of keys, so a packed batch in its own order would
 // end with some workgroups at the longest tiles and the chip idle (8 prompts of 350 to 1500:
@@ -228,12 +192,21 @@ struct RunningRows {
   v16f acc[D / 32];
 };
 
-// The weights of a tile, from its scores; s becomes exp2(scale (s - m) + shift).
+// What a weight's exponent is counted from: a score s under maximum m weighs exp2(c s - base), with
+// c = scale log2(e).
 //
 // fp16 holds 2^-24 to 2^15 and weights reach 2^8 before the maximum moves, so they are scaled up
 // by 2^7 (the sum of weights with them): what is 2^-25 of the largest weight and less rounded
 // to nothing while the sum counted it, which left a row whose first token takes nearly all
 // weight, and holds little, without the others' part. bf16 has the exponents of fp32.
+template <int DT>
+__device__ inline float weight_base(float m, float c) {
+#pragma clang fp contract(off)  // a fused form would hold the shift in a register: at 64 dims the 129th, three waves a SIMD instead of four
+  constexpr float shift = DT == AYK_F16 ? 7.0f : 0.0f;
+  return m == -INFINITY ? 0.0f : m * c - shift;
+}
+
+// The weights of a tile, from its scores: s becomes exp2(c s - base).
 template <int DT, int D, int U>
 __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
   // The chain starts with an operation that the compiler knows to read the products' results:
@@ -252,12 +225,7 @@ __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) r.acc[t] *= keep;
   }
-  constexpr float shift = DT == AYK_F16 ? 7.0f : 0.0f;
-  float base = 0.0f;
-  {
-#pragma clang fp contract(off)  // a fused form would hold the shift in a register: 129, three waves a SIMD instead of four
-    if (r.m != -INFINITY) base = r.m * c - shift;
-  }
+  const float base = weight_base<DT>(r.m, c);
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -280,6 +248,13 @@ __device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lds, ui
 }
 __device__ inline uint32_t lds_address(const uint8_t* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
+}
+
+// This lane's number in its wave, in a form that holds no register before its use.
+__device__ inline int lane_number() {
+  int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
 template <int DT, int D, int KEYS>
@@ -437,33 +412,37 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
     if (i + 1 < to) turn(i + 1, 1);
   }
 
-  const float l = sum_halves(r.l);
-  if (a.splits > 1) {
-    if (w0 + row >= len_q) return;
-    float* p = a.partial + (((sq.q0 + w0 + row) * a.heads + head) * a.splits + part) * (a.dim + 4);
-    if (half == 0) {
-      p[a.dim] = r.m;
-      p[a.dim + 1] = l;
-    }
-    if (r.m == -INFINITY) return;  // nothing seen, or nothing but NaN (then l is NaN): the join reads no sums
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (32 * t + 8 * e < a.dim)
-          *reinterpret_cast<v4f*>(p + 32 * t + 8 * e + 4 * half) = v4f{r.acc[t][4 * e], r.acc[t][4 * e + 1], r.acc[t][4 * e + 2], r.acc[t][4 * e + 3]};
-    return;
-  }
-  const float f = l == 0.0f ? 0.0f : 1.0f / l;
-  float odd = 0.0f;
+  // The lane's numbers, anew: kept over the loop, their registers would decide how many workgroups
+  // share a CU.
+  const int lane_now = lane_number(), half_now = lane_now / 32, row_now = lane_now % 32;
+  const int64_t row_at = w0 + row_now < len_q ? w0 + row_now : len_q - 1;
+  const float l = sum_halves(r.l), f = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  float nan = 0.0f;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) odd = r.acc[t][e] != r.acc[t][e] ? NAN : odd;
-  uint64_t again = __ballot(odd != odd && l == l && w0 + row < len_q);
-  {
+    for (int e = 0; e < 16; ++e) nan = r.acc[t][e] != r.acc[t][e] ? NAN : nan;
+  const bool live = w0 + row_now < len_q;
+  uint64_t odd = __ballot(nan != nan && l == l && live);
+  odd |= odd >> 32 | odd << 32;
+  const bool is_odd = odd >> lane_now & 1, write = live && !is_odd;
+  uint16_t* row_out = a.out + ((sq.q0 + row_at) * a.heads + head) * a.dim;
+  float* part_of = a.partial + (((sq.q0 + row_at) * a.heads + head) * a.splits + part) * (a.dim + 4);
+  if (a.splits > 1) {
+    if (live && half_now == 0) {
+      part_of[a.dim] = r.m;
+      part_of[a.dim + 1] = l;
+    }
+    if (write && r.m != -INFINITY) {  // else nothing seen, or nothing but NaN (then l is NaN): the join reads no sums
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (32 * t + 8 * e < a.dim)
+            *reinterpret_cast<v4f*>(part_of + 32 * t + 8 * e + 4 * half_now) = v4f{r.acc[t][4 * e], r.acc[t][4 * e + 1], r.acc[t][4 * e + 2], r.acc[t][4 * e + 3]};
+    }
+  } else {
     // Runs of eight dims lie half in lane l and half in l + 32: of two runs each lane gets one.
-    uint16_t* o = a.out + ((sq.q0 + my_row) * a.heads + head) * a.dim + 8 * half;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -476,14 +455,82 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
           run[w] = pair[0];
           run[2 + w] = pair[1];
         }
-        if (w0 + row < len_q && 32 * t + 8 * e + 8 * half < a.dim) *reinterpret_cast<v4u*>(o + 32 * t + 8 * e) = run;
+        if (write && 32 * t + 8 * e + 8 * half_now < a.dim) *reinterpret_cast<v4u*>(row_out + 32 * t + 8 * e + 8 * half_now) = run;
       }
   }
-  again |= again >> 32;
-  for (again &= 0xFFFFFFFFull; again; again &= again - 1) {
-    const int64_t i = w0 + __builtin_ctzll(again);
-    attend_row_wave<DT>(a.q.p + (sq.q0 + i) * a.q.row + head * a.q.head, a.dim, visible_to(i + ahead, len_k, a.causal, a.window, a.sinks),
-                        kp, a.k.row, vp, a.v.row, a.scale, a.out + ((sq.q0 + i) * a.heads + head) * a.dim);
+  if (!odd) return;
+
+  // Rows whose sums came out NaN though their weights did not: a value that is not finite stood
+  // at a position that the row must not see, and a product with a weight of 0 spread it (or the row
+  // does see one). The wave takes its keys again under the maxima and sums that it has, from memory
+  // and 32 dims at a time (with more of them this part, not the loop above, would decide the
+  // registers). Values that are not finite count 0 in the product; where a row sees them,
+  // +infinity or NaN and -infinity or NaN, products of ones tell. 8192 positions of 64 heads with
+  // NaN everywhere: 14 ms.
+  const float base = weight_base<DT>(r.m, a.scale_log2);
+  constexpr uint32_t kInf = DT == AYK_BF16 ? 0x7F80u : 0x7C00u, kOne = DT == AYK_BF16 ? 0x3F80u : 0x3C00u;
+  for (int d0 = 0; d0 < a.dim; d0 += 32) {
+    v16f acc = {};
+    for (int b = from * kSub; b < to * kSub; ++b) {
+      const int key = tl.at(b / kSub) * KEYS + 32 * (b % kSub);
+      if (key >= any_end || (key + 32 <= any_first && key >= any_kept)) continue;
+      v16f s = {};
+      const int64_t most = len_k - 1, kr = key + row_now < most ? key + row_now : most;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const v4u k = 16 * d + 8 * half_now < a.dim ? *reinterpret_cast<const v4u*>(kp + kr * a.k.row + 16 * d + 8 * half_now) : v4u{0, 0, 0, 0};
+        s = mfma32<DT>(k, qf[d], s);
+        if (d % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+      v4u p[2], seen[2];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float x[2];
+        uint32_t ones = 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int j = key + 8 * (e / 4) + 4 * half_now + e % 4 + c;
+          const bool on = j < end && (j >= first || j < kept) && s[e + c] != -INFINITY;
+          x[c] = on ? exp2_fast(fmaf(s[e + c], a.scale_log2, -base)) : 0.0f;
+          ones |= on ? kOne << 16 * c : 0u;
+        }
+        p[e / 8][e % 8 / 2] = pack2<DT>(x[0], x[1]);
+        seen[e / 8][e % 8 / 2] = ones;
+      }
+      const int dim = d0 + row_now;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        v4u v{0, 0, 0, 0}, up{0, 0, 0, 0}, down{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int64_t j = key + 16 * k + 8 * (e / 4) + 4 * half_now + e % 4;
+          const uint32_t bits = dim < a.dim ? vp[(j < most ? j : most) * a.v.row + dim] : 0u, size = bits & 0x7FFFu;
+          v[e / 2] |= (size < kInf ? bits : 0u) << 16 * (e % 2);
+          up[e / 2] |= (size > kInf || bits == kInf ? kOne : 0u) << 16 * (e % 2);
+          down[e / 2] |= (size > kInf || bits == (kInf | 0x8000u) ? kOne : 0u) << 16 * (e % 2);
+        }
+        acc = mfma32<DT>(v, p[k], acc);
+        auto add = [&](v4u where, float what) {
+          if (!__ballot(where[0] | where[1] | where[2] | where[3])) return;
+          const v16f times = mfma32<DT>(where, seen[k], v16f{});
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[e] += times[e] > 0.0f ? what : 0.0f;
+        };
+        add(up, INFINITY);
+        add(down, -INFINITY);
+      }
+    }
+    if (is_odd) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = d0 + 8 * e + 4 * half_now;
+        const v4f four = v4f{acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]} * f;
+        if (at >= a.dim) continue;
+        if (a.splits > 1) *reinterpret_cast<v4f*>(part_of + at) = four;
+        else *reinterpret_cast<uint2*>(row_out + at) = make_uint2(pack2<DT>(four[0], four[1]), pack2<DT>(four[2], four[3]));
+      }
+    }
   }
 }
 
@@ -492,7 +539,7 @@ template <int DT>
 __global__ __launch_bounds__(kRowThreads) void varlen_join_kernel(VarlenArgs a) {
   const int lane = threadIdx.x % 32;
   const int64_t all = a.total_q * a.heads, mine = (int64_t)blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32;
-  const int64_t at = mine < all ? mine : all - 1;  // no lane leaves: the wave may search below
+  const int64_t at = mine < all ? mine : all - 1;  // no lane leaves: its neighbours read it below
   const int width = a.dim + 4;
   const float* p = a.partial + at * a.splits * width;
   const float mine_m = lane < a.splits ? p[lane * width + a.dim] : -INFINITY;  // kMostSplits <= 32
@@ -500,7 +547,8 @@ __global__ __launch_bounds__(kRowThreads) void varlen_join_kernel(VarlenArgs a) 
   float top = mine_m, l;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 32));
-  const float mine_f = mine_m == -INFINITY ? 0.0f : exp2_fast((mine_m - top) * a.scale_log2);
+  float mine_f = mine_m == -INFINITY ? 0.0f : exp2_fast((mine_m - top) * a.scale_log2);
+  if (mine_m != -INFINITY && mine_f < 0x1p-126f) mine_f = 0x1p-126f;  // an infinity seen weighs more than nothing
   l = mine_l * mine_f;  // of a part that saw nothing 0; of one whose scores were all NaN, which leave no maximum, NaN
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) l += __shfl_xor(l, off, 32);
@@ -517,26 +565,11 @@ __global__ __launch_bounds__(kRowThreads) void varlen_join_kernel(VarlenArgs a) 
   }
   uint16_t* o = a.out + at * a.dim;
   const float r = l == 0.0f ? 0.0f : 1.0f / l;
-  float odd = 0.0f;
 #pragma unroll
   for (int d = 0; d < 2; ++d) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) odd = acc[d][e] != acc[d][e] ? NAN : odd;
     const int dim = 128 * d + 4 * lane;
     if (dim < a.dim && mine < all)
       *reinterpret_cast<uint2*>(o + dim) = make_uint2(pack2<DT>(acc[d][0] * r, acc[d][1] * r), pack2<DT>(acc[d][2] * r, acc[d][3] * r));
-  }
-  const uint64_t again = __ballot(odd != odd && l == l && mine < all);
-  for (int h = 0; h < 2; ++h) {
-    if (!(again >> (32 * h) & 0xFFFFFFFFu)) continue;
-    const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + threadIdx.x / kWave * 2 + h, row = item / a.heads;
-    const int head = (int)(item % a.heads);
-    int b;
-    const Sequence sq = find_sequence(a, (int)row, [](int first, int) { return first; }, &b);
-    const int64_t len_k = sq.k1 - sq.k0, position = row - sq.q0 + len_k - (sq.q1 - sq.q0);
-    attend_row_wave<DT>(a.q.p + row * a.q.row + head * a.q.head, a.dim, visible_to(position, len_k, a.causal, a.window, a.sinks),
-                        a.k.p + sq.k0 * a.k.row + head / a.group * a.k.head, a.k.row, a.v.p + sq.k0 * a.v.row + head / a.group * a.v.head,
-                        a.v.row, a.scale, a.out + item * a.dim);
   }
 }
 
@@ -644,7 +677,6 @@ extern "C" int ayk_varlen_attention_split(const void* q, int64_t q_row_stride, i
     a.group = (int)(heads / kv_heads);
     a.dim = (int)dim;
     a.causal = causal;
-    a.scale = scale;
     a.scale_log2 = scale == 0.0f ? 1.0f : fabsf(scale) * kLog2e;
     a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
     a.q_keep = scale == 0.0f ? 0u : 0xFFFFFFFFu;
