@@ -36,6 +36,8 @@ __device__ inline float load_elem(const void* p, int64_t i) {
 constexpr int elem_size(int dt) { return dt == AYK_E4M3 || dt == AYK_E5M2 ? 1 : dt == AYK_F32 ? 4 : 2; }
 
 constexpr int kRowThreads = 256;
+// Workgroups of 256 threads along a grid's first dimension, at most: its work items are counted in 32 bits.
+constexpr int64_t kMostGroups = 0xFFFFFF;
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMaxDim = 256;
 

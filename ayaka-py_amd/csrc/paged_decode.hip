@@ -733,13 +733,13 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
   const PagedCache c{static_cast<const uint8_t*>(key_cache), static_cast<const uint8_t*>(value_cache), num_pages, page_size,
                      kv_heads * dim * elem_size(cache_dtype), block_tables, table_stride, table_width};
   const bool bf = q_dtype == AYK_BF16;
-  // The matrix kernels count positions, slots and items in 32 bits and load 16 bytes at a time.
+  // The matrix kernels count positions and slots in 32 bits and load 16 bytes at a time.
   const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
   const int pack = pack_of(heads, kv_heads, dim);
   const int64_t items = batch * tiles * (kv_heads / pack);
   if (matrix_dim(dim, cache_dtype) && aligned16(key_cache) && aligned16(value_cache) && most < 0x7FFFFF00 && num_pages > 0 &&
       num_pages * page_size < 0x7FFFFF00 && page_size < 0x7FFFFF00 && c.row_bytes < 0x7FFFFFFF &&
-      items < 0x7FFFFFFF) {
+      items <= kMostGroups) {
     DecodeArgs a{};
     a.q = static_cast<const uint16_t*>(q);
     a.q_row = q_row_stride;
@@ -778,6 +778,7 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
       return bf ? launch_dim<AYK_BF16, AYK_E5M2>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E5M2>(a, dim, pack, split, st);
     return bf ? launch_dim<AYK_BF16, AYK_BF16>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_F16>(a, dim, pack, split, st);
   }
+  if (batch > kMostGroups) return fail(AYK_EINVAL, "%s: the batch exceeds the grid of the row kernel", op);
   const dim3 grid((unsigned)batch, (unsigned)heads);
 #define AYK_PDR(Q, C)                                                                                                  \
   hipLaunchKernelGGL((paged_decode_rows_kernel<Q, C>), grid, dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(q), \

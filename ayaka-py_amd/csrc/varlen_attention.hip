@@ -660,7 +660,7 @@ extern "C" int ayk_varlen_attention_split(const void* q, int64_t q_row_stride, i
   };
   if (dim % 8 == 0 && rows16(q, q_row_stride, q_head_stride) && rows16(k, k_row_stride, k_head_stride) &&
       rows16(v, v_row_stride, v_head_stride) && aligned16(out) && batch < 0x1000000 &&
-      (total_q / kTileRows + batch + 2) * heads < 0x3FFFFFF) {
+      (total_q / kTileRows + batch + 2) * heads <= kMostGroups) {
     VarlenArgs a{};
     a.q = qp;
     a.k = kp;
@@ -686,6 +686,7 @@ extern "C" int ayk_varlen_attention_split(const void* q, int64_t q_row_stride, i
                    ? splits_of(a) : 1;
     return dtype == AYK_BF16 ? launch_dims<AYK_BF16>(a, st) : launch_dims<AYK_F16>(a, st);
   }
+  if (total_q > kMostGroups) return fail(AYK_EINVAL, "%s: rows exceed the grid of the row kernel", op);
   const dim3 grid((unsigned)total_q, (unsigned)heads);
 #define AYK_VAR(Q)                                                                                                     \
   hipLaunchKernelGGL((varlen_rows_kernel<Q>), grid, dim3(kRowThreads), 0, st, qp, kp, vp, starts_q, starts_k, batch,    \
