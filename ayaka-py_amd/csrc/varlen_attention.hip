@@ -669,8 +669,8 @@ extern "C" int ayk_varlen_attention_split(const void* q, int64_t q_row_stride, i
     a.starts_k = starts_k;
     a.total_q = total_q;
     a.total_k = total_k;
-    a.window = window;
-    a.sinks = sinks;
+    a.window = window < 0x7FFFFFFF ? window : 0x7FFFFFFF;  // beyond every position, and their sum stays in 64 bits
+    a.sinks = sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF;
     a.out = static_cast<uint16_t*>(out);
     a.batch = (int)batch;
     a.heads = (int)heads;
