@@ -4,8 +4,8 @@
 //   s_j = scale k_scale <q[b, h], K[slot(j), g]>,  p = softmax over the visible j,
 //   out[b, h] = v_scale sum_j p_j V[slot(j), g],   slot(j) = table[b][j / P] P + j % P
 //
-// with g = h / (heads / kv_heads). HBM-bound: every visible K and V row is read once for all
-// the query heads that share it.
+// with g = h / (heads / kv_heads). HBM-bound: every visible K and V row is read once for the
+// query heads that share it, sixteen at a time.
 #include "attn_frag.h"
 #include "attn_rows.h"
 
@@ -597,11 +597,14 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(Decode
 
 bool is_cache_dtype(int dt) { return dt == AYK_F16 || dt == AYK_BF16 || dt == AYK_E4M3 || dt == AYK_E5M2; }
 
-
-// A call whose table can name as much as the last-level cache holds finds little of it there and
+// A call whose table can name more than the last-level cache holds finds little of it there and
 // reads K and V past the caches, which they would fill for nothing. Through them and past them,
-// us: 48 x 6000 of 4 kv heads of 256 bf16 dims 217 / 196, 160 x 4000 of 128 e4m3 dims (unequal)
-// 89 / 83; below, 4 x 8000 of 8 heads (67 MB) 23.4 / 25.5.
+// us: 48 x 6000 of 4 kv heads of 256 bf16 dims 214 / 195, 160 x 4000 of 8 of 128 e4m3 dims (unequal)
+// 155 / 152. Around the border it matters little, and less than it costs a cache that holds
+// the rows: 1 x 131072 of 8 (256 MiB) 63 / 63, 32 x 4096 (unequal, 151 MB) 44 / 45 on rows that are
+// in no cache, 42 / 44 where part of them are. Rows that several tiles of heads read stay in the
+// caches: 64 heads over one of 128 e4m3 dims, 16 x 65536, 109 / 140; 128 over one of 256 bf16
+// dims, 8 x 131072, 631 / 1057.
 constexpr int64_t kLastLevelCache = 256ll << 20;  // bytes
 
 constexpr int kMostRuns = 1024;  // workgroups of a split launch that the chip holds at once, at most
@@ -622,7 +625,8 @@ int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
     // Whole lines only: of others the two loads that share a line would both fetch it (1 x
     // 100000 of 192 e4m3 dims 77 / 81 us, 32 x 4000 of 96 46 / 55).
     constexpr bool kLines = EXACT && D * Shape<CT, D>::kElem % 128 == 0;
-    if (kLines && a.once)
+    const bool once = kLines && a.once;
+    if (once)
       hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK, EXACT, kLines>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
     else
       hipLaunchKernelGGL((paged_decode_split_kernel<QT, CT, D, PACK, EXACT, false>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
@@ -636,7 +640,7 @@ int launch_matrix(const DecodeArgs& a, bool split, hipStream_t st) {
     else
       hipLaunchKernelGGL((paged_decode_join_kernel<QT, D / PACK, PACK, 4, 4>), dim3((unsigned)a.batch, (unsigned)cdiv(a.heads, 4)),
                          dim3(4 * kWave), 0, st, a, runs);
-    note_plan("paged_decode split");
+    note_plan(once ? "paged_decode split, past the caches" : "paged_decode split");
   }
   return check_launch("paged_decode_attention");
 }
@@ -771,7 +775,7 @@ int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride,
     const bool split = deals_out(batch, heads, kv_heads, dim, elem_size(cache_dtype), longest_of(most, window, sinks)) &&
                        workspace != nullptr && aligned16(workspace) &&
                        workspace_bytes >= ayk_paged_decode_attention_workspace_bytes(batch, heads, kv_heads, dim);
-    a.once = longest_of(most, window, sinks) >= kLastLevelCache / (2 * c.row_bytes) / batch;
+    a.once = tiles == 1 && longest_of(most, window, sinks) > kLastLevelCache / (2 * c.row_bytes) / batch;
     if (cache_dtype == AYK_E4M3)
       return bf ? launch_dim<AYK_BF16, AYK_E4M3>(a, dim, pack, split, st) : launch_dim<AYK_F16, AYK_E4M3>(a, dim, pack, split, st);
     if (cache_dtype == AYK_E5M2)
