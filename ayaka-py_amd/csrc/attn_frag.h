@@ -61,14 +61,18 @@ __device__ inline uint2 read_transposed(const uint8_t* lds) {
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The largest of three, NaN losing to numbers (fmaxf alone costs a canonicalization an operand).
-// The compiler does not count the wait that a read of a matrix product's result needs for an
-// assembly statement: at least one operand must come from another instruction that read the
-// same product's result.
-__device__ inline float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
+// The largest of a lane's scores in one or two products' results, NaN losing to numbers. v_max3 is
+// assembly, as fmaxf alone costs a canonicalization an operand. The compiler does not count the wait
+// that a read of a matrix product's result needs for an assembly statement; so the chain, every
+// link of which waits for the one before, begins with an fmaxf that reads both results.
+template <int U>
+__device__ inline float max_of_products(const v16f (&s)[U]) {
+  static_assert(U == 1 || U == 2, "the first fmaxf reads every product's result");
+  float top = fmaxf(s[0][14], s[U - 1][15]);
+#pragma unroll
+  for (int i = 0; i < 16; i += 3 - U)
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(top) : "v"(top), "v"(s[0][i]), "v"(U == 2 ? s[U - 1][i] : s[0][i + 1]));
+  return top;
 }
 
 // Maximum and sum over the lanes l, l ^ 32, and over l, l ^ 16, l ^ 32, l ^ 48.

@@ -209,12 +209,7 @@ __device__ inline float weight_base(float m, float c) {
 // The weights of a tile, from its scores: s becomes exp2(c s - base).
 template <int DT, int D, int U>
 __device__ inline void softmax_tile(RunningRows<D>& r, v16f (&s)[U], float c) {
-  // The chain starts with an operation that the compiler knows to read the products' results:
-  // it waits for them, which it would not for the assembly of max3 alone.
-  float top = fmaxf(s[0][14], s[U - 1][15]);
-#pragma unroll
-  for (int i = 0; i < 16; i += 3 - U) top = max3(top, s[0][i], U == 2 ? s[U - 1][i] : s[0][i + 1]);
-  top = max_halves(top);
+  const float top = max_halves(max_of_products(s));
   // The maximum moves only when a score beats it by 2^8: until then weights may reach 256,
   // which no sum or 16-bit type minds, and O need not be rescaled.
   if (__ballot((top - r.m) * c > 8.0f)) {
