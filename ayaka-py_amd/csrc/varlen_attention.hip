@@ -235,11 +235,14 @@ __device__ inline void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt
 
 // 16 bytes a lane from offset `at` of a buffer to lds + 16 lane, in assembly: the compiler
 // takes a transposed read of LDS to depend on every direct load in flight and would wait for
-// the next tile's before a tile's second product. The waits are the kernel's own (tile_barrier),
-// and there is no output register. The idle cycles are those that the write of m0, and of the
-// descriptor's registers by readfirstlane, need before a load reads them.
+// the next tile's before a tile's second product; a memory clobber would bring those waits back.
+// So nothing here orders the load with reads of LDS: those of the stage that it fills lie before
+// the tile_barrier in front of it or behind the next one, which every path to them passes. The
+// waits are the kernel's own (tile_barrier), and there is no output register. The idle cycles are those
+// that the write of m0, and of the descriptor's registers by readfirstlane, need before a load
+// reads them.
 __device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lds, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(at), "s"(from), "s"(lds));
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(at), "s"(from), "{m0}"(lds));
 }
 __device__ inline uint32_t lds_address(const uint8_t* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
