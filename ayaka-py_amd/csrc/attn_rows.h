@@ -45,9 +45,9 @@ constexpr int kMaxDim = 256;
 // turn, lane l of a wave the elements l, l + 64, ... of a row. `row_of(j, &k, &v)` gives the
 // addresses of position j's rows, or false where the position has none. The running
 // maximum and sum of the softmax are fp32, per wave, joined in LDS. Output 0 where nothing
-// is visible. For shapes the matrix kernels do not take (dims not a multiple of 16,
-// unaligned rows): one exp and 2 dim multiply-adds a position and query, no reuse of K or V
-// between the heads that share them.
+// is visible. For what the matrix kernels do not take (rows that are not whole 16-byte pieces or
+// not aligned to them, grids past their limits): one exp and 2 dim multiply-adds a position and query,
+// no reuse of K or V between the heads that share them.
 template <int QT, int CT, typename RowOf>
 __device__ inline void attend_row(const void* q, int64_t dim, const Visible& vis, RowOf row_of, float scale, float v_scale,
                                   void* out) {

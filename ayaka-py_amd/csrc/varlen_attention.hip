@@ -91,7 +91,7 @@ struct VarlenArgs {
 // Sequences 1 .. batch, and two without keys, 0 and batch + 1: the rows before the first
 // sequence and after the last, which give 0. find_sequence gives the last one whose order
 // key, order(first row, index), is at most `target`: every lane asks for one of 64 first
-// rows, so that a search is one round trip up to 62 sequences and two up to 3900.
+// rows, so that a search is one round trip up to 61 sequences and two up to 4030.
 template <typename Order>
 __device__ inline Sequence find_sequence(const VarlenArgs& a, int target, Order order, int* index) {
   const int lane = threadIdx.x % kWave;
@@ -146,7 +146,12 @@ __device__ inline int v_swizzle(int row) { return D % 128 == 0 ? (row & 3) << 2 
 // t R .. sees (ahead + (t + 1) R) / KEYS tiles of keys, so a packed batch in its own order would
 // end with some workgroups at the longest tiles and the chip idle (8 prompts of 350 to 1500:
 // 122 us). Lane b holds sequence b; the length at which the count of longer tiles passes `rank`
-// is found by bisection. Causal, at most 62 sequences; false past the last tile.
+// is found by bisection. Causal, at most kMostRanked sequences; false past the last tile.
+//
+// In their own order and in this one, us: 8 prompts of up to 1500 (32 heads of 128 dims) 107 / 99, 32 of
+// them 337 / 335, 61 of them 623 / 636. Many tiles fill the end by themselves, so that nothing is
+// lost past 61 sequences (64 of them: 646).
+constexpr int kMostRanked = kWave - 3;  // a lane for each, two for the rows around them and one for the end
 template <int R, int KEYS>
 __device__ inline bool find_ranked(const VarlenArgs& a, int rank, Sequence* sq, int* tile) {
   const int lane = threadIdx.x % kWave, b = lane < a.batch + 2 ? lane : a.batch + 2;
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void varlen_tile_kernel(VarlenArgs
   const int part = blockIdx.x / a.heads % a.splits, rank = blockIdx.x / a.heads / a.splits;
   Sequence sq;
   int tile;  // of the sequence
-  if (a.causal && a.batch > 1 && a.batch <= 61) {
+  if (a.causal && a.batch > 1 && a.batch <= kMostRanked) {
     if (!find_ranked<kRows, KEYS>(a, rank, &sq, &tile)) return;
   } else {
     int b;
