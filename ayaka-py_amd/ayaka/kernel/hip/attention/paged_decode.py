@@ -90,7 +90,9 @@ def paged_decode_attention(
         key_cache, value_cache: contiguous ``[pages, page_size, kv_heads, head_dim]``,
             e4m3fn / e5m2 or the query's dtype; ``heads`` is a multiple of ``kv_heads``.
         block_tables: int32 ``[batch, max_pages]``; entries past a sequence's last page are
-            not read, and the positions of a page outside the cache count as hidden.
+            not read, and the positions of a page outside the cache count as hidden. The launch
+            is chosen from the width: short sequences through a table for long ones take up
+            to 5 us more than through one of their own width.
         seq_lens: int32 ``[batch]``; 0 (padding rows) gives a zero output.
         softmax_scale: factor of the scores, ``head_dim ** -0.5`` as a rule.
         k_scale, v_scale: dequantization scales of an fp8 cache (the inverses of what

@@ -108,8 +108,9 @@ __device__ inline bool short_way(float amax, float amax_y) {
   return amax >= 0x1p-100f && amax < INFINITY && amax_y >= 1e-10f && amax_y < INFINITY;
 }
 
-// 8192 rows of 8192 bf16 with a residual, 470 MB: 75 us, 6.3 TB/s, above the rate of a large copy; 32
-// rows of 7168 with group scales: 4.6 us of the kernel, one row's chain of load, sum, amax.
+// 8192 rows of 8192 bf16 with a residual, 470 MB: 75 us of the kernel, 6.3 TB/s, above the rate of a
+// large copy; 75 to 83 us a call by what else runs. 32 rows of 7168 with group scales: 4.7 us of the
+// kernel, one row's chain of load, sum, amax.
 //
 // One workgroup of NT threads per row, the row's h in VPT 16-byte vectors' worth of fp32 a
 // thread: thread t holds vectors t, t + NT, ... 2^log_gl lanes, neighbours in one wave, hold a
@@ -122,9 +123,11 @@ __device__ inline bool short_way(float amax, float amax_y) {
 // million codes above 91 are not those of exact arithmetic, 1234 by way of y.
 //
 // Where a call's operands pass what the last-level cache holds, the row is read past the caches
-// (ONCE), which then keep the outputs that the next kernel reads: 83 us become 75. Below that x
-// may still lie in the cache of the kernel that wrote it: 4096 rows of 8192 without a residual
-// take 20 us, 24 past the caches.
+// (ONCE), which then keep the outputs that the next kernel reads. Through them and past them, us: 8192
+// rows of 8192 82 / 75, with UE8M0 scales 85 / 77, 4096 of 16384 85 / 76; nothing more where the
+// outputs alone pass the caches (16384 of 8192 162 / 164, 8192 of 8192 fp32 155 / 157). Below that x may
+// still lie in the cache of the kernel that wrote it: 4096 rows of 8192 without a residual take 20 us,
+// 24 past the caches.
 template <typename T, int MODE, int NT, int VPT, bool ONCE>
 __global__ __launch_bounds__(NT) void rms_quant_vec_kernel(
     const typename T::storage* __restrict__ x, int64_t ldx, const typename T::storage* __restrict__ res, int64_t ldr,

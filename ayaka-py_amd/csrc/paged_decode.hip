@@ -58,9 +58,8 @@ __global__ __launch_bounds__(kRowThreads) void paged_decode_rows_kernel(
 // is byte permutes within the lane).
 //
 // Bound by HBM where the cache read is long (64 sequences of 8192, 4 kv heads of 128 bf16 dims:
-// 1.07 GB in 197 us, 5.5 TB/s, the rate of a large read on this card); 131072 e4m3 positions of
-// 8 kv heads, 268 MB, take 63 us: 50 of the read and the rest of the second launch and the
-// start. A wave has one block's K and V in flight (8 KB at 128 e4m3 dims), asked for as soon as
+// 1.07 GB in 196 us, 5.5 TB/s, the rate of a large read on this card); 131072 e4m3 positions of
+// 8 kv heads, 268 MB, take 62 us: 56 of the split kernel and 6 of the second launch. A wave has one block's K and V in flight (8 KB at 128 e4m3 dims), asked for as soon as
 // the registers of the block before are free.
 constexpr int kBlock = 32;              // positions a wave takes at a time
 constexpr int kStep = 4 * kBlock;       // positions a workgroup takes at a time
@@ -660,7 +659,10 @@ int launch_dim(const DecodeArgs& a, int64_t dim, int pack, bool split, hipStream
 }
 // The longest sequence (as far as the table's width says) whose items stay whole, a workgroup
 // each, in one launch: dealing out steps costs a second launch, partial results and a start
-// amid an item, a whole item the time of its blocks one after the other. 32 query heads over 8
+// amid an item, a whole item the time of its blocks one after the other. Lengths are on the device, so
+// a table far wider than they need costs a call its second launch: 1 x 37 through a table of 32768
+// or 131072 positions 19, through its own 15; 32 x 500 19 / 14, 64 x 500 22 / 16, 64 x 2000 62 / 58,
+// 200 x 700 67 / 67 (host included). 32 query heads over 8
 // of 128 e4m3 dims, whole and dealt out, us: 1 x 2000 18 / 20, 1 x 3000 23 / 21, 32 x 2000 33
 // / 38, 24 x 4000 41 / 33 (at most a workgroup a CU: eight waves, about 80 KB each); 48 x 1500
 // 40 / 43, 48 x 2000 39 / 35 (unequal; up to two a CU); 64 x 2000 44 / 46, 200 x 700 44 / 64,

@@ -66,13 +66,13 @@ __global__ __launch_bounds__(kRowThreads) void varlen_rows_kernel(Packed q, Pack
 // cross lanes, a row's maximum and sum are within a lane but for one swap of halves, and V is
 // read transposed from LDS (ds_read_b64_tr_b16).
 //
-// 8192 causal positions of 64 heads of 128 bf16 dims, 1.10 TFLOP: 1.03 ms, 1.07 PFLOP/s, 75% of
-// what a bf16 product of 8192^3 reaches on this card. Both hold the power limit: with zeros
-// for inputs the same launch runs at 2.4 GHz instead of 1.9 and takes 0.77 ms. There the matrix
-// units are busy 58% of the time; three waves a SIMD hide most of the exponentials, the LDS
-// latency and the barriers. More waves a workgroup with more stages (8 x 4: 1.07 ms), loads
-// spread over the products (1.08), priorities for the products and row sums by a product with
-// ones (1.10) were measured and are not used.
+// 8192 causal positions of 64 heads of 128 bf16 dims, 1.10 TFLOP: 1.01 to 1.06 ms from card to card, 1.04
+// to 1.09 PFLOP/s, about 75% of what a bf16 product of 8192^3 reaches. Both hold the power limit:
+// with zeros for inputs the same launch runs at 2.4 GHz instead of 1.9 and takes 0.73 ms. The
+// matrix units are busy 59% of the time; three waves a SIMD hide most of the exponentials, the LDS
+// latency and the barriers. Beside a time of 1.03, more waves a workgroup with more stages (8 x 4: 1.07 ms),
+// loads spread over the products (1.08), priorities for the products and row sums by a product
+// with ones (1.10) were measured and are not used.
 constexpr int kMostSplits = 16;
 constexpr int kWaveRows = 32, kTileWaves = 4, kTileRows = kTileWaves * kWaveRows, kTileThreads = kTileWaves * kWave;
 
@@ -144,9 +144,8 @@ __device__ inline int v_swizzle(int row) { return D % 128 == 0 ? (row & 3) << 2 
 
 // The tile that is number `rank` of all from the longest on: the tile of a sequence's rows
 // t R .. sees (ahead + (t + 1) R) / KEYS tiles of keys, so a packed batch in its own order would
-// end with some workgroups at the longest tiles and the chip idle (8 prompts of 350 to 1500:
-// 122 us). Lane b holds sequence b; the length at which the count of longer tiles passes `rank`
-// is found by bisection. Causal, at most kMostRanked sequences; false past the last tile.
+// end with some workgroups at the longest tiles and the chip idle. Lane b holds sequence b; the
+// length at which the count of longer tiles passes `rank` is found by bisection. Causal, at most kMostRanked sequences; false past the last tile.
 //
 // In their own order and in this one, us: 8 prompts of up to 1500 (32 heads of 128 dims) 107 / 99, 32 of
 // them 337 / 335, 61 of them 623 / 636. Many tiles fill the end by themselves, so that nothing is
@@ -582,7 +581,7 @@ int64_t whole_groups(int64_t batch, int64_t total_q, int64_t heads) {
 }
 // How many workgroups share a tile's keys: with fewer tiles than the chip holds workgroups their
 // keys are split, down to 512 keys a part (by the mean length: what the sequences hold is known
-// on the device only). 512 rows of 32 heads behind 7000 keys: 160 us whole, 83 us split.
+// on the device only). 512 rows of 32 heads behind 7000 keys: 160 us whole, 81 us split.
 int most_splits(int64_t batch, int64_t total_q, int64_t heads) {
   if (batch < 1 || total_q < 1 || heads < 1) return 1;
   const int64_t s = 512 / whole_groups(batch, total_q, heads);
@@ -605,12 +604,12 @@ int launch_tiles(VarlenArgs a, hipStream_t st) {
   return check_launch("varlen_attention");
 }
 
-// Keys of a tile. At 128 dims 32 keys leave a wave with 164 registers (64: 187), so that three
-// workgroups share a CU: with more than two for each, eight prompts of 350 to 1500 took
-// 109 us, with 64 keys 114; with two, which then pay only for more barriers, 512 rows behind
-// 7000 keys took 87, with 64 keys 83. Four workgroups of 64 dims fit either way (a window of
-// 1024 in 16000 rows: 112 and 109 us). From 192 on two fit with 32 keys and one with 64
-// (4096 rows, 32 heads: 218 and 360 us).
+// Keys of a tile. At 128 dims 32 keys leave a wave with 166 registers (64: 180), so that three
+// workgroups share a CU: with more than two for each, eight prompts of up to 1500 take
+// 97 us, with 64 keys 106; with two, which then pay only for more barriers, 512 rows behind
+// 7000 keys take 85, with 64 keys 81. Four workgroups of 64 dims fit either way (a window of
+// 1024 in 16000 rows: 111 and 109 us). From 192 on two fit with 32 keys and one with 64
+// (4096 rows, 32 heads: 210 and 277 us).
 template <int DT>
 int launch_dims(const VarlenArgs& a, hipStream_t st) {
   if (a.dim <= 64) return launch_tiles<DT, 64, 64>(a, st);

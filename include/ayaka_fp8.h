@@ -315,8 +315,9 @@ int ayk_rms_norm_quant_fp8(const void* x, int x_dtype, int64_t rows, int64_t k, 
  * [num_pages, page_size, kv_heads, dim] contiguous, of the query's 16-bit dtype or fp8 with
  * one scale per plane. A length past table_width * page_size is cut there, and positions of
  * a page outside [0, num_pages) count as hidden: neither is read. out: [batch, heads, dim]
- * contiguous, the query's dtype. A workspace smaller than the query's answer, or none,
- * leaves the work of each sequence unsplit. */
+ * contiguous, the query's dtype. The launch is chosen from table_width, as lengths are read on the
+ * device only. A workspace smaller than the query's answer, or none, leaves the work of each
+ * sequence unsplit. */
 int ayk_paged_decode_attention(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
                                const void* key_cache, const void* value_cache, int cache_dtype,
                                int64_t num_pages, int64_t page_size, const int32_t* block_tables,
