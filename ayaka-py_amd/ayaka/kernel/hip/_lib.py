@@ -7,6 +7,7 @@ or stale library raises :class:`~ayaka.utils.import_utils.CapabilityError`.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import pathlib
@@ -68,15 +69,25 @@ SIGNATURES: dict[str, list[Any]] = {
     "ayk_fp8_grouped_blockwise_mm": [_p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _l, _p, _i, _p],
     "ayk_fp8_grouped_blockwise_mm_tables": [_p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _l, _p, _i, _p, _p, _p, _p, _p, _p, _l,
                                             _p, _l, _i, _p],
+    "ayk_fp8_block_moe_small": [_p, _i, _l, _l, _p, _p, _p, _p, _l, _l, _l, _p, _p, _l, _p, _l, _p, _z, _p],
+    "ayk_fp8_block_moe_small_workspace_bytes": [_l, _l, _l, _l],
     "ayk_int8_scaled_mm": [_p, _l, _p, _l, _l, _l, _l, _p, _p, _p, _i, _p, _i, _l, _p, _z, _p],
     "ayk_int8_scaled_mm_workspace_bytes": [_l, _l, _l],
     "ayk_kv_cache_write": [_p, _p, _i, _l, _l, _l, _p, _p, _i, _l, _p, _f, _f, _p],
     "ayk_kv_cache_gather": [_p, _i, _l, _l, _p, _l, _p, _i, _f, _i, _p],
+    "ayk_rope_kv_write": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _l, _l, _l, _l, _p, _p, _l, _l, _i, _p, _l, _l, _p, _l, _l, _p, _p,
+                          _i, _l, _p, _f, _f, _p],
+    "ayk_rope_kv_write_mxfp4": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _l, _l, _l, _l, _p, _p, _l, _l, _i, _p, _l, _l, _p, _l, _l,
+                                _p, _p, _p, _p, _l, _l, _p, _p],
+    "ayk_kv_gather_mxfp4": [_p, _p, _l, _l, _l, _l, _p, _l, _p, _i, _p],
     "ayk_rms_norm_quant_fp8": [_p, _i, _l, _l, _l, _p, _l, _p, _i, _f, _l, _i, _p, _p, _l, _l, _p, _p],
     "ayk_paged_decode_attention": [_p, _i, _l, _l, _p, _p, _i, _l, _l, _p, _l, _l, _p, _l, _l, _l, _l, _f, _f, _f, _l, _l,
                                    _p, _p, _z, _p],
     "ayk_paged_decode_attention_workspace_bytes": [_l, _l, _l, _l],
     "ayk_paged_decode_attention_split_bytes": [_l, _l, _l, _l, _i, _l, _l, _l],
+    "ayk_paged_decode_attention_mxfp4": [_p, _i, _l, _l, _p, _p, _p, _p, _l, _l, _p, _l, _l, _p, _l, _l, _l, _l, _f, _l, _l, _p, _p,
+                                         _z, _p],
+    "ayk_paged_decode_attention_mxfp4_split_bytes": [_l, _l, _l, _l, _l, _l, _l],
     "ayk_varlen_attention": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _p, _p, _l, _l, _l, _l, _l, _l, _f, _i, _l, _l, _p, _p],
     "ayk_varlen_attention_split": [_p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _p, _p, _l, _l, _l, _l, _l, _l, _f, _i, _l, _l, _p,
                                    _p, _z, _p],
@@ -105,6 +116,8 @@ _RESTYPES: dict[str, Any] = {
     "ayk_paged_decode_attention_workspace_bytes": _z,
     "ayk_varlen_attention_split_workspace_bytes": _z,
     "ayk_paged_decode_attention_split_bytes": _z,
+    "ayk_paged_decode_attention_mxfp4_split_bytes": _z,
+    "ayk_fp8_block_moe_small_workspace_bytes": _z,
     "ayk_fp8_weight_only_gemv_static_max_bytes": _z,
 }
 
@@ -158,6 +171,15 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor) -> Any:
+    """Context in which ``t``'s device is the current one (kernels are launched on that)."""
+    index = t.device.index
+    return _here if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 # Entry points by name, bound on first use (load_library takes a lock on every call).

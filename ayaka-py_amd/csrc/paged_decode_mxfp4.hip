@@ -1,0 +1,475 @@
+// Attention of one new token per sequence over the 4-bit paged cache that rope_kv_write_mxfp4 fills
+// (gfx950).
+//
+//   s_j = scale <q[b, h], K[slot(j), g]>,  p = softmax over the visible j,
+//   out[b, h] = sum_j p_j V[slot(j), g],   slot(j) = table[b][j / P] P + j % P
+//
+// with g = h / (heads / kv_heads) and K, V the values that codes and scales stand for. HBM-bound at 4.25
+// bits an element, or by the instructions that widen them: every visible row is read once for the
+// query heads that share it, sixteen at a time.
+//
+// The products are those of the 16-bit matrix instruction: S^T = K Q^T, then O^T = V^T P^T, for 32
+// positions a wave. K and V are widened to bf16 with their scale by one converter instruction for two
+// elements, exactly, whatever the scale: fp16 would overflow or lose groups of small or large scale. An
+// fp16 query is split into two bf16 numbers, exactly (8 + 3 bits), and so are the weights, rounded to
+// 16 bits; the products that this adds hide behind the widening.
+#include <type_traits>
+
+#include "mxfp4.h"
+#include "paged_decode.h"
+
+namespace ayk {
+namespace {
+
+struct MxArgs : DecodeArgs {
+  const uint8_t *ks, *vs;  // scales
+  uint32_t page_rows;      // kv_heads page_size: rows of a page
+};
+
+// What a wave holds of an item: D dims (the next of 64, 128, 256).
+template <int D>
+struct MxShape {
+  static constexpr int kSteps = D / 32;                    // 32-dim steps of the score product
+  static constexpr int kParts = D == 256 ? 2 : 1;          // 16-byte pieces of a K row in each of its four lanes
+  static constexpr int kPartWords = D == 64 ? 2 : 4;
+  static constexpr int kCols = D / 16;                     // dims of a V row in each of its sixteen lanes
+  static constexpr int kWavesPerSimd = D == 64 ? 4 : D == 128 ? 3 : 1;
+};
+
+// First dim of lane quad `quad`'s eight k slots at step s of the score product.
+template <int D>
+__device__ inline int mx_k_dim(int s, int quad) {
+  return D == 64 ? 16 * quad + 8 * s : 128 * (s / 4) + 32 * quad + 8 * (s % 4);
+}
+
+template <bool ONCE, typename T>
+__device__ inline T mx_load(const uint8_t* p, bool on) {
+  T v{};
+  if constexpr (ONCE && sizeof(T) >= 4) {
+    if (on) v = __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  } else {
+    if (on) v = *reinterpret_cast<const T*>(p);
+  }
+  return v;
+}
+
+template <int QT, int D, bool EXACT, int WAVES, bool ONCE>
+__device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int tile, int from, int to, Running<D>& r) {
+  using S = MxShape<D>;
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  constexpr bool kSplitQ = QT == AYK_F16;
+  const int lane = item_lane(), wave = threadIdx.x / kWave, col = lane % 16, quad = lane / 16;
+  const Blocks bl = blocks_of(a, len);
+  r.m = -INFINITY;
+  r.l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) r.acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const int most = bl.count < 4 * to ? bl.count : 4 * to;
+  int i = __builtin_amdgcn_readfirstlane(4 * from + wave);
+  if (i >= most) return;
+
+  // Q of this lane's head in the order of the score product's k slots.
+  const int at = tile * kHeadTile + col, head = g * a.group + at;
+  const bool has_head = at < a.group;
+  v4u qf[S::kSteps], ql[kSplitQ ? S::kSteps : 1];
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    qf[s] = v4u{0, 0, 0, 0};
+    const int dim = mx_k_dim<D>(s, quad);
+    if (has_head && (EXACT || dim < a.dim)) {
+      const uint16_t* p = a.q + b * a.q_row + head * a.q_head + dim;
+      if (a.q_aligned) {
+        qf[s] = *reinterpret_cast<const v4u*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[s][e] = (uint32_t)p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
+      }
+    }
+    if constexpr (kSplitQ) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = f16_bits_to_f32((uint16_t)qf[s][e]), y = f16_bits_to_f32((uint16_t)(qf[s][e] >> 16));
+        const uint32_t hi = pack2<AYK_BF16>(x, y);
+        // (an infinite x leaves no second part)
+        const float lx = x - u2f(hi << 16), ly = y - u2f(hi & 0xFFFF0000u);
+        qf[s][e] = hi;
+        ql[s][e] = pack2<AYK_BF16>(lx == lx ? lx : 0.0f, ly == ly ? ly : 0.0f);
+      }
+    }
+  }
+
+  const int32_t* table = a.table + b * a.table_stride;
+  const uint32_t page_size = (uint32_t)a.page_size, row_bytes = EXACT ? D / 2 : (uint32_t)a.dim / 2;
+  const uint32_t groups = EXACT ? D / kMxGroup : (uint32_t)a.dim / kMxGroup;
+  const uint8_t* kc = a.k + (uint64_t)g * page_size * row_bytes;
+  const uint8_t* vc = a.v + (uint64_t)g * page_size * row_bytes;
+  const uint8_t* ks = a.ks + (uint64_t)g * page_size * groups;
+  const uint8_t* vs = a.vs + (uint64_t)g * page_size * groups;
+  auto page_index = [&](uint32_t j) { return a.page_shift >= 0 ? j >> a.page_shift : j / page_size; };
+  // Lane l looks after position l % 32 of a block, and reads the page of its eight positions (a page
+  // holds eights whole) a block ahead of the rows.
+  auto position = [&](int blk) { return kBlock * (blk < bl.first_blocks ? blk : blk + bl.jump) + lane % kBlock; };
+  auto page_of = [&](int blk) {
+    const int first = position(blk) & ~7;
+    return first < bl.end ? table[page_index(first)] : -1;
+  };
+  auto known = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
+  auto seen_of = [&](int blk, int page) {
+    const int j = position(blk);
+    return (uint32_t)__ballot(known(page) && j < bl.end && (j >= bl.first || j < bl.kept));
+  };
+  auto row_of = [&](int blk, int page) {  // of the eight's first position (page unknown: any row)
+    const uint32_t first = position(blk) & ~7;
+    return known(page) ? (uint32_t)page * a.page_rows + (first - page_index(first) * page_size) : 0u;
+  };
+  // Row 4 (l / 16) + i of score tile t is position 8 (l / 16) + 4 t + i: the lane's weights are then
+  // those of eight positions in a row, in the order of V's k slots.
+  uint32_t kw[2][S::kParts * S::kPartWords], kse[2][S::kParts], vw[8][D == 256 ? 2 : 1], vse[D == 64 ? 4 : 8];
+  auto issue_k = [&](uint32_t row) {
+    const uint32_t eight = (uint32_t)__builtin_amdgcn_ds_bpermute(32 * (col / 4), (int)row);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint64_t at = eight + 4 * t + col % 4;
+#pragma unroll
+      for (int h = 0; h < S::kParts; ++h) {
+        const bool on = EXACT || mx_k_dim<D>(4 * h, quad) < a.dim;
+        if constexpr (D == 64) {
+          *reinterpret_cast<v2u*>(kw[t]) = mx_load<ONCE, v2u>(kc + at * row_bytes + 8 * quad, on);
+          kse[t][0] = mx_load<false, uint8_t>(ks + at * groups + quad / 2, on);
+        } else {
+          *reinterpret_cast<v4u*>(kw[t] + 4 * h) = mx_load<ONCE, v4u>(kc + at * row_bytes + 64 * h + 16 * quad, on);
+          kse[t][h] = mx_load<false, uint8_t>(ks + at * groups + 4 * h + quad, on);
+        }
+      }
+    }
+  };
+  constexpr bool kVector = EXACT && D != 256;  // the scales of eight rows as one or two 16-byte loads
+  const bool v_on = EXACT || col * S::kCols < a.dim;
+  const int v_group = col * S::kCols / kMxGroup;
+  auto issue_v = [&](uint32_t row) {
+    const uint64_t eight = (uint32_t)__builtin_amdgcn_ds_bpermute(32 * quad, (int)row);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* p = vc + (eight + j) * row_bytes + col * S::kCols / 2;
+      if constexpr (D == 64) vw[j][0] = mx_load<ONCE, uint16_t>(p, v_on);
+      else if constexpr (D == 128) vw[j][0] = mx_load<ONCE, uint32_t>(p, v_on);
+      else *reinterpret_cast<v2u*>(vw[j]) = mx_load<ONCE, v2u>(p, v_on);
+      if constexpr (!kVector) {
+        if constexpr (D == 64) {
+          if (j % 2 == 0) vse[j / 2] = 0;
+          vse[j / 2] |= (uint32_t)mx_load<false, uint8_t>(vs + (eight + j) * groups + v_group, v_on) << (16 * (j % 2) + 8 * v_group);
+        } else {
+          vse[j] = mx_load<false, uint8_t>(vs + (eight + j) * groups + v_group, v_on);
+        }
+      }
+    }
+    if constexpr (kVector) {
+#pragma unroll
+      for (int w = 0; w < (D == 64 ? 4 : 8); w += 4)
+        *reinterpret_cast<v4u*>(vse + w) = *reinterpret_cast<const v4u*>(vs + eight * groups + 4 * w);
+    }
+  };
+
+  int page = page_of(i);
+  uint32_t seen = seen_of(i, page), row = row_of(i, page);
+  page = i + WAVES < most ? page_of(i + WAVES) : -1;
+  issue_k(row);
+  issue_v(row);
+  while (true) {
+    const bool more = i + WAVES < most;
+    const uint32_t now = seen;
+    v4f s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int d = 0; d < S::kSteps; ++d) {
+        const uint32_t w = kw[t][d];
+        const float sc = u2f(kse[t][S::kParts == 2 ? d / 4 : 0] << 23);
+        const v4u f{mx4_widen2<0>(w, sc), mx4_widen2<1>(w, sc), mx4_widen2<2>(w, sc), mx4_widen2<3>(w, sc)};
+        s[t] = mfma16<AYK_BF16>(f, qf[d], s[t]);
+        if constexpr (kSplitQ) s[t] = mfma16<AYK_BF16>(f, ql[d], s[t]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) {
+      seen = seen_of(i + WAVES, page);
+      row = row_of(i + WAVES, page);
+      if (i + 2 * WAVES < most) page = page_of(i + 2 * WAVES);
+      issue_k(row);
+    }
+    float x[8], vsc[8], top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = s[j / 4][j % 4] * a.scale_log2;
+      const uint32_t code = D == 64 ? vse[j / 2] >> (16 * (j % 2) + 8 * v_group) : kVector ? vse[j] >> (8 * v_group) : vse[j];
+      vsc[j] = u2f((code & 0xFFu) << 23);
+    }
+    if (now != 0xFFFFFFFFu) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool on = (now >> (8 * quad + j)) & 1;
+        x[j] = on ? x[j] : -INFINITY;
+        vsc[j] = on ? vsc[j] : 0.0f;  // a weight of 0 times a hidden NaN
+#pragma unroll
+        for (int w = 0; w < (D == 256 ? 2 : 1); ++w) vw[j][w] = on ? vw[j][w] : 0u;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+    top = fmaxf(r.m, max_quads(top));
+    if (__ballot(top > r.m)) {  // wave-uniform: some head's maximum grew
+      const float keep = r.m == -INFINITY ? 0.0f : exp2_fast(r.m - top);
+      r.m = top;
+      r.l *= keep;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) r.acc[t] *= keep;
+    }
+    const float base = r.m == -INFINITY ? 0.0f : r.m;  // nothing visible so far weighs 0
+    v4u p, pl;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      x[j] = exp2_fast(x[j] - base);
+      x[j + 1] = exp2_fast(x[j + 1] - base);
+      r.l += x[j];
+      r.l += x[j + 1];
+      p[j / 2] = pack2<AYK_BF16>(x[j], x[j + 1]);
+      pl[j / 2] = pack2<AYK_BF16>(x[j] - u2f(p[j / 2] << 16), x[j + 1] - u2f(p[j / 2] & 0xFFFF0000u));
+    }
+    // V^T: two dims of two positions side by side, from one converter instruction a position.
+    auto product = [&](auto byte) {
+      constexpr int kByte = decltype(byte)::value;
+      v4u f[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = mx4_widen2<kByte % 4>(vw[2 * j][kByte / 4], vsc[2 * j]);
+        const uint32_t w = mx4_widen2<kByte % 4>(vw[2 * j + 1][kByte / 4], vsc[2 * j + 1]);
+        f[0][j] = __builtin_amdgcn_perm(w, u, 0x05040100u);
+        f[1][j] = __builtin_amdgcn_perm(w, u, 0x07060302u);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        r.acc[2 * kByte + e] = mfma16<AYK_BF16>(f[e], p, r.acc[2 * kByte + e]);
+        r.acc[2 * kByte + e] = mfma16<AYK_BF16>(f[e], pl, r.acc[2 * kByte + e]);
+      }
+    };
+    product(std::integral_constant<int, 0>{});
+    product(std::integral_constant<int, 1>{});
+    if constexpr (D >= 128) {
+      product(std::integral_constant<int, 2>{});
+      product(std::integral_constant<int, 3>{});
+    }
+    if constexpr (D >= 256) {
+      product(std::integral_constant<int, 4>{});
+      product(std::integral_constant<int, 5>{});
+      product(std::integral_constant<int, 6>{});
+      product(std::integral_constant<int, 7>{});
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!more) break;
+    issue_v(row);
+    i += WAVES;
+  }
+}
+
+// Wave 0 writes an item: rounded to the output, or as a partial result (a row of D sums, the maximum
+// and the sum for every head). Element i of the lane's tiles is dims kCols (4 quad + i) ...
+template <int QT, int D, bool EXACT>
+__device__ inline void write_mx(const MxArgs& a, int b, int g, int tile, const Running<D>& r, float* partial) {
+  constexpr int kCols = D / 16;
+  const int lane = item_lane(), col = lane % 16, quad = lane / 16, at = tile * kHeadTile + col;
+  const float l = sum_quads(r.l);
+  if (at >= a.group) return;
+  if (partial) {
+    float* p = partial + col * (D + 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < kCols; ++t) p[(4 * quad + i) * kCols + t] = r.acc[t][i];
+    if (quad == 0) {
+      p[D] = r.m;
+      p[D + 1] = l;
+    }
+    return;
+  }
+  uint16_t* o = a.out + ((int64_t)b * a.heads + g * a.group + at) * (EXACT ? D : a.dim);
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int dim = (4 * quad + i) * kCols;
+    if (!EXACT && dim >= a.dim) continue;
+#pragma unroll
+    for (int t = 0; t < kCols; t += 2) *reinterpret_cast<uint32_t*>(o + dim + t) = pack2<QT>(r.acc[t][i] * f, r.acc[t + 1][i] * f);
+  }
+}
+
+// One workgroup per sequence, kv head and head tile, whose waves take its blocks in turn.
+template <int QT, int D, bool EXACT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, (MxShape<D>::kWavesPerSimd)) void mx_decode_kernel(MxArgs a) {
+  __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
+  const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
+  Running<D> r;
+  attend_mx<QT, D, EXACT, WAVES, false>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
+  join_waves<D, WAVES>(r, lds);
+  if (threadIdx.x < kWave) write_mx<QT, D, EXACT>(a, b, g, tile, r, nullptr);
+}
+
+// Long sequences: the steps of all items are dealt out evenly, a run of consecutive ones to every
+// workgroup, whatever the lengths. A run may end one item, hold some whole and begin another; what
+// it does not hold whole it leaves as a partial result, in slot 0 (the run begins inside the item) or
+// slot 1 (it ends inside).
+template <int QT, int D, bool EXACT, bool ONCE>
+__global__ __launch_bounds__(kDecodeThreads, (MxShape<D>::kWavesPerSimd)) void mx_decode_split_kernel(MxArgs a) {
+  __shared__ float lds[2][D / 4 + 2][kWave];
+  const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
+  const int total = __builtin_amdgcn_readfirstlane(total_steps(a));
+  const int share = (total + gridDim.x - 1) / (int)gridDim.x;
+  const int run = blockIdx.x;
+  int at = run * share;
+  const int end = at + share < total ? at + share : total;
+  int before = 0;  // steps of the sequences before chunk
+  for (int chunk = 0; chunk < a.batch && at < end; chunk += kWave) {
+    const int len = chunk + lane < a.batch ? a.lens[chunk + lane] : 0, mine = steps_of(a, len);
+    const int upto = wave_scan(mine);
+    while (at < end) {
+      // the first sequence whose items end past `at`
+      const uint64_t past = __ballot(before + upto * per > at);
+      if (!past) break;
+      const int k = __builtin_ctzll(past);
+      const int steps = __builtin_amdgcn_readlane(mine, k);
+      const int start = before + (__builtin_amdgcn_readlane(upto, k) - steps) * per;
+      const int item = (at - start) / steps, first = (at - start) - item * steps;
+      const int last = first + (end - at) < steps ? first + (end - at) : steps;
+      Running<D> r;
+      const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
+      attend_mx<QT, D, EXACT, 4, ONCE>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
+      join_waves<D, 4>(r, lds);
+      float* partial = nullptr;
+      if (first > 0 || last < steps) partial = a.partial + ((int64_t)run * 2 + (first > 0 ? 0 : 1)) * a.rows * (D + 2);
+      if (threadIdx.x < kWave) write_mx<QT, D, EXACT>(a, b, g, tile, r, partial);
+      at += last - first;
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1) * per;
+  }
+}
+
+template <int QT, int D, bool EXACT>
+int launch_mx(const MxArgs& a, bool split, hipStream_t st) {
+  if (!split) {
+    const unsigned items = (unsigned)(a.batch * a.tiles * a.kv_items);
+    // Two waves a SIMD where a CU has one workgroup at most.
+    constexpr int kMostWaves = MxShape<D>::kWavesPerSimd >= 2 ? 8 : 4;
+    if (items <= 256) hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, kMostWaves>), dim3(items), dim3(kMostWaves * kWave), 0, st, a);
+    else hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, 4>), dim3(items), dim3(4 * kWave), 0, st, a);
+    note_plan("paged_decode_mxfp4 whole");
+  } else {
+    constexpr int runs = 256 * MxShape<D>::kWavesPerSimd;
+    hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT, false>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    launch_join<QT, D, 1>(a, runs, st);
+    note_plan("paged_decode_mxfp4 split");
+  }
+  return check_launch("paged_decode_attention_mxfp4");
+}
+template <int QT>
+int launch_mx_dim(const MxArgs& a, bool split, hipStream_t st) {
+#define AYK_PDM(D) \
+  if (a.dim <= D) return a.dim == D ? launch_mx<QT, D, true>(a, split, st) : launch_mx<QT, D, false>(a, split, st)
+  AYK_PDM(64);
+  AYK_PDM(128);
+  AYK_PDM(256);
+#undef AYK_PDM
+  return fail(AYK_EINVAL, "paged_decode_attention_mxfp4: dim=%d", a.dim);
+}
+
+int64_t mx_width(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+int64_t mx_longest(int64_t most, int64_t window, int64_t sinks) {
+  return window > 0 && sinks < most && window < most - sinks ? window + sinks + 2 * kBlock : most;
+}
+bool mx_deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest) {
+  const int64_t items = batch * cdiv(heads / kv_heads, kHeadTile) * kv_heads;
+  const int64_t limit = (items <= 256 ? 640 : items < 512 ? 400 : 560) * 1024 / mx_width(dim);
+  return longest > limit && items * (cdiv(longest, kStep) + 1) < 0x40000000;
+}
+
+}  // namespace
+}  // namespace ayk
+
+using namespace ayk;
+
+extern "C" {
+
+size_t ayk_paged_decode_attention_mxfp4_split_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t most,
+                                                        int64_t window, int64_t sinks) {
+  if (dim < 1 || dim > kMaxDim || dim % kMxGroup || kv_heads < 1 || heads < kv_heads || batch < 1 || most < 0 || window < 0 || sinks < 0)
+    return 0;
+  if (!mx_deals_out(batch, heads, kv_heads, dim, mx_longest(most, window, sinks))) return 0;
+  return (size_t)(2 * kMostRuns * kHeadTile * (mx_width(dim) + 2)) * sizeof(float);
+}
+
+int ayk_paged_decode_attention_mxfp4(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride, const void* key_codes,
+                                     const void* key_scales, const void* value_codes, const void* value_scales, int64_t num_pages,
+                                     int64_t page_size, const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                                     const int32_t* seq_lens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, float scale,
+                                     int64_t window, int64_t sinks, void* out, void* workspace, size_t workspace_bytes,
+                                     ayk_stream_t stream) {
+  const char* op = "paged_decode_attention_mxfp4";
+  if (q_dtype != AYK_F16 && q_dtype != AYK_BF16) return fail(AYK_EINVAL, "%s: query must be float16 or bfloat16", op);
+  if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1 || dim > kMaxDim || dim % kMxGroup)
+    return fail(AYK_EINVAL, "%s: bad shape batch=%lld heads=%lld kv_heads=%lld dim=%lld (dim a multiple of %d, at most %d)", op,
+                (long long)batch, (long long)heads, (long long)kv_heads, (long long)dim, kMxGroup, kMaxDim);
+  if (q_row_stride < 0 || q_head_stride < 0 || num_pages < 0 || page_size < 8 || page_size % 8 || table_width < 0 || table_stride < 0)
+    return fail(AYK_EINVAL, "%s: bad strides, pages (page_size a multiple of 8) or table width", op);
+  if (window < 0 || sinks < 0) return fail(AYK_EINVAL, "%s: window and sinks must not be negative", op);
+  if (!(scale - scale == 0.0f)) return fail(AYK_EINVAL, "%s: the scale must be finite", op);
+  // Positions and the rows of a plane are counted in 32 bits.
+  if (page_size > 0x7FFFFF00 || table_width > 0x7FFFFF00 / page_size)
+    return fail(AYK_EINVAL, "%s: the table names more than 2^31 positions", op);
+  if (kv_heads > 0x7FFFFFFF / page_size || num_pages > 0xFFFFFF00ll / (kv_heads * page_size))
+    return fail(AYK_EINVAL, "%s: a plane has more than 2^32 rows of a head", op);
+  if (batch == 0) return AYK_OK;
+  const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
+  if (heads > 65535 || batch > kMostGroups || batch * tiles * kv_heads > kMostGroups)
+    return fail(AYK_EINVAL, "%s: batch and heads exceed the grid", op);
+  if (q == nullptr || out == nullptr || seq_lens == nullptr || (table_width > 0 && block_tables == nullptr) ||
+      (num_pages > 0 && (key_codes == nullptr || key_scales == nullptr || value_codes == nullptr || value_scales == nullptr)))
+    return fail(AYK_EINVAL, "%s: missing operand", op);
+  for (const void* p : {key_codes, key_scales, value_codes, value_scales, static_cast<const void*>(out)})
+    if (!aligned16(p)) return fail(AYK_EINVAL, "%s: the planes and the output must be 16-byte aligned", op);
+  if (int rc = check_device()) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  MxArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.k = static_cast<const uint8_t*>(key_codes);
+  a.v = static_cast<const uint8_t*>(value_codes);
+  a.ks = static_cast<const uint8_t*>(key_scales);
+  a.vs = static_cast<const uint8_t*>(value_scales);
+  a.page_rows = (uint32_t)(kv_heads * page_size);
+  a.table = block_tables;
+  a.table_stride = table_stride;
+  a.num_pages = (int)(num_pages < 0x7FFFFFFF ? num_pages : 0x7FFFFFFF);
+  a.page_size = (int)page_size;
+  a.longest = num_pages > 0 ? (int)most : 0;  // no page: nothing is visible, nothing is read
+  a.lens = seq_lens;
+  a.batch = (int)batch;
+  a.heads = (int)heads;
+  a.dim = (int)dim;
+  a.kv_items = (int)kv_heads;
+  a.group = (int)group;
+  a.tiles = (int)tiles;
+  a.rows = (int)(group < kHeadTile ? group : kHeadTile);
+  a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctzll((uint64_t)page_size);
+  a.scale_log2 = scale * kLog2e;
+  a.v_scale = 1.0f;
+  a.window = (int)(window < 0x7FFFFFFF ? window : 0x7FFFFFFF);
+  a.sinks = (int)(sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF);
+  a.out = static_cast<uint16_t*>(out);
+  a.partial = static_cast<float*>(workspace);
+  a.q_aligned = aligned16(q) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0;
+  const size_t need = ayk_paged_decode_attention_mxfp4_split_bytes(batch, heads, kv_heads, dim, most, window, sinks);
+  const bool split = need > 0 && workspace != nullptr && aligned16(workspace) && workspace_bytes >= need;
+  return q_dtype == AYK_BF16 ? launch_mx_dim<AYK_BF16>(a, split, st) : launch_mx_dim<AYK_F16>(a, split, st);
+}
+
+}  // extern "C"

@@ -198,6 +198,21 @@ int ayk_fp8_grouped_blockwise_mm_tables(const void* a, const void* b, const floa
                                         int64_t* b_scales_ptrs, int32_t* layout_sfa, int64_t ld_sfa, int32_t* layout_sfb,
                                         int64_t ld_sfb, int transpose, ayk_stream_t stream);
 
+/* No counterpart in the reference: a mixture-of-experts layer for few tokens (at most 64) with
+ * e4m3 experts under 128 x 128 block scales:
+ *   out[t] = sum_j weights[t, j] * down[e] (silu(gate[e] x[t]) * (up[e] x[t])),  e = ids[t, j]
+ * gate_up is [experts, 2 * inner, hidden] (gate rows, then up rows) with scales [experts, 2 * inner /
+ * 128, hidden / 128], down is [experts, hidden, inner] with [experts, hidden / 128, inner / 128], all
+ * contiguous, hidden and inner multiples of 128. x is [tokens, hidden] F16/BF16 and out its dtype,
+ * not quantized: products are of the 16-bit activations, sums fp32. Entries of ids outside
+ * [0, experts) count nothing; one that a token names twice counts with both weights. weights and ids
+ * are [tokens, topk] contiguous. The workspace is needed, 16-byte aligned. */
+int ayk_fp8_block_moe_small(const void* x, int x_dtype, int64_t ldx, int64_t tokens, const void* gate_up,
+                            const float* gate_up_scale, const void* down, const float* down_scale, int64_t experts,
+                            int64_t hidden, int64_t inner, const float* weights, const int32_t* ids, int64_t topk,
+                            void* out, int64_t ldo, void* workspace, size_t workspace_bytes, ayk_stream_t stream);
+size_t ayk_fp8_block_moe_small_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts, int64_t inner);
+
 /* Replaces ayaka::mxfp8_scaled_mm (gemm/fp8_mxfp8_gemm.py:163; oracle reference/gemm.py:73-92).
  * out = sum_g (a[:, g] @ w[:, g]^T) * 2^(a_scale[m,g]-127) * 2^(w_scale[n,g]-127) + bias
  * over 32-wide K groups g; UE8M0 code 0 decodes to 0 and 0xFF to NaN.
@@ -288,6 +303,42 @@ int ayk_kv_cache_gather(const void* cache, int cache_dtype, int64_t num_slots, i
                         const int64_t* slots, int64_t n, void* dest, int dest_dtype, float scale,
                         int dequantize, ayk_stream_t stream);
 
+/* No counterpart in the reference: position rotation of a step's queries and keys with the append
+ * to the cache of ayk_kv_cache_write. Rows of q are [tokens, heads, dim] and of k and v [tokens,
+ * kv_heads, dim], with the given strides in elements and the elements of a head side by side.
+ * cos_sin is [table_rows, rotary_dim] contiguous: the cosines of a position's rotary_dim / 2 angles,
+ * then the sines. (x, y) -> (x cos - y sin, y cos + x sin), each operation rounded to fp32, for the
+ * pairs (d, d + rotary_dim / 2), or (2d, 2d + 1) when interleaved; dims from rotary_dim on pass
+ * through; rotary_dim 0: no rotation (positions and cos_sin unused). q_out, and k_out unless NULL, get
+ * the rotated rows in the query's dtype and may be q and k themselves. The caches take the rotated
+ * fp32 keys, and the values, as ayk_kv_cache_write does; cache_dtype: fp8 or the keys' dtype. A token
+ * whose slot is outside [0, num_slots) is not written; one whose position is outside the table
+ * neither, and its rows of q_out and k_out are zeros. No slot may come twice. heads may be 0. */
+int ayk_rope_kv_write(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
+                      int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride, int dtype,
+                      int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, const int64_t* positions,
+                      const float* cos_sin, int64_t table_rows, int64_t rotary_dim, int interleaved, void* q_out,
+                      int64_t qo_row_stride, int64_t qo_head_stride, void* k_out, int64_t ko_row_stride,
+                      int64_t ko_head_stride, void* key_cache, void* value_cache, int cache_dtype, int64_t num_slots,
+                      const int64_t* slots, float k_inverse, float v_inverse, ayk_stream_t stream);
+/* The same into a 4-bit cache. A plane is codes [num_pages, kv_heads, page_size, dim / 2] (OCP
+ * e2m1, the even dim in the low half of a byte) and scales [num_pages, kv_heads, page_size, dim / 32]
+ * (UE8M0: value 2^(code - 127), 0xFF NaN), both contiguous. A group of 32 dims takes the least scale
+ * under which no magnitude exceeds 6, codes are rounded to nearest even; zeros have scale code 0, a
+ * group with an infinity or NaN has 0xFF. dim % 32 == 0; slot = page * page_size + offset. */
+int ayk_rope_kv_write_mxfp4(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
+                            int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride, int dtype,
+                            int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, const int64_t* positions,
+                            const float* cos_sin, int64_t table_rows, int64_t rotary_dim, int interleaved, void* q_out,
+                            int64_t qo_row_stride, int64_t qo_head_stride, void* k_out, int64_t ko_row_stride,
+                            int64_t ko_head_stride, void* key_codes, void* key_scales, void* value_codes,
+                            void* value_scales, int64_t num_pages, int64_t page_size, const int64_t* slots,
+                            ayk_stream_t stream);
+/* dest[i] = the values of slot slots[i] of one 4-bit plane, [n, kv_heads, dim] in fp32, fp16 or bf16.
+ * A slot outside the plane gives zeros. */
+int ayk_kv_gather_mxfp4(const void* codes, const void* scales, int64_t num_pages, int64_t page_size, int64_t kv_heads,
+                        int64_t dim, const int64_t* slots, int64_t n, void* dest, int dest_dtype, ayk_stream_t stream);
+
 /* ------------------------------------------------------------------ norm
  * No counterpart in the reference's FP8 path: h = x + residual (x without one), rounded to
  * x's dtype into residual_out; y = h * weight / sqrt(mean(h^2) + eps) in fp32 from the
@@ -330,6 +381,20 @@ size_t ayk_paged_decode_attention_workspace_bytes(int64_t batch, int64_t heads, 
  * 0 where every sequence stays whole. */
 size_t ayk_paged_decode_attention_split_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int cache_dtype,
                                               int64_t most, int64_t window, int64_t sinks);
+
+/* The same over the 4-bit cache of ayk_rope_kv_write_mxfp4. page_size % 8 == 0, dim % 32 == 0, all four
+ * planes 16-byte aligned. The products are of the decoded values, exact but for the weights, which
+ * are rounded to 16 significant bits. _split_bytes: the workspace of calls whose longest possible
+ * sequence is `most` = table_width * page_size positions (0: none needed). */
+int ayk_paged_decode_attention_mxfp4(const void* q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                     const void* key_codes, const void* key_scales, const void* value_codes,
+                                     const void* value_scales, int64_t num_pages, int64_t page_size,
+                                     const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                                     const int32_t* seq_lens, int64_t batch, int64_t heads, int64_t kv_heads,
+                                     int64_t dim, float scale, int64_t window, int64_t sinks, void* out,
+                                     void* workspace, size_t workspace_bytes, ayk_stream_t stream);
+size_t ayk_paged_decode_attention_mxfp4_split_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                                                        int64_t most, int64_t window, int64_t sinks);
 
 /* Packed sequences: sequence b holds query rows [starts_q[b], starts_q[b + 1]) and key rows
  * [starts_k[b], starts_k[b + 1]); its queries are the last positions of its keys (more
