@@ -70,7 +70,7 @@ SIGNATURES: dict[str, list[Any]] = {
     "ayk_fp8_grouped_blockwise_mm_tables": [_p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _l, _p, _i, _p, _p, _p, _p, _p, _p, _l,
                                             _p, _l, _i, _p],
     "ayk_fp8_block_moe_small": [_p, _i, _l, _l, _p, _p, _p, _p, _l, _l, _l, _p, _p, _l, _p, _l, _p, _z, _p],
-    "ayk_fp8_block_moe_small_workspace_bytes": [_l, _l, _l, _l],
+    "ayk_fp8_block_moe_small_scratch_bytes": [_l, _l, _l, _l, _l],
     "ayk_int8_scaled_mm": [_p, _l, _p, _l, _l, _l, _l, _p, _p, _p, _i, _p, _i, _l, _p, _z, _p],
     "ayk_int8_scaled_mm_workspace_bytes": [_l, _l, _l],
     "ayk_kv_cache_write": [_p, _p, _i, _l, _l, _l, _p, _p, _i, _l, _p, _f, _f, _p],
@@ -117,7 +117,7 @@ _RESTYPES: dict[str, Any] = {
     "ayk_varlen_attention_split_workspace_bytes": _z,
     "ayk_paged_decode_attention_split_bytes": _z,
     "ayk_paged_decode_attention_mxfp4_split_bytes": _z,
-    "ayk_fp8_block_moe_small_workspace_bytes": _z,
+    "ayk_fp8_block_moe_small_scratch_bytes": _z,
     "ayk_fp8_weight_only_gemv_static_max_bytes": _z,
 }
 

@@ -111,7 +111,7 @@ def fp8_block_moe_small(
         x = x.clone(memory_format=torch.contiguous_format)
     topk_weights, topk_ids = topk_weights.contiguous(), topk_ids.contiguous()
     experts, inner, topk = down.shape[0], down.shape[2], topk_ids.shape[1]
-    need = _lib.query("ayk_fp8_block_moe_small_workspace_bytes", tokens, topk, experts, inner)
+    need = _lib.query("ayk_fp8_block_moe_small_scratch_bytes", tokens, topk, experts, hidden, inner)
     with _lib.on_device(x):
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
         _lib.call("ayk_fp8_block_moe_small", x.data_ptr(), _lib.dtype_code(x.dtype), x.stride(0) if tokens > 1 else hidden, tokens,

@@ -18,6 +18,8 @@ namespace {
 
 constexpr int kMoeTokens = 64;     // tokens of a call, at most: a bit each of a mask
 constexpr int kMoeExperts = 1024;  // experts of a layer, at most: a mask each in LDS
+constexpr int kMoeTopk = 0x7FFF;
+constexpr int kMoeWidth = 0x1000000;
 constexpr int kMoeThreads = 512;
 constexpr int kMoeWaves = kMoeThreads / kWave;
 constexpr int kMoeBlock = 128;
@@ -31,7 +33,9 @@ struct MoeArgs {
   const float* weights;
   uint16_t* out;
   int64_t ldo;
-  uint16_t* h;  // [rows][inner / 8][first parts of eight, second parts of eight]
+  uint16_t* h;     // [rows][inner / 8][first parts of eight, second parts of eight]
+  float* partial;  // [runs][tokens][hidden], of the second launch
+  int* arrived;    // [hidden / 128]: workgroups that left theirs; the first launch clears it
   int tokens, topk, experts, hidden, inner;
 };
 
@@ -39,24 +43,24 @@ struct MoeArgs {
 // first of its rows of h (a row a token, in the tokens' order). A pure function of ids, so both kernels
 // number the rows alike.
 struct MoeList {
-  uint64_t mask[kMoeExperts];
-  uint64_t tokens[kMoeExperts];  // of the list's entries
+  uint64_t tokens[kMoeExperts];
   uint16_t expert[kMoeExperts], row[kMoeExperts];
   int count;
 };
-__device__ inline void list_experts(const MoeArgs& a, MoeList& l) {
-  for (int e = threadIdx.x; e < a.experts; e += kMoeThreads) l.mask[e] = 0;
+// masks: room for kMoeExperts in LDS while the list is made.
+__device__ inline void list_experts(const MoeArgs& a, MoeList& l, uint64_t* masks) {
+  for (int e = threadIdx.x; e < a.experts; e += kMoeThreads) masks[e] = 0;
   __syncthreads();
   for (int p = threadIdx.x; p < a.tokens * a.topk; p += kMoeThreads) {
     const int e = a.ids[p];
-    if ((uint32_t)e < (uint32_t)a.experts) atomicOr((unsigned long long*)&l.mask[e], 1ull << (p / a.topk));
+    if ((uint32_t)e < (uint32_t)a.experts) atomicOr((unsigned long long*)&masks[e], 1ull << (p / a.topk));
   }
   __syncthreads();
   if (threadIdx.x < kWave) {
     int count = 0, rows = 0;
     for (int e0 = 0; e0 < a.experts; e0 += kWave) {
       const int e = e0 + threadIdx.x;
-      const uint64_t mask = e < a.experts ? l.mask[e] : 0;
+      const uint64_t mask = e < a.experts ? masks[e] : 0;
       const uint64_t used = __ballot(mask != 0);
       const int mine = __popcll(mask), upto = wave_scan(mine);
       if (mask) {
@@ -90,32 +94,34 @@ template <int DT>
 __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) {
   __shared__ MoeList list;
   __shared__ float part[kMoeWaves][2][16][16];
-  list_experts(a, list);
+  list_experts(a, list, reinterpret_cast<uint64_t*>(part));
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = lane % 16, quad = lane / 16;
   const int slices = a.inner / 16, blocks = a.hidden / kMoeBlock;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < blocks; i += kMoeThreads) a.arrived[i] = 0;
   for (int item = blockIdx.x; item < list.count * slices; item += gridDim.x) {
     const int u = item / slices, n0 = (item - u * slices) * 16, e = list.expert[u];
     const uint64_t tokens = list.tokens[u];
-    const uint8_t* gate = a.gate_up + ((int64_t)e * 2 * a.inner + n0 + col) * a.hidden + 32 * quad;
+    const uint8_t* gate = a.gate_up + ((int64_t)e * 2 * a.inner + n0 + col) * a.hidden + 16 * quad;
     const uint8_t* up = gate + (int64_t)a.inner * a.hidden;
     const float* gate_scale = a.gate_up_scale + ((int64_t)e * 2 * (a.inner / kMoeBlock) + n0 / kMoeBlock) * blocks;
     const float* up_scale = gate_scale + (int64_t)(a.inner / kMoeBlock) * blocks;
     const int rows = __popcll(tokens);
     for (int r0 = 0; r0 < rows; r0 += 16) {
       const bool live = r0 + col < rows;
-      const uint16_t* x = a.x + nth_bit(tokens, r0 + col) * a.ldx + 32 * quad;
+      const uint16_t* x = a.x + nth_bit(tokens, r0 + col) * a.ldx + 16 * quad;
       v4f g{0, 0, 0, 0}, w{0, 0, 0, 0};
       for (int b = wave; b < blocks; b += kMoeWaves) {
         v4u gw[2], uw[2], xs[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          gw[i] = *reinterpret_cast<const v4u*>(gate + b * kMoeBlock + 16 * i);
-          uw[i] = *reinterpret_cast<const v4u*>(up + b * kMoeBlock + 16 * i);
+          gw[i] = *reinterpret_cast<const v4u*>(gate + b * kMoeBlock + 64 * i);
+          uw[i] = *reinterpret_cast<const v4u*>(up + b * kMoeBlock + 64 * i);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           xs[i] = v4u{0, 0, 0, 0};
-          if (live) xs[i] = *reinterpret_cast<const v4u*>(x + b * kMoeBlock + 8 * i);
+          if (live) xs[i] = *reinterpret_cast<const v4u*>(x + b * kMoeBlock + 64 * (i / 2) + 8 * (i % 2));
         }
         v4f gs{0, 0, 0, 0}, us{0, 0, 0, 0};
 #pragma unroll
@@ -159,64 +165,245 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   }
 }
 
-// Sixteen output channels of all tokens: the waves share out the blocks of 128 k of all experts. A
-// column is a token, so the sums of all its experts stay in one accumulator; an expert's sums join only
-// the columns of its own tokens, whatever its weights hold.
-template <int DT, int TILES>
+// 128 output channels of all tokens, sixteen a wave. The blocks of 128 k of all experts in a row are one
+// list, of which every workgroup of a channel block takes an equal run; the runs' sums meet in fp32
+// partial results, which the last workgroup to finish adds in the runs' order. Sums of an expert's
+// rows join those of their tokens in LDS, where each lane owns its cells: results do not depend on
+// the order of waves.
+//
+// All that the loop reads comes through LDS by direct loads: the weights of a wave kDownAhead blocks
+// ahead (registers would have to be named at compile time, which blocks of unequal chunks do not
+// allow), the rows of h, which the waves share, in chunks of up to kDownPairs (row, block) pairs of
+// 512 bytes, a chunk ahead. The waits are counted by hand: the loads of a wave land in order.
+constexpr int kDownAhead = 4;
+constexpr int kDownPairs = 32;
+constexpr int kPairBytes = 4 * kMoeBlock;
+constexpr int kTokenFloats = kMoeBlock + 4;  // a token's channels, and a shift of four banks
+constexpr int kRingBytes = kDownAhead * 2048;
+
+__device__ inline uint32_t lds_address(const void* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
+}
+// 16 bytes a lane to lds + 16 lane, in assembly: the compiler would make every read of LDS wait for
+// all direct loads in flight. Nothing but wait_loads and the barriers orders them with reads. The idle
+// cycles are those that the write of m0 needs before a load reads it.
+__device__ inline void load_to_lds(const uint8_t* from, uint32_t at, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(at), "s"(from), "{m0}"(lds));
+}
+__device__ inline void load_to_lds(const uint8_t* from, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(lds));
+}
+// Until at most N of the wave's loads are in flight.
+template <int N>
+__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+
+// A block's weights (the lane's sixteen bytes of two loads) and the first and second parts of eight
+// rows' k slots for its four steps, from LDS; the reads are done when the block ends.
+struct DownRows {
+  v4u part[8];  // step s: first parts at 2 s, second parts at 2 s + 1
+};
+__device__ inline void read_rows(uint32_t at, DownRows& r) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %8 offset:256\n\tds_read_b128 %5, %9 offset:256\n\tds_read_b128 %6, %10 offset:256\n\t"
+      "ds_read_b128 %7, %11 offset:256\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r.part[0]), "=&v"(r.part[1]), "=&v"(r.part[2]), "=&v"(r.part[3]), "=&v"(r.part[4]), "=&v"(r.part[5]),
+        "=&v"(r.part[6]), "=&v"(r.part[7])
+      : "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48)
+      : "memory");
+}
+__device__ inline void read_block(uint32_t weights, uint32_t at, v4u (&w)[2], DownRows& r) {
+  asm volatile(
+      "ds_read_b128 %8, %10\n\tds_read_b128 %9, %10 offset:1024\n\t"
+      "ds_read_b128 %0, %11\n\tds_read_b128 %1, %12\n\tds_read_b128 %2, %13\n\tds_read_b128 %3, %14\n\t"
+      "ds_read_b128 %4, %11 offset:256\n\tds_read_b128 %5, %12 offset:256\n\tds_read_b128 %6, %13 offset:256\n\t"
+      "ds_read_b128 %7, %14 offset:256\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r.part[0]), "=&v"(r.part[1]), "=&v"(r.part[2]), "=&v"(r.part[3]), "=&v"(r.part[4]), "=&v"(r.part[5]),
+        "=&v"(r.part[6]), "=&v"(r.part[7]), "=&v"(w[0]), "=&v"(w[1])
+      : "v"(weights), "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48)
+      : "memory");
+}
+
+// A walk over the chunks of a workgroup's run, [unit, last) in the list of (expert, block). Every
+// member is the same in all lanes.
+struct DownWalk {
+  int unit, last, blocks;  // the chunk's first unit; the run's end; blocks of an expert
+  int u, b, r0, count;     // entry of the list, first block, first row, blocks of the chunk (0: the run is over)
+  int expert, first_row, all;  // of the entry: expert, first row of h, rows
+  int rows, stride;        // rows of the chunk, and rounded up to a power of two
+  __device__ void set(const MoeList& l) {
+    count = 0;
+    if (unit >= last) return;
+    u = unit / blocks;
+    b = unit - u * blocks;
+    expert = __builtin_amdgcn_readfirstlane(l.expert[u]);
+    first_row = __builtin_amdgcn_readfirstlane(l.row[u]);
+    all = __builtin_amdgcn_readfirstlane(__popcll(l.tokens[u]));
+    rows = all - r0 < 32 ? all - r0 : 32;
+    stride = rows <= 1 ? 1 : 1 << (32 - __builtin_clz(rows - 1));
+    const int most = kDownPairs / stride;
+    count = blocks - b < last - unit ? blocks - b : last - unit;
+    if (count > most) count = most;
+  }
+  __device__ void next(const MoeList& l) {
+    r0 += 32;
+    if (r0 >= all) {
+      r0 = 0;
+      unit += count;
+    }
+    set(l);
+  }
+};
+
+template <int DT>
 __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   __shared__ MoeList list;
-  __shared__ float part[kMoeWaves][TILES][16][16];
-  list_experts(a, list);
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = lane % 16, quad = lane / 16;
-  const int blocks = a.inner / kMoeBlock, units = list.count * blocks, n0 = blockIdx.x * 16;
-  v4f total[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) total[t] = v4f{0, 0, 0, 0};
-  const int first = (int)((int64_t)units * wave / kMoeWaves), last = (int)((int64_t)units * (wave + 1) / kMoeWaves);
-  for (int i = first; i < last; ++i) {
-    const int u = i / blocks, b = i - u * blocks, e = list.expert[u];
-    const uint64_t tokens = list.tokens[u];
-    const uint8_t* w = a.down + ((int64_t)e * a.hidden + n0 + col) * a.inner + b * kMoeBlock + 32 * quad;
-    const float scale = a.down_scale[((int64_t)e * (a.hidden / kMoeBlock) + n0 / kMoeBlock) * blocks + b];
-    v4u raw[2], f[4];
-    raw[0] = *reinterpret_cast<const v4u*>(w);
-    raw[1] = *reinterpret_cast<const v4u*>(w + 16);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) f[s] = widen8<AYK_BF16>(raw[s / 2][2 * (s % 2)], raw[s / 2][2 * (s % 2) + 1]);
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      if (((tokens >> (16 * t)) & 0xFFFF) == 0) continue;
-      const int at = 16 * t + col;
-      const bool live = (tokens >> at) & 1;
-      const int row = list.row[u] + __popcll(tokens & ((1ull << at) - 1));
-      const uint16_t* h = a.h + ((int64_t)row * a.inner + b * kMoeBlock + 32 * quad) * 2;
-      v4f sum{0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        v4u hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
-        if (live) {
-          hi = *reinterpret_cast<const v4u*>(h + 16 * s);
-          lo = *reinterpret_cast<const v4u*>(h + 16 * s + 8);
-        }
-        sum = mfma16<AYK_BF16>(f[s], hi, sum);
-        sum = mfma16<AYK_BF16>(f[s], lo, sum);
+  __shared__ alignas(1024) uint8_t stage[2][kDownPairs * kPairBytes];
+  __shared__ alignas(1024) uint8_t rings[kMoeWaves][kRingBytes];
+  extern __shared__ float sums[];  // [tokens][kTokenFloats]
+  list_experts(a, list, reinterpret_cast<uint64_t*>(stage));
+  for (int i = threadIdx.x; i < a.tokens * kTokenFloats; i += kMoeThreads) sums[i] = 0.0f;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quad = lane / 16;
+  const int blocks = a.inner / kMoeBlock, panels = a.hidden / kMoeBlock, n0 = blockIdx.x * kMoeBlock;
+  const int64_t units = (int64_t)__builtin_amdgcn_readfirstlane(list.count) * blocks;
+  DownWalk walk;
+  walk.blocks = blocks;
+  walk.unit = (int)(units * blockIdx.y / gridDim.y);
+  walk.last = (int)(units * (blockIdx.y + 1) / gridDim.y);
+  walk.r0 = 0;
+  walk.set(list);
+  if (walk.count) {
+    // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes.
+    const uint8_t* panel = a.down + (int64_t)(n0 + 16 * wave) * a.inner;
+    const uint32_t lane_at = (uint32_t)col * a.inner + 16 * quad, ring = lds_address(rings[wave]);
+    const int64_t expert_bytes = (int64_t)a.hidden * a.inner;
+    DownWalk ahead = walk;
+    int at = 0, slot = 0;  // block within ahead's chunk; the ring's place that is read, and then filled, next
+    int64_t offset = ahead.expert * expert_bytes + (int64_t)ahead.b * kMoeBlock;
+    // Past the run's end the last block is loaded again, so that the waits count the same loads throughout.
+    auto issue = [&](int to) {
+      load_to_lds(panel + offset, lane_at, ring + 2048 * to);
+      load_to_lds(panel + offset + 64, lane_at, ring + 2048 * to + 1024);
+      if (++at < ahead.count) {
+        offset += kMoeBlock;
+      } else if (ahead.count) {
+        at = 0;
+        ahead.next(list);
+        if (ahead.count) offset = ahead.expert * expert_bytes + (int64_t)ahead.b * kMoeBlock;
       }
-      if (live) total[t] += sum * scale;
+    };
+    // Rows: a wave takes four pairs, two a load, and lane l piece l % 32 of its pair. Pieces are
+    // exchanged within a pair so that the same piece of sixteen pairs lies in sixteen groups of banks.
+    auto fetch = [&](const DownWalk& w, int buffer) {
+      const int shift = __builtin_ctz(w.stride);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int pair = 4 * wave + 2 * i + lane / 32, row = pair & (w.stride - 1), block = pair >> shift;
+        const int64_t r = w.first_row + w.r0 + (row < w.rows ? row : 0);
+        const int k = w.b + (block < w.count ? block : 0);
+        load_to_lds(reinterpret_cast<const uint8_t*>(a.h) + (r * a.inner + k * kMoeBlock) * 4 + 16 * ((lane % 32) ^ (pair & 15)),
+                    lds_address(stage[buffer] + (4 * wave + 2 * i) * kPairBytes));
+      }
+    };
+    fetch(walk, 0);
+#pragma unroll
+    for (int s = 0; s < kDownAhead; ++s) issue(s);
+    wait_loads<2 * kDownAhead>();
+    __builtin_amdgcn_s_barrier();
+    int buffer = 0;
+    while (true) {
+      DownWalk following = walk;
+      following.next(list);
+      fetch(following.count ? following : walk, buffer ^ 1);
+      // (by way of the constant address space: a vector load would not be among the counted ones)
+      const auto scale = (__attribute__((address_space(4))) const float*)a.down_scale + ((int64_t)walk.expert * panels + blockIdx.x) * blocks + walk.b;
+      const bool two = walk.rows > 16;
+      v4f total[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      for (int c = 0; c < walk.count; ++c) {
+        const int pair = c * walk.stride + (col & (walk.stride - 1));
+        const uint32_t rows = lds_address(stage[buffer]) + pair * kPairBytes + 16 * ((4 * quad) ^ (pair & 15));
+        const float sc = scale[c];
+        v4u w[2], f[4];
+        DownRows r;
+        wait_loads<2 * (kDownAhead - 1)>();
+        read_block(ring + 2048 * slot + 16 * lane, rows, w, r);
+        issue(slot);
+        slot = (slot + 1) % kDownAhead;
+        v4f sum[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          f[s] = widen8<AYK_BF16>(w[s / 2][2 * (s % 2)], w[s / 2][2 * (s % 2) + 1]);
+          sum[0] = mfma16<AYK_BF16>(f[s], r.part[2 * s], sum[0]);
+          sum[1] = mfma16<AYK_BF16>(f[s], r.part[2 * s + 1], sum[1]);
+        }
+        total[0] += (sum[0] + sum[1]) * sc;
+        if (two) {
+          read_rows(rows + 16 * kPairBytes, r);
+          sum[0] = sum[1] = v4f{0, 0, 0, 0};
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            sum[0] = mfma16<AYK_BF16>(f[s], r.part[2 * s], sum[0]);
+            sum[1] = mfma16<AYK_BF16>(f[s], r.part[2 * s + 1], sum[1]);
+          }
+          total[1] += (sum[0] + sum[1]) * sc;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (16 * r + col < walk.rows) {
+          float* to = sums + nth_bit(list.tokens[walk.u], walk.r0 + 16 * r + col) * kTokenFloats + 16 * wave + 4 * quad;
+          *reinterpret_cast<v4f*>(to) += total[r];
+        }
+      }
+      if (following.count == 0) break;
+      // The next rows are older than the weights asked for since: those of kDownAhead blocks or more
+      // have been waited past them, of fewer they are counted.
+      static_assert(kDownAhead == 4, "the counts below");
+      if (walk.count == 1) wait_loads<2>();
+      else if (walk.count == 2) wait_loads<4>();
+      else if (walk.count == 3) wait_loads<6>();
+      __builtin_amdgcn_s_barrier();
+      buffer ^= 1;
+      walk = following;
     }
+    wait_loads<0>();  // no load may still write LDS, and those counted by the compiler begin anew
   }
-#pragma unroll
-  for (int t = 0; t < TILES; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) part[wave][t][col][4 * quad + i] = total[t][i];
+  const int tokens = a.tokens;
   __syncthreads();
-  for (int i = threadIdx.x; i < TILES * 256; i += kMoeThreads) {
-    const int t = i / 16, n = i % 16;
-    if (t >= a.tokens) continue;
-    float sum = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kMoeWaves; ++v) sum += part[v][t / 16][t % 16][n];
-    store_f32(a.out, DT, t * a.ldo + n0 + n, sum);
+  if (gridDim.y == 1) {
+    for (int i = threadIdx.x; i < tokens * kMoeBlock; i += kMoeThreads)
+      store_f32(a.out, DT, i / kMoeBlock * a.ldo + n0 + i % kMoeBlock, sums[i / kMoeBlock * kTokenFloats + i % kMoeBlock]);
+    return;
   }
+  // Partial results pass from one chip part's cache to another's as atomics of the agent's scope, which
+  // go to memory and come from there. A fence would do the same for plain ones by writing back the
+  // whole cache, once a wave: 35 us of the launch. What orders them is that the stores are done, for all
+  // waves, before the count goes up.
+  const int64_t plane = (int64_t)tokens * a.hidden;
+  for (int i = threadIdx.x; i < tokens * kMoeBlock; i += kMoeThreads)
+    __hip_atomic_store(a.partial + blockIdx.y * plane + (int64_t)(i / kMoeBlock) * a.hidden + n0 + i % kMoeBlock,
+                       sums[i / kMoeBlock * kTokenFloats + i % kMoeBlock], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  wait_loads<0>();  // and stores
+  __syncthreads();
+  __shared__ int arrived;
+  if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(a.arrived + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived != (int)gridDim.y - 1) return;
+  for (int i = threadIdx.x; i < tokens * kMoeBlock; i += kMoeThreads) {
+    const float* p = a.partial + (int64_t)(i / kMoeBlock) * a.hidden + n0 + i % kMoeBlock;
+    float sum = 0.0f;
+    for (int r = 0; r < (int)gridDim.y; ++r) sum += __hip_atomic_load(p + r * plane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    store_f32(a.out, DT, i / kMoeBlock * a.ldo + n0 + i % kMoeBlock, sum);
+  }
+}
+
+// Runs of a channel block in the second launch: as many as give the chip a workgroup a CU, none
+// shorter than two blocks of what the call may name at most.
+int down_runs(int64_t tokens, int64_t topk, int64_t experts, int64_t hidden, int64_t inner) {
+  const int64_t pairs = tokens * topk, used = pairs < experts ? pairs : experts;
+  const int64_t units = used * (inner / kMoeBlock), most = cdiv(units, 2), want = 256 / (hidden / kMoeBlock);
+  const int64_t runs = want < most ? want : most;
+  return (int)(runs < 1 ? 1 : runs);
 }
 
 template <int DT>
@@ -224,11 +411,14 @@ int launch_moe(const MoeArgs& a, hipStream_t st) {
   const int64_t pairs = (int64_t)a.tokens * a.topk, used = pairs < a.experts ? pairs : a.experts;
   const int64_t items = used * (a.inner / 16);
   hipLaunchKernelGGL((moe_gate_up_kernel<DT>), dim3((unsigned)(items < 512 ? items : 512)), dim3(kMoeThreads), 0, st, a);
-  const dim3 grid((unsigned)(a.hidden / 16));
-  if (a.tokens <= 16) hipLaunchKernelGGL((moe_down_kernel<DT, 1>), grid, dim3(kMoeThreads), 0, st, a);
-  else if (a.tokens <= 32) hipLaunchKernelGGL((moe_down_kernel<DT, 2>), grid, dim3(kMoeThreads), 0, st, a);
-  else hipLaunchKernelGGL((moe_down_kernel<DT, 4>), grid, dim3(kMoeThreads), 0, st, a);
+  const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner));
+  hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), a.tokens * kTokenFloats * sizeof(float), st, a);
   return check_launch("fp8_block_moe_small");
+}
+
+// Rows of h: a token's experts, each once.
+size_t moe_h_bytes(int64_t tokens, int64_t topk, int64_t experts, int64_t inner) {
+  return (size_t)(tokens * (topk < experts ? topk : experts) * inner) * 4;
 }
 
 }  // namespace
@@ -238,11 +428,12 @@ using namespace ayk;
 
 extern "C" {
 
-size_t ayk_fp8_block_moe_small_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts, int64_t inner) {
-  if (tokens < 1 || tokens > kMoeTokens || topk < 1 || topk > 0x7FFF || experts < 1 || experts > kMoeExperts || inner < 1 || inner > 0x7FFFFFFF)
+size_t ayk_fp8_block_moe_small_scratch_bytes(int64_t tokens, int64_t topk, int64_t experts, int64_t hidden, int64_t inner) {
+  if (tokens < 1 || tokens > kMoeTokens || topk < 1 || topk > kMoeTopk || experts < 1 || experts > kMoeExperts || hidden < kMoeBlock ||
+      hidden > kMoeWidth || inner < kMoeBlock || inner > kMoeWidth)
     return 0;
-  const int64_t most = topk < experts ? topk : experts;  // rows of h: a token's experts, each once
-  return (size_t)(tokens * most * inner) * 4;
+  return moe_h_bytes(tokens, topk, experts, inner) +
+         (size_t)(down_runs(tokens, topk, experts, hidden, inner) * tokens * hidden + hidden / kMoeBlock) * sizeof(float);
 }
 
 int ayk_fp8_block_moe_small(const void* x, int x_dtype, int64_t ldx, int64_t tokens, const void* gate_up, const float* gate_up_scale,
@@ -253,10 +444,10 @@ int ayk_fp8_block_moe_small(const void* x, int x_dtype, int64_t ldx, int64_t tok
   if (x_dtype != AYK_F16 && x_dtype != AYK_BF16) return fail(AYK_EINVAL, "%s: x must be float16 or bfloat16", op);
   if (tokens < 0 || tokens > kMoeTokens) return fail(AYK_EINVAL, "%s: at most %d tokens, got %lld", op, kMoeTokens, (long long)tokens);
   if (experts < 1 || experts > kMoeExperts) return fail(AYK_EINVAL, "%s: 1 to %d experts, got %lld", op, kMoeExperts, (long long)experts);
-  if (hidden < kMoeBlock || inner < kMoeBlock || hidden % kMoeBlock || inner % kMoeBlock || hidden > 0x1000000 || inner > 0x1000000)
+  if (hidden < kMoeBlock || inner < kMoeBlock || hidden % kMoeBlock || inner % kMoeBlock || hidden > kMoeWidth || inner > kMoeWidth)
     return fail(AYK_EINVAL, "%s: hidden and inner must be multiples of %d, got %lld and %lld", op, kMoeBlock, (long long)hidden,
                 (long long)inner);
-  if (topk < 1 || topk > 0x7FFF) return fail(AYK_EINVAL, "%s: bad topk %lld", op, (long long)topk);
+  if (topk < 1 || topk > kMoeTopk) return fail(AYK_EINVAL, "%s: bad topk %lld", op, (long long)topk);
   if (ldx < hidden || ldo < hidden) return fail(AYK_EINVAL, "%s: row strides must be at least hidden", op);
   if (tokens == 0) return AYK_OK;
   if (x == nullptr || gate_up == nullptr || gate_up_scale == nullptr || down == nullptr || down_scale == nullptr || weights == nullptr ||
@@ -265,7 +456,7 @@ int ayk_fp8_block_moe_small(const void* x, int x_dtype, int64_t ldx, int64_t tok
   if (!aligned16(x) || ldx % 8 || !aligned16(gate_up) || !aligned16(down))
     return fail(AYK_EINVAL, "%s: x's rows and the weights must be 16-byte aligned", op);
   if (workspace == nullptr || !aligned16(workspace) ||
-      workspace_bytes < ayk_fp8_block_moe_small_workspace_bytes(tokens, topk, experts, inner))
+      workspace_bytes < ayk_fp8_block_moe_small_scratch_bytes(tokens, topk, experts, hidden, inner))
     return fail(AYK_EWORKSPACE, "%s: the workspace is missing, misaligned or too small", op);
   if (int rc = check_device()) return rc;
   MoeArgs a{};
@@ -280,6 +471,8 @@ int ayk_fp8_block_moe_small(const void* x, int x_dtype, int64_t ldx, int64_t tok
   a.out = static_cast<uint16_t*>(out);
   a.ldo = ldo;
   a.h = static_cast<uint16_t*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + moe_h_bytes(tokens, topk, experts, inner));
+  a.arrived = reinterpret_cast<int*>(a.partial + down_runs(tokens, topk, experts, hidden, inner) * tokens * hidden);
   a.tokens = (int)tokens, a.topk = (int)topk, a.experts = (int)experts, a.hidden = (int)hidden, a.inner = (int)inner;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return x_dtype == AYK_BF16 ? launch_moe<AYK_BF16>(a, st) : launch_moe<AYK_F16>(a, st);

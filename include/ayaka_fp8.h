@@ -211,7 +211,8 @@ int ayk_fp8_block_moe_small(const void* x, int x_dtype, int64_t ldx, int64_t tok
                             const float* gate_up_scale, const void* down, const float* down_scale, int64_t experts,
                             int64_t hidden, int64_t inner, const float* weights, const int32_t* ids, int64_t topk,
                             void* out, int64_t ldo, void* workspace, size_t workspace_bytes, ayk_stream_t stream);
-size_t ayk_fp8_block_moe_small_workspace_bytes(int64_t tokens, int64_t topk, int64_t experts, int64_t inner);
+size_t ayk_fp8_block_moe_small_scratch_bytes(int64_t tokens, int64_t topk, int64_t experts, int64_t hidden,
+                                             int64_t inner);
 
 /* Replaces ayaka::mxfp8_scaled_mm (gemm/fp8_mxfp8_gemm.py:163; oracle reference/gemm.py:73-92).
  * out = sum_g (a[:, g] @ w[:, g]^T) * 2^(a_scale[m,g]-127) * 2^(w_scale[n,g]-127) + bias

@@ -133,10 +133,14 @@ def test_c_entries_with_nothing_to_do():
 def test_workspaces():
     for change in ({"ws": None}, {"ws": 8}, {"wb": 1}):
         assert _moe(**change) == _lib.AYK_EWORKSPACE
-    moe = lambda *a: _lib.query("ayk_fp8_block_moe_small_workspace_bytes", *a)  # noqa: E731
-    assert moe(64, 8, 256, 2048) == 64 * 8 * 2048 * 4
-    assert moe(64, 100, 8, 2048) == 64 * 8 * 2048 * 4  # a row for every expert that a token can name
-    for bad in ((65, 8, 256, 2048), (0, 8, 256, 2048), (64, 0, 256, 2048), (64, 8, 1025, 2048), (64, 8, 256, 0)):
+    moe = lambda *a: _lib.query("ayk_fp8_block_moe_small_scratch_bytes", *a)  # noqa: E731
+    # what lies between the projections, four partial results of 56 channel blocks, a counter of each
+    assert moe(64, 8, 256, 7168, 2048) == 64 * 8 * 2048 * 4 + 4 * 64 * 7168 * 4 + 56 * 4
+    # a row for every expert that a token can name
+    assert moe(64, 100, 8, 7168, 2048) - moe(64, 8, 8, 7168, 2048) == 0
+    assert moe(1, 1, 1, 128, 128) == 128 * 4 + 128 * 4 + 4
+    for bad in ((65, 8, 256, 7168, 2048), (0, 8, 256, 7168, 2048), (64, 0, 256, 7168, 2048), (64, 8, 1025, 7168, 2048),
+                (64, 8, 256, 7168, 0), (64, 8, 256, 0, 2048), (64, 8, 256, 2**25, 2048), (64, 2**15, 256, 7168, 2048)):
         assert moe(*bad) == 0
     split = lambda *a: _lib.query("ayk_paged_decode_attention_mxfp4_split_bytes", *a)  # noqa: E731
     for dim, width in ((32, 64), (64, 64), (96, 128), (128, 128), (160, 256)):
