@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kMoeTokens = 64;     // tokens of a call, at most: a bit each of a mask
 constexpr int kMoeExperts = 1024;  // experts of a layer, at most: a mask each in LDS
+constexpr int kMoePairs = 1024;   // (token, choice) pairs that the first launch holds in LDS
 constexpr int kMoeTopk = 0x7FFF;
 constexpr int kMoeWidth = 0x1000000;
 constexpr int kMoeThreads = 512;
@@ -88,99 +89,9 @@ __device__ inline v4u widen8(uint32_t a, uint32_t b) {
   return v4u{widen2<AYK_E4M3, DT, false>(a), widen2<AYK_E4M3, DT, true>(a), widen2<AYK_E4M3, DT, false>(b), widen2<AYK_E4M3, DT, true>(b)};
 }
 
-// Gate and up projections of sixteen inner channels for the tokens of one expert, the activation, and h.
-// The waves of a workgroup take blocks of 128 k in turn and join their sums in LDS.
-template <int DT>
-__global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) {
-  __shared__ MoeList list;
-  __shared__ float part[kMoeWaves][2][16][16];
-  list_experts(a, list, reinterpret_cast<uint64_t*>(part));
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, col = lane % 16, quad = lane / 16;
-  const int slices = a.inner / 16, blocks = a.hidden / kMoeBlock;
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < blocks; i += kMoeThreads) a.arrived[i] = 0;
-  for (int item = blockIdx.x; item < list.count * slices; item += gridDim.x) {
-    const int u = item / slices, n0 = (item - u * slices) * 16, e = list.expert[u];
-    const uint64_t tokens = list.tokens[u];
-    const uint8_t* gate = a.gate_up + ((int64_t)e * 2 * a.inner + n0 + col) * a.hidden + 16 * quad;
-    const uint8_t* up = gate + (int64_t)a.inner * a.hidden;
-    const float* gate_scale = a.gate_up_scale + ((int64_t)e * 2 * (a.inner / kMoeBlock) + n0 / kMoeBlock) * blocks;
-    const float* up_scale = gate_scale + (int64_t)(a.inner / kMoeBlock) * blocks;
-    const int rows = __popcll(tokens);
-    for (int r0 = 0; r0 < rows; r0 += 16) {
-      const bool live = r0 + col < rows;
-      const uint16_t* x = a.x + nth_bit(tokens, r0 + col) * a.ldx + 16 * quad;
-      v4f g{0, 0, 0, 0}, w{0, 0, 0, 0};
-      for (int b = wave; b < blocks; b += kMoeWaves) {
-        v4u gw[2], uw[2], xs[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          gw[i] = *reinterpret_cast<const v4u*>(gate + b * kMoeBlock + 64 * i);
-          uw[i] = *reinterpret_cast<const v4u*>(up + b * kMoeBlock + 64 * i);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          xs[i] = v4u{0, 0, 0, 0};
-          if (live) xs[i] = *reinterpret_cast<const v4u*>(x + b * kMoeBlock + 64 * (i / 2) + 8 * (i % 2));
-        }
-        v4f gs{0, 0, 0, 0}, us{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          gs = mfma16<DT>(widen8<DT>(gw[i / 2][2 * (i % 2)], gw[i / 2][2 * (i % 2) + 1]), xs[i], gs);
-          us = mfma16<DT>(widen8<DT>(uw[i / 2][2 * (i % 2)], uw[i / 2][2 * (i % 2) + 1]), xs[i], us);
-        }
-        const float sg = gate_scale[b], su = up_scale[b];
-        g += gs * sg;
-        w += us * su;
-      }
-      __syncthreads();  // the last tile's readers are done
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        part[wave][0][col][4 * quad + i] = g[i];
-        part[wave][1][col][4 * quad + i] = w[i];
-      }
-      __syncthreads();
-      if (threadIdx.x < 256) {
-        const int r = threadIdx.x / 16, n = threadIdx.x % 16;
-        if (r0 + r < rows) {
-          float gate_sum = 0.0f, up_sum = 0.0f;
-#pragma unroll
-          for (int v = 0; v < kMoeWaves; ++v) {
-            gate_sum += part[v][0][r][n];
-            up_sum += part[v][1][r][n];
-          }
-          const int t = nth_bit(tokens, r0 + r);
-          float weight = 0.0f;
-          for (int j = 0; j < a.topk; ++j)
-            if (a.ids[t * a.topk + j] == e) weight += a.weights[t * a.topk + j];
-          const float y = weight * (gate_sum / (1.0f + expf(-gate_sum)) * up_sum);
-          const uint16_t hi = f32_to_bf16_bits(y);
-          const float rest = y - bf16_bits_to_f32(hi);
-          uint16_t* to = a.h + ((int64_t)(list.row[u] + r0 + r) * a.inner + n0 + n / 8 * 8) * 2 + n % 8;
-          to[0] = hi;
-          to[8] = f32_to_bf16_bits(rest == rest ? rest : 0.0f);  // an infinity has no second part
-        }
-      }
-    }
-  }
-}
-
-// 128 output channels of all tokens, sixteen a wave. The blocks of 128 k of all experts in a row are one
-// list, of which every workgroup of a channel block takes an equal run; the runs' sums meet in fp32
-// partial results, which the last workgroup to finish adds in the runs' order. Sums of an expert's
-// rows join those of their tokens in LDS, where each lane owns its cells: results do not depend on
-// the order of waves.
-//
-// All that the loop reads comes through LDS by direct loads: the weights of a wave kDownAhead blocks
-// ahead (registers would have to be named at compile time, which blocks of unequal chunks do not
-// allow), the rows of h, which the waves share, in chunks of up to kDownPairs (row, block) pairs of
-// 512 bytes, a chunk ahead. The waits are counted by hand: the loads of a wave land in order.
-constexpr int kDownAhead = 4;
-constexpr int kDownPairs = 32;
-constexpr int kPairBytes = 4 * kMoeBlock;
-constexpr int kTokenFloats = kMoeBlock + 4;  // a token's channels, and a shift of four banks
-constexpr int kRingBytes = kDownAhead * 2048;
-
+// All that the kernels' loops read comes through LDS by direct loads, some blocks ahead: registers
+// would have to be named at compile time, which blocks of unequal chunks do not allow. The waits are
+// counted by hand: the loads of a wave land in order.
 __device__ inline uint32_t lds_address(const void* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
 }
@@ -196,6 +107,242 @@ __device__ inline void load_to_lds(const uint8_t* from, uint32_t lds) {
 // Until at most N of the wave's loads are in flight.
 template <int N>
 __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+// A barrier behind this wave's accesses to LDS; direct loads stay in flight (__syncthreads waits for
+// stores to global memory, and with them for every load).
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+// Sixteen bytes a lane of both loads of a half block of weights; with it the k slots of the four steps
+// of this lane's row. The reads are done when the block ends.
+__device__ inline void read_half(uint32_t weights, v4u (&w)[2]) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(w[0]), "=&v"(w[1])
+               : "v"(weights)
+               : "memory");
+}
+__device__ inline void read_rows_and_half(uint32_t weights, uint32_t at, v4u (&w)[2], v4u (&x)[4]) {
+  asm volatile(
+      "ds_read_b128 %4, %6\n\tds_read_b128 %5, %6 offset:1024\n\tds_read_b128 %0, %7\n\tds_read_b128 %1, %8\n\t"
+      "ds_read_b128 %2, %9\n\tds_read_b128 %3, %10\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(w[0]), "=&v"(w[1])
+      : "v"(weights), "v"(at), "v"(at ^ 16), "v"(at ^ 128), "v"(at ^ 144)
+      : "memory");
+}
+
+
+// Gate and up projections of sixteen inner channels for the tokens of one expert, the activation, and h:
+// an item. The waves of a workgroup take blocks of 128 k in turn and join their sums in LDS. A wave's
+// weights run kGateAhead half blocks ahead, across items; the tokens' rows of x come in chunks
+// of up to kGatePairs (row, block) pairs of 256 bytes, a chunk ahead.
+constexpr int kGateAhead = 4;  // half blocks: gate or up rows
+constexpr int kGatePairs = 128;
+constexpr int kGatePairBytes = 2 * kMoeBlock;
+constexpr int kGateRows = 16;  // of a pass over an item
+
+// A walk over the chunks of a workgroup's items. Every member is the same in all lanes.
+struct GateWalk {
+  int item, items, step, slices, blocks;
+  int u, slice, r0, b0, count;  // list entry, sixteen channels, first row, first block, blocks (0: no more)
+  int expert, first_row, all, rows, stride;
+  uint64_t tokens;  // of the pass
+  __device__ void enter(const MoeList& l) {  // item, r0
+    count = 0;
+    b0 = 0;
+    if (item >= items) return;
+    u = item / slices;
+    slice = item - u * slices;
+    expert = __builtin_amdgcn_readfirstlane(l.expert[u]);
+    first_row = __builtin_amdgcn_readfirstlane(l.row[u]);
+    const uint64_t named = l.tokens[u];
+    tokens = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)named) |
+             (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(named >> 32)) << 32;
+    all = __popcll(tokens);
+    for (int r = 0; r < r0; ++r) tokens &= tokens - 1;
+    rows = all - r0 < kGateRows ? all - r0 : kGateRows;
+    stride = rows <= 1 ? 1 : 1 << (32 - __builtin_clz(rows - 1));
+    size();
+  }
+  __device__ void size() {
+    const int most = kGatePairs / stride;  // whole eights: every wave's share
+    count = blocks - b0 < most ? blocks - b0 : most;
+  }
+  __device__ bool ends_item() const { return b0 + count == blocks; }
+  __device__ void next(const MoeList& l) {
+    if (!ends_item()) {
+      b0 += count;
+      size();
+      return;
+    }
+    r0 += kGateRows;
+    if (r0 >= all) {
+      r0 = 0;
+      item += step;
+    }
+    enter(l);
+  }
+};
+
+template <int DT>
+__global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) {
+  __shared__ MoeList list;
+  __shared__ alignas(1024) uint8_t stage[2][kGatePairs * kGatePairBytes];
+  __shared__ alignas(1024) uint8_t rings[kMoeWaves][kGateAhead * 2048];
+  __shared__ int32_t ids[kMoePairs];
+  __shared__ float weights[kMoePairs];
+  const int pairs = a.tokens * a.topk;
+  const bool held = pairs <= kMoePairs;  // else they are read where they are used
+  if (held)
+    for (int p = threadIdx.x; p < pairs; p += kMoeThreads) {
+      ids[p] = a.ids[p];
+      weights[p] = a.weights[p];
+    }
+  list_experts(a, list, reinterpret_cast<uint64_t*>(stage));
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quad = lane / 16;
+  const int blocks = a.hidden / kMoeBlock, block_rows = a.inner / kMoeBlock;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < blocks; i += kMoeThreads) a.arrived[i] = 0;
+  GateWalk walk;
+  walk.slices = a.inner / 16;
+  walk.blocks = blocks;
+  walk.item = blockIdx.x;
+  walk.step = gridDim.x;
+  walk.items = __builtin_amdgcn_readfirstlane(list.count) * walk.slices;
+  walk.r0 = 0;
+  walk.enter(list);
+  if (walk.count == 0) return;
+
+  // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes. A wave's
+  // blocks of a chunk are its number and every eighth from there; past the last the same loads are
+  // issued again, so that the waits count the same throughout.
+  const uint32_t lane_at = (uint32_t)col * a.hidden + 16 * quad, ring = lds_address(rings[wave]);
+  GateWalk ahead = walk;
+  int at = wave;  // block within ahead's chunk
+  while (ahead.count && at >= ahead.count) ahead.next(list);
+  const int64_t up_bytes = (int64_t)a.inner * a.hidden;
+  const uint8_t* from = a.gate_up;
+  auto point = [&]() {
+    if (ahead.count)
+      from = a.gate_up + ((int64_t)ahead.expert * 2 * a.inner + 16 * ahead.slice) * a.hidden + (int64_t)(ahead.b0 + at) * kMoeBlock;
+  };
+  point();
+  auto issue = [&](int to, bool up) {
+    load_to_lds(from + (up ? up_bytes : 0), lane_at, ring + 2048 * to);
+    load_to_lds(from + (up ? up_bytes : 0) + 64, lane_at, ring + 2048 * to + 1024);
+    if (!up || !ahead.count) return;
+    at += kMoeWaves;
+    if (at >= ahead.count) {
+      do {
+        ahead.next(list);
+        at = wave;
+      } while (ahead.count && at >= ahead.count);
+    }
+    point();
+  };
+  // Rows: a wave takes sixteen pairs, four a load, and lane l piece l % 16 of its pair. Pieces are
+  // exchanged within a pair so that the same piece of sixteen rows lies in sixteen groups of banks.
+  auto fetch = [&](const GateWalk& w, int buffer) {
+    const int shift = __builtin_ctz(w.stride);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pair = 16 * wave + 4 * i + lane / 16, row = pair & (w.stride - 1), block = pair >> shift;
+      const int64_t t = nth_bit(w.tokens, row < w.rows ? row : 0);
+      const int k = w.b0 + (block < w.count ? block : 0);
+      load_to_lds(reinterpret_cast<const uint8_t*>(a.x + t * a.ldx + (int64_t)k * kMoeBlock) + 16 * ((lane % 16) ^ (pair & 15)),
+                  lds_address(stage[buffer] + (16 * wave + 4 * i) * kGatePairBytes));
+    }
+  };
+  fetch(walk, 0);
+#pragma unroll
+  for (int s = 0; s < kGateAhead; ++s) issue(s, s % 2 == 1);
+  wait_loads<2 * kGateAhead>();
+  __builtin_amdgcn_s_barrier();
+  int buffer = 0, slot = 0;
+  v4f g{0, 0, 0, 0}, w{0, 0, 0, 0};
+  while (true) {
+    GateWalk following = walk;
+    following.next(list);
+    fetch(following.count ? following : walk, buffer ^ 1);
+    // (by way of the constant address space: a vector load would not be among the counted ones)
+    const auto gate_scale = (__attribute__((address_space(4))) const float*)a.gate_up_scale +
+                            ((int64_t)walk.expert * 2 * block_rows + walk.slice / 8) * blocks + walk.b0;
+    const auto up_scale = gate_scale + (int64_t)block_rows * blocks;
+    int mine = 0;
+    for (int c = wave; c < walk.count; c += kMoeWaves, ++mine) {
+      const int pair = c * walk.stride + (col & (walk.stride - 1));
+      const uint32_t rows = lds_address(stage[buffer]) + pair * kGatePairBytes + 16 * ((2 * quad) ^ (pair & 15));
+      const float sg = gate_scale[c], su = up_scale[c];
+      v4u xs[4], raw[2];
+      v4f sum{0, 0, 0, 0}, other{0, 0, 0, 0};
+      wait_loads<2 * (kGateAhead - 1)>();
+      read_rows_and_half(ring + 2048 * slot + 16 * lane, rows, raw, xs);
+      issue(slot, false);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = mfma16<DT>(widen8<DT>(raw[i / 2][2 * (i % 2)], raw[i / 2][2 * (i % 2) + 1]), xs[i], sum);
+      g += sum * sg;
+      wait_loads<2 * (kGateAhead - 1)>();
+      read_half(ring + 2048 * (slot + 1) + 16 * lane, raw);
+      issue(slot + 1, true);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) other = mfma16<DT>(widen8<DT>(raw[i / 2][2 * (i % 2)], raw[i / 2][2 * (i % 2) + 1]), xs[i], other);
+      w += other * su;
+      slot = (slot + 2) % kGateAhead;
+    }
+    // The next rows are older than the weights asked for since: those of two blocks have been waited
+    // past them, of one they are counted.
+    if (mine == 1) wait_loads<4>();
+    else if (mine == 0) wait_loads<0>();
+    if (walk.ends_item()) {
+      auto part = reinterpret_cast<float(*)[2][16][16]>(stage[buffer]);  // [wave]: its rows have all been read
+      __builtin_amdgcn_s_barrier();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part[wave][0][col][4 * quad + i] = g[i];
+        part[wave][1][col][4 * quad + i] = w[i];
+      }
+      g = w = v4f{0, 0, 0, 0};
+      lds_barrier();
+      const int r = threadIdx.x / 16, n = threadIdx.x % 16;
+      if (r < walk.rows) {
+        float gate_sum = 0.0f, up_sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kMoeWaves; ++v) {
+          gate_sum += part[v][0][r][n];
+          up_sum += part[v][1][r][n];
+        }
+        const int t = nth_bit(walk.tokens, r);
+        float weight = 0.0f;
+        if (held) {
+          for (int p = t * a.topk; p < (t + 1) * a.topk; ++p) weight += ids[p] == walk.expert ? weights[p] : 0.0f;
+        } else {
+          for (int p = t * a.topk; p < (t + 1) * a.topk; ++p)
+            if (a.ids[p] == walk.expert) weight += a.weights[p];
+        }
+        const float y = weight * (gate_sum / (1.0f + expf(-gate_sum)) * up_sum);
+        const uint16_t hi = f32_to_bf16_bits(y);
+        const float rest = y - bf16_bits_to_f32(hi);
+        uint16_t* to = a.h + ((int64_t)(walk.first_row + walk.r0 + r) * a.inner + 16 * walk.slice + n / 8 * 8) * 2 + n % 8;
+        to[0] = hi;
+        to[8] = f32_to_bf16_bits(rest == rest ? rest : 0.0f);  // an infinity has no second part
+      }
+    }
+    if (following.count == 0) break;
+    lds_barrier();
+    buffer ^= 1;
+    walk = following;
+  }
+  wait_loads<0>();  // no load may still write LDS
+}
+
+// 128 output channels of all tokens, sixteen a wave. The blocks of 128 k of all experts in a row are one
+// list, of which every workgroup of a channel block takes an equal run; the runs' sums meet in fp32
+// partial results, which the last workgroup to finish adds in the runs' order. Sums of an expert's
+// rows join those of their tokens in LDS, where each lane owns its cells: results do not depend on
+// the order of waves.
+// A wave's weights run kDownAhead blocks ahead; the rows of h, which the waves share, come in chunks of
+// up to kDownPairs (row, block) pairs of 512 bytes, a chunk ahead.
+constexpr int kDownAhead = 4;
+constexpr int kDownPairs = 32;
+constexpr int kPairBytes = 4 * kMoeBlock;
+constexpr int kTokenFloats = kMoeBlock + 4;  // a token's channels, and a shift of four banks
+constexpr int kRingBytes = kDownAhead * 2048;
 
 // A block's weights (the lane's sixteen bytes of two loads) and the first and second parts of eight
 // rows' k slots for its four steps, from LDS; the reads are done when the block ends.
@@ -410,7 +557,7 @@ template <int DT>
 int launch_moe(const MoeArgs& a, hipStream_t st) {
   const int64_t pairs = (int64_t)a.tokens * a.topk, used = pairs < a.experts ? pairs : a.experts;
   const int64_t items = used * (a.inner / 16);
-  hipLaunchKernelGGL((moe_gate_up_kernel<DT>), dim3((unsigned)(items < 512 ? items : 512)), dim3(kMoeThreads), 0, st, a);
+  hipLaunchKernelGGL((moe_gate_up_kernel<DT>), dim3((unsigned)(items < 256 ? items : 256)), dim3(kMoeThreads), 0, st, a);
   const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner));
   hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), a.tokens * kTokenFloats * sizeof(float), st, a);
   return check_launch("fp8_block_moe_small");
