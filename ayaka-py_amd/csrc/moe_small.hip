@@ -78,11 +78,19 @@ __device__ inline void list_experts(const MoeArgs& a, MoeList& l, uint64_t* mask
   __syncthreads();
 }
 
-// The n-th set bit of a mask (0 where there are fewer).
-__device__ inline int nth_bit(uint64_t mask, int n) {
-  for (int i = 0; i < n; ++i) mask &= mask - 1;
-  return mask ? __builtin_ctzll(mask) : 0;
+// Lane r: the r-th token of a mask (a lane past the last holds any token).
+__device__ inline int token_table(uint64_t mask) {
+  const int lane = threadIdx.x % kWave, rank = __popcll(mask & ((1ull << lane) - 1));
+  // every lane pushes its number to a lane of its own: the set ones to the front, in order
+  const int to = (mask >> lane) & 1 ? rank : __popcll(mask) + lane - rank;
+  return __builtin_amdgcn_ds_permute(4 * to, lane);
 }
+__device__ inline int token_of(int table, int row) { return __builtin_amdgcn_ds_bpermute(4 * row, table); }
+__device__ inline uint64_t uniform(uint64_t v) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
+}
+__device__ inline int power_of_two_from(int n) { return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)); }
 
 template <int DT>
 __device__ inline v4u widen8(uint32_t a, uint32_t b) {
@@ -104,6 +112,10 @@ __device__ inline void load_to_lds(const uint8_t* from, uint32_t at, uint32_t ld
 __device__ inline void load_to_lds(const uint8_t* from, uint32_t lds) {
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(lds));
 }
+// Four bytes a lane to lds + 4 lane.
+__device__ inline void word_to_lds(const float* from, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" : : "v"(from), "{m0}"(lds));
+}
 // Until at most N of the wave's loads are in flight.
 template <int N>
 __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
@@ -118,15 +130,15 @@ __device__ inline void read_half(uint32_t weights, v4u (&w)[2]) {
                : "v"(weights)
                : "memory");
 }
-__device__ inline void read_rows_and_half(uint32_t weights, uint32_t at, v4u (&w)[2], v4u (&x)[4]) {
+__device__ inline void read_rows_and_half(uint32_t weights, uint32_t at, uint32_t scales, v4u (&w)[2], v4u (&x)[4], float (&scale)[2]) {
   asm volatile(
-      "ds_read_b128 %4, %6\n\tds_read_b128 %5, %6 offset:1024\n\tds_read_b128 %0, %7\n\tds_read_b128 %1, %8\n\t"
-      "ds_read_b128 %2, %9\n\tds_read_b128 %3, %10\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(w[0]), "=&v"(w[1])
-      : "v"(weights), "v"(at), "v"(at ^ 16), "v"(at ^ 128), "v"(at ^ 144)
+      "ds_read_b128 %4, %8\n\tds_read_b128 %5, %8 offset:1024\n\tds_read_b128 %0, %9\n\tds_read_b128 %1, %10\n\t"
+      "ds_read_b128 %2, %11\n\tds_read_b128 %3, %12\n\tds_read_b32 %6, %13\n\tds_read_b32 %7, %13 offset:64\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(w[0]), "=&v"(w[1]), "=&v"(scale[0]), "=&v"(scale[1])
+      : "v"(weights), "v"(at), "v"(at ^ 16), "v"(at ^ 128), "v"(at ^ 144), "v"(scales)
       : "memory");
 }
-
 
 // Gate and up projections of sixteen inner channels for the tokens of one expert, the activation, and h:
 // an item. The waves of a workgroup take blocks of 128 k in turn and join their sums in LDS. A wave's
@@ -137,30 +149,27 @@ constexpr int kGatePairs = 128;
 constexpr int kGatePairBytes = 2 * kMoeBlock;
 constexpr int kGateRows = 16;  // of a pass over an item
 
-// A walk over the chunks of a workgroup's items. Every member is the same in all lanes.
+// A walk over the chunks of a workgroup's items, a run of consecutive ones. All but `table` is the
+// same in all lanes.
 struct GateWalk {
-  int item, items, step, slices, blocks;
+  int item, last, slices, blocks;
   int u, slice, r0, b0, count;  // list entry, sixteen channels, first row, first block, blocks (0: no more)
   int expert, first_row, all, rows, stride;
-  uint64_t tokens;  // of the pass
-  __device__ void enter(const MoeList& l) {  // item, r0
-    count = 0;
-    b0 = 0;
-    if (item >= items) return;
+  int table;  // the entry's tokens
+  __device__ void enter(const MoeList& l) {  // the entry of `item`
     u = item / slices;
     slice = item - u * slices;
     expert = __builtin_amdgcn_readfirstlane(l.expert[u]);
     first_row = __builtin_amdgcn_readfirstlane(l.row[u]);
-    const uint64_t named = l.tokens[u];
-    tokens = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)named) |
-             (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(named >> 32)) << 32;
+    const uint64_t tokens = uniform(l.tokens[u]);
+    table = token_table(tokens);
     all = __popcll(tokens);
-    for (int r = 0; r < r0; ++r) tokens &= tokens - 1;
-    rows = all - r0 < kGateRows ? all - r0 : kGateRows;
-    stride = rows <= 1 ? 1 : 1 << (32 - __builtin_clz(rows - 1));
+    r0 = b0 = 0;
     size();
   }
   __device__ void size() {
+    rows = all - r0 < kGateRows ? all - r0 : kGateRows;
+    stride = power_of_two_from(rows);
     const int most = kGatePairs / stride;  // whole eights: every wave's share
     count = blocks - b0 < most ? blocks - b0 : most;
   }
@@ -171,12 +180,20 @@ struct GateWalk {
       size();
       return;
     }
+    b0 = 0;
     r0 += kGateRows;
     if (r0 >= all) {
       r0 = 0;
-      item += step;
+      if (++item >= last) {
+        count = 0;
+        return;
+      }
+      if (++slice == slices) {
+        enter(l);
+        return;
+      }
     }
-    enter(l);
+    size();
   }
 };
 
@@ -185,6 +202,7 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   __shared__ MoeList list;
   __shared__ alignas(1024) uint8_t stage[2][kGatePairs * kGatePairBytes];
   __shared__ alignas(1024) uint8_t rings[kMoeWaves][kGateAhead * 2048];
+  __shared__ float scales[2][kMoeWaves][kWave];  // of a chunk: a wave's blocks of gate rows, then of up rows
   __shared__ int32_t ids[kMoePairs];
   __shared__ float weights[kMoePairs];
   const int pairs = a.tokens * a.topk;
@@ -202,12 +220,11 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   GateWalk walk;
   walk.slices = a.inner / 16;
   walk.blocks = blocks;
-  walk.item = blockIdx.x;
-  walk.step = gridDim.x;
-  walk.items = __builtin_amdgcn_readfirstlane(list.count) * walk.slices;
-  walk.r0 = 0;
+  const int64_t items = (int64_t)__builtin_amdgcn_readfirstlane(list.count) * walk.slices;
+  walk.item = (int)(items * blockIdx.x / gridDim.x);
+  walk.last = (int)(items * (blockIdx.x + 1) / gridDim.x);
+  if (walk.item == walk.last) return;
   walk.enter(list);
-  if (walk.count == 0) return;
 
   // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes. A wave's
   // blocks of a chunk are its number and every eighth from there; past the last the same loads are
@@ -243,46 +260,48 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int pair = 16 * wave + 4 * i + lane / 16, row = pair & (w.stride - 1), block = pair >> shift;
-      const int64_t t = nth_bit(w.tokens, row < w.rows ? row : 0);
+      const int64_t t = token_of(w.table, w.r0 + (row < w.rows ? row : 0));
       const int k = w.b0 + (block < w.count ? block : 0);
       load_to_lds(reinterpret_cast<const uint8_t*>(a.x + t * a.ldx + (int64_t)k * kMoeBlock) + 16 * ((lane % 16) ^ (pair & 15)),
                   lds_address(stage[buffer] + (16 * wave + 4 * i) * kGatePairBytes));
     }
+    // The block scales come with them: read where they are used, they cost a trip to memory an item.
+    const int block = wave + kMoeWaves * (lane % 16);
+    word_to_lds(a.gate_up_scale + ((int64_t)(2 * w.expert + (lane / 16 & 1)) * block_rows + w.slice / 8) * blocks + w.b0 +
+                    (block < w.count ? block : 0),
+                lds_address(scales[buffer][wave]));
   };
   fetch(walk, 0);
 #pragma unroll
   for (int s = 0; s < kGateAhead; ++s) issue(s, s % 2 == 1);
   wait_loads<2 * kGateAhead>();
   __builtin_amdgcn_s_barrier();
-  int buffer = 0, slot = 0;
+  int buffer = 0, slot = 0, weighed = -1;
+  float weight_table = 0.0f;
   v4f g{0, 0, 0, 0}, w{0, 0, 0, 0};
   while (true) {
     GateWalk following = walk;
     following.next(list);
     fetch(following.count ? following : walk, buffer ^ 1);
-    // (by way of the constant address space: a vector load would not be among the counted ones)
-    const auto gate_scale = (__attribute__((address_space(4))) const float*)a.gate_up_scale +
-                            ((int64_t)walk.expert * 2 * block_rows + walk.slice / 8) * blocks + walk.b0;
-    const auto up_scale = gate_scale + (int64_t)block_rows * blocks;
     int mine = 0;
     for (int c = wave; c < walk.count; c += kMoeWaves, ++mine) {
       const int pair = c * walk.stride + (col & (walk.stride - 1));
       const uint32_t rows = lds_address(stage[buffer]) + pair * kGatePairBytes + 16 * ((2 * quad) ^ (pair & 15));
-      const float sg = gate_scale[c], su = up_scale[c];
       v4u xs[4], raw[2];
+      float scale[2];
       v4f sum{0, 0, 0, 0}, other{0, 0, 0, 0};
       wait_loads<2 * (kGateAhead - 1)>();
-      read_rows_and_half(ring + 2048 * slot + 16 * lane, rows, raw, xs);
+      read_rows_and_half(ring + 2048 * slot + 16 * lane, rows, lds_address(scales[buffer][wave]) + 4 * mine, raw, xs, scale);
       issue(slot, false);
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum = mfma16<DT>(widen8<DT>(raw[i / 2][2 * (i % 2)], raw[i / 2][2 * (i % 2) + 1]), xs[i], sum);
-      g += sum * sg;
+      g += sum * scale[0];
       wait_loads<2 * (kGateAhead - 1)>();
       read_half(ring + 2048 * (slot + 1) + 16 * lane, raw);
       issue(slot + 1, true);
 #pragma unroll
       for (int i = 0; i < 4; ++i) other = mfma16<DT>(widen8<DT>(raw[i / 2][2 * (i % 2)], raw[i / 2][2 * (i % 2) + 1]), xs[i], other);
-      w += other * su;
+      w += other * scale[1];
       slot = (slot + 2) % kGateAhead;
     }
     // The next rows are older than the weights asked for since: those of two blocks have been waited
@@ -300,20 +319,26 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
       g = w = v4f{0, 0, 0, 0};
       lds_barrier();
       const int r = threadIdx.x / 16, n = threadIdx.x % 16;
+      if (walk.u != weighed) {  // the weights of a new entry's rows, row l to lane l
+        weighed = walk.u;
+        weight_table = 0.0f;
+        if (lane < walk.all) {
+          const int p0 = walk.table * a.topk;
+          if (held) {
+            for (int p = p0; p < p0 + a.topk; ++p) weight_table += ids[p] == walk.expert ? weights[p] : 0.0f;
+          } else {
+            for (int p = p0; p < p0 + a.topk; ++p)
+              if (a.ids[p] == walk.expert) weight_table += a.weights[p];
+          }
+        }
+      }
+      const float weight = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(4 * (walk.r0 + r), (int)f2u(weight_table)));
       if (r < walk.rows) {
         float gate_sum = 0.0f, up_sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < kMoeWaves; ++v) {
           gate_sum += part[v][0][r][n];
           up_sum += part[v][1][r][n];
-        }
-        const int t = nth_bit(walk.tokens, r);
-        float weight = 0.0f;
-        if (held) {
-          for (int p = t * a.topk; p < (t + 1) * a.topk; ++p) weight += ids[p] == walk.expert ? weights[p] : 0.0f;
-        } else {
-          for (int p = t * a.topk; p < (t + 1) * a.topk; ++p)
-            if (a.ids[p] == walk.expert) weight += a.weights[p];
         }
         const float y = weight * (gate_sum / (1.0f + expf(-gate_sum)) * up_sum);
         const uint16_t hi = f32_to_bf16_bits(y);
@@ -359,46 +384,64 @@ __device__ inline void read_rows(uint32_t at, DownRows& r) {
       : "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48)
       : "memory");
 }
-__device__ inline void read_block(uint32_t weights, uint32_t at, v4u (&w)[2], DownRows& r) {
+__device__ inline void read_block(uint32_t weights, uint32_t at, uint32_t scales, v4u (&w)[2], DownRows& r, float& scale) {
   asm volatile(
-      "ds_read_b128 %8, %10\n\tds_read_b128 %9, %10 offset:1024\n\t"
-      "ds_read_b128 %0, %11\n\tds_read_b128 %1, %12\n\tds_read_b128 %2, %13\n\tds_read_b128 %3, %14\n\t"
-      "ds_read_b128 %4, %11 offset:256\n\tds_read_b128 %5, %12 offset:256\n\tds_read_b128 %6, %13 offset:256\n\t"
-      "ds_read_b128 %7, %14 offset:256\n\ts_waitcnt lgkmcnt(0)"
+      "ds_read_b128 %8, %11\n\tds_read_b128 %9, %11 offset:1024\n\t"
+      "ds_read_b128 %0, %12\n\tds_read_b128 %1, %13\n\tds_read_b128 %2, %14\n\tds_read_b128 %3, %15\n\t"
+      "ds_read_b128 %4, %12 offset:256\n\tds_read_b128 %5, %13 offset:256\n\tds_read_b128 %6, %14 offset:256\n\t"
+      "ds_read_b128 %7, %15 offset:256\n\tds_read_b32 %10, %16\n\ts_waitcnt lgkmcnt(0)"
       : "=&v"(r.part[0]), "=&v"(r.part[1]), "=&v"(r.part[2]), "=&v"(r.part[3]), "=&v"(r.part[4]), "=&v"(r.part[5]),
-        "=&v"(r.part[6]), "=&v"(r.part[7]), "=&v"(w[0]), "=&v"(w[1])
-      : "v"(weights), "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48)
+        "=&v"(r.part[6]), "=&v"(r.part[7]), "=&v"(w[0]), "=&v"(w[1]), "=&v"(scale)
+      : "v"(weights), "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48), "v"(scales)
       : "memory");
 }
 
-// A walk over the chunks of a workgroup's run, [unit, last) in the list of (expert, block). Every
-// member is the same in all lanes.
+// A walk over the chunks of a workgroup's run, [unit, last) in the list of (expert, block). All but
+// `table` is the same in all lanes. An entry of more than kDownRows rows takes a chunk's blocks in
+// passes, one after the other.
+constexpr int kDownRows = 32;
 struct DownWalk {
-  int unit, last, blocks;  // the chunk's first unit; the run's end; blocks of an expert
-  int u, b, r0, count;     // entry of the list, first block, first row, blocks of the chunk (0: the run is over)
+  int unit, last, blocks;      // the chunk's first unit; the run's end; blocks of an expert
+  int u, b, r0, count;         // entry of the list, first block, first row, blocks of the chunk (0: the run is over)
   int expert, first_row, all;  // of the entry: expert, first row of h, rows
-  int rows, stride;        // rows of the chunk, and rounded up to a power of two
-  __device__ void set(const MoeList& l) {
-    count = 0;
-    if (unit >= last) return;
+  int rows, stride;            // rows of the pass, and rounded up to a power of two
+  int table;                   // the entry's tokens
+  __device__ void enter(const MoeList& l) {  // the entry of `unit`
     u = unit / blocks;
     b = unit - u * blocks;
     expert = __builtin_amdgcn_readfirstlane(l.expert[u]);
     first_row = __builtin_amdgcn_readfirstlane(l.row[u]);
-    all = __builtin_amdgcn_readfirstlane(__popcll(l.tokens[u]));
-    rows = all - r0 < 32 ? all - r0 : 32;
-    stride = rows <= 1 ? 1 : 1 << (32 - __builtin_clz(rows - 1));
+    const uint64_t tokens = uniform(l.tokens[u]);
+    table = token_table(tokens);
+    all = __popcll(tokens);
+    pass(0);
+    size();
+  }
+  __device__ void pass(int first) {
+    r0 = first;
+    rows = all - r0 < kDownRows ? all - r0 : kDownRows;
+    stride = power_of_two_from(rows);
+  }
+  __device__ void size() {  // by the first pass, which has most rows
     const int most = kDownPairs / stride;
     count = blocks - b < last - unit ? blocks - b : last - unit;
     if (count > most) count = most;
   }
   __device__ void next(const MoeList& l) {
-    r0 += 32;
-    if (r0 >= all) {
-      r0 = 0;
-      unit += count;
+    if (r0 + kDownRows < all) {
+      pass(r0 + kDownRows);
+      return;
     }
-    set(l);
+    unit += count;
+    b += count;
+    if (unit >= last) {
+      count = 0;
+    } else if (b == blocks) {
+      enter(l);
+    } else {
+      if (r0) pass(0);
+      size();
+    }
   }
 };
 
@@ -407,7 +450,8 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   __shared__ MoeList list;
   __shared__ alignas(1024) uint8_t stage[2][kDownPairs * kPairBytes];
   __shared__ alignas(1024) uint8_t rings[kMoeWaves][kRingBytes];
-  extern __shared__ float sums[];  // [tokens][kTokenFloats]
+  __shared__ float scales[2][kMoeWaves][kWave];  // of a chunk's blocks
+  extern __shared__ float sums[];                // [tokens][kTokenFloats]
   list_experts(a, list, reinterpret_cast<uint64_t*>(stage));
   for (int i = threadIdx.x; i < a.tokens * kTokenFloats; i += kMoeThreads) sums[i] = 0.0f;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quad = lane / 16;
@@ -417,9 +461,8 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   walk.blocks = blocks;
   walk.unit = (int)(units * blockIdx.y / gridDim.y);
   walk.last = (int)(units * (blockIdx.y + 1) / gridDim.y);
-  walk.r0 = 0;
-  walk.set(list);
-  if (walk.count) {
+  if (walk.unit < walk.last) {
+    walk.enter(list);
     // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes.
     const uint8_t* panel = a.down + (int64_t)(n0 + 16 * wave) * a.inner;
     const uint32_t lane_at = (uint32_t)col * a.inner + 16 * quad, ring = lds_address(rings[wave]);
@@ -451,6 +494,8 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
         load_to_lds(reinterpret_cast<const uint8_t*>(a.h) + (r * a.inner + k * kMoeBlock) * 4 + 16 * ((lane % 32) ^ (pair & 15)),
                     lds_address(stage[buffer] + (4 * wave + 2 * i) * kPairBytes));
       }
+      word_to_lds(a.down_scale + ((int64_t)w.expert * panels + blockIdx.x) * blocks + w.b + (lane < w.count ? lane : 0),
+                  lds_address(scales[buffer][wave]));
     };
     fetch(walk, 0);
 #pragma unroll
@@ -458,22 +503,20 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
     wait_loads<2 * kDownAhead>();
     __builtin_amdgcn_s_barrier();
     int buffer = 0;
+    v4f total[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // of the entry's pass
     while (true) {
       DownWalk following = walk;
       following.next(list);
       fetch(following.count ? following : walk, buffer ^ 1);
-      // (by way of the constant address space: a vector load would not be among the counted ones)
-      const auto scale = (__attribute__((address_space(4))) const float*)a.down_scale + ((int64_t)walk.expert * panels + blockIdx.x) * blocks + walk.b;
       const bool two = walk.rows > 16;
-      v4f total[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
       for (int c = 0; c < walk.count; ++c) {
         const int pair = c * walk.stride + (col & (walk.stride - 1));
         const uint32_t rows = lds_address(stage[buffer]) + pair * kPairBytes + 16 * ((4 * quad) ^ (pair & 15));
-        const float sc = scale[c];
+        float scale;
         v4u w[2], f[4];
         DownRows r;
         wait_loads<2 * (kDownAhead - 1)>();
-        read_block(ring + 2048 * slot + 16 * lane, rows, w, r);
+        read_block(ring + 2048 * slot + 16 * lane, rows, lds_address(scales[buffer][wave]) + 4 * c, w, r, scale);
         issue(slot);
         slot = (slot + 1) % kDownAhead;
         v4f sum[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -483,7 +526,7 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
           sum[0] = mfma16<AYK_BF16>(f[s], r.part[2 * s], sum[0]);
           sum[1] = mfma16<AYK_BF16>(f[s], r.part[2 * s + 1], sum[1]);
         }
-        total[0] += (sum[0] + sum[1]) * sc;
+        total[0] += (sum[0] + sum[1]) * scale;
         if (two) {
           read_rows(rows + 16 * kPairBytes, r);
           sum[0] = sum[1] = v4f{0, 0, 0, 0};
@@ -492,14 +535,15 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
             sum[0] = mfma16<AYK_BF16>(f[s], r.part[2 * s], sum[0]);
             sum[1] = mfma16<AYK_BF16>(f[s], r.part[2 * s + 1], sum[1]);
           }
-          total[1] += (sum[0] + sum[1]) * sc;
+          total[1] += (sum[0] + sum[1]) * scale;
         }
       }
+      if (following.count == 0 || following.u != walk.u || following.r0 != walk.r0) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if (16 * r + col < walk.rows) {
-          float* to = sums + nth_bit(list.tokens[walk.u], walk.r0 + 16 * r + col) * kTokenFloats + 16 * wave + 4 * quad;
-          *reinterpret_cast<v4f*>(to) += total[r];
+        for (int r = 0; r < 2; ++r) {
+          const int t = token_of(walk.table, walk.r0 + 16 * r + col);
+          if (16 * r + col < walk.rows) *reinterpret_cast<v4f*>(sums + t * kTokenFloats + 16 * wave + 4 * quad) += total[r];
+          total[r] = v4f{0, 0, 0, 0};
         }
       }
       if (following.count == 0) break;
@@ -552,6 +596,10 @@ int down_runs(int64_t tokens, int64_t topk, int64_t experts, int64_t hidden, int
   const int64_t runs = want < most ? want : most;
   return (int)(runs < 1 ? 1 : runs);
 }
+
+// LDS of the second launch: what its declarations take, and the tokens' sums.
+constexpr size_t kDownLds = sizeof(MoeList) + 2 * kDownPairs * kPairBytes + kMoeWaves * (kRingBytes + 2 * 4 * kWave) + 64;
+static_assert(kDownLds + kMoeTokens * kTokenFloats * sizeof(float) <= 160 * 1024, "LDS of a CU");
 
 template <int DT>
 int launch_moe(const MoeArgs& a, hipStream_t st) {

@@ -64,6 +64,17 @@ def test_all_tokens_name_one_expert(gpu):
     check(c, gpu, "one expert")
 
 
+@pytest.mark.parametrize("tokens", [17, 31, 33, 40, 64])
+@pytest.mark.parametrize("inner", [128, 640, 1152])
+def test_many_rows_of_few_experts(gpu, tokens, inner):
+    """Entries of more rows than a pass holds, beside entries of one row, over several blocks."""
+    c = moe_case(tokens, 6, 2, 640, inner, seed=tokens)
+    c["topk_ids"][:, 0] = 2
+    c["topk_ids"][:, 1] = torch.where(torch.arange(tokens) < tokens - 3, 4, -1)
+    c["topk_ids"][-1, 1] = 5
+    check(c, gpu, f"{tokens} rows, inner={inner}")
+
+
 def test_weights_of_any_sign_and_size(gpu):
     c = moe_case(6, 4, 2, 256, 128, seed=4)
     c["topk_weights"] = torch.tensor([[0.0, 1.0], [-1.0, 2.0], [1e-30, 1.0], [300.0, -5.0], [0.0, 0.0], [1.0, 1.0]])
