@@ -50,9 +50,41 @@ struct MoeList {
 };
 // masks: room for kMoeExperts in LDS while the list is made.
 __device__ inline void list_experts(const MoeArgs& a, MoeList& l, uint64_t* masks) {
+  const int pairs = a.tokens * a.topk;
+  if (pairs <= kWave) {  // a pair a lane of the first wave: every lane compares its expert with all
+    if (threadIdx.x < kWave) {
+      const int lane = threadIdx.x;
+      const int mine = lane < pairs ? a.ids[lane] : -1;
+      const bool named = (uint32_t)mine < (uint32_t)a.experts;
+      uint64_t mask = 0;
+      bool first = named;
+      for (int q = 0; q < pairs; ++q) {
+        const bool same = named && __builtin_amdgcn_readlane(mine, q) == mine;
+        if (same) mask |= 1ull << (q / a.topk);
+        first &= !(same && q < lane);
+      }
+      const uint64_t leaders = __ballot(first);
+      const int count = __popcll(mask);
+      int at = 0, rows = 0;  // entries before this lane's, and their rows
+      for (uint64_t rest = leaders; rest; rest &= rest - 1) {
+        const int q = __builtin_ctzll(rest);
+        const bool before = __builtin_amdgcn_readlane(mine, q) < mine;
+        at += before ? 1 : 0;
+        rows += before ? __builtin_amdgcn_readlane(count, q) : 0;
+      }
+      if (first) {
+        l.expert[at] = (uint16_t)mine;
+        l.tokens[at] = mask;
+        l.row[at] = (uint16_t)rows;
+      }
+      if (lane == 0) l.count = __popcll(leaders);
+    }
+    __syncthreads();
+    return;
+  }
   for (int e = threadIdx.x; e < a.experts; e += kMoeThreads) masks[e] = 0;
   __syncthreads();
-  for (int p = threadIdx.x; p < a.tokens * a.topk; p += kMoeThreads) {
+  for (int p = threadIdx.x; p < pairs; p += kMoeThreads) {
     const int e = a.ids[p];
     if ((uint32_t)e < (uint32_t)a.experts) atomicOr((unsigned long long*)&masks[e], 1ull << (p / a.topk));
   }
@@ -451,7 +483,7 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   __shared__ alignas(1024) uint8_t stage[2][kDownPairs * kPairBytes];
   __shared__ alignas(1024) uint8_t rings[kMoeWaves][kRingBytes];
   __shared__ float scales[2][kMoeWaves][kWave];  // of a chunk's blocks
-  extern __shared__ float sums[];                // [tokens][kTokenFloats]
+  extern __shared__ float sums[];                // [tokens][kTokenFloats], room for kMoeThreads at least
   list_experts(a, list, reinterpret_cast<uint64_t*>(stage));
   for (int i = threadIdx.x; i < a.tokens * kTokenFloats; i += kMoeThreads) sums[i] = 0.0f;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quad = lane / 16;
@@ -580,10 +612,30 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(a.arrived + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (arrived != (int)gridDim.y - 1) return;
-  for (int i = threadIdx.x; i < tokens * kMoeBlock; i += kMoeThreads) {
-    const float* p = a.partial + (int64_t)(i / kMoeBlock) * a.hidden + n0 + i % kMoeBlock;
+  // A few threads a cell where the cells are few; eight loads at a time, as each goes to memory.
+  const int cells = tokens * kMoeBlock, runs = gridDim.y, share = cells < kMoeThreads ? kMoeThreads / cells : 1;
+  for (int i = threadIdx.x; i < cells * share; i += kMoeThreads) {
+    const int cell = i % cells, first = i / cells;
+    const float* p = a.partial + (int64_t)(cell / kMoeBlock) * a.hidden + n0 + cell % kMoeBlock;
     float sum = 0.0f;
-    for (int r = 0; r < (int)gridDim.y; ++r) sum += __hip_atomic_load(p + r * plane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int r0 = first; r0 < runs; r0 += 8 * share) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = r0 + k * share;
+        v[k] = r < runs ? __hip_atomic_load(p + r * plane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += v[k];
+    }
+    if (share == 1) store_f32(a.out, DT, cell / kMoeBlock * a.ldo + n0 + cell % kMoeBlock, sum);
+    else sums[i] = sum;
+  }
+  if (share == 1) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < cells; i += kMoeThreads) {
+    float sum = 0.0f;
+    for (int k = 0; k < share; ++k) sum += sums[k * cells + i];
     store_f32(a.out, DT, i / kMoeBlock * a.ldo + n0 + i % kMoeBlock, sum);
   }
 }
@@ -607,7 +659,7 @@ int launch_moe(const MoeArgs& a, hipStream_t st) {
   const int64_t items = used * (a.inner / 16);
   hipLaunchKernelGGL((moe_gate_up_kernel<DT>), dim3((unsigned)(items < 256 ? items : 256)), dim3(kMoeThreads), 0, st, a);
   const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner));
-  hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), a.tokens * kTokenFloats * sizeof(float), st, a);
+  hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), (a.tokens < 4 ? 4 : a.tokens) * kTokenFloats * sizeof(float), st, a);
   return check_launch("fp8_block_moe_small");
 }
 
