@@ -43,14 +43,9 @@ __device__ inline int mx_k_dim(int s, int quad) {
 }
 
 template <bool ONCE, typename T>
-__device__ inline T mx_load(const uint8_t* p, bool on) {
-  T v{};
-  if constexpr (ONCE && sizeof(T) >= 4) {
-    if (on) v = __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
-  } else {
-    if (on) v = *reinterpret_cast<const T*>(p);
-  }
-  return v;
+__device__ inline T mx_load(const uint8_t* p) {
+  if constexpr (ONCE && sizeof(T) >= 4) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else return *reinterpret_cast<const T*>(p);
 }
 
 template <int QT, int D, bool EXACT, int WAVES, bool ONCE>
@@ -107,19 +102,19 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
   const uint8_t* vs = a.vs + (uint64_t)g * page_size * groups;
   auto page_index = [&](uint32_t j) { return a.page_shift >= 0 ? j >> a.page_shift : j / page_size; };
   // Lane l looks after position l % 32 of a block, and reads the page of its eight positions (a page
-  // holds eights whole) a block ahead of the rows.
+  // holds eights whole) a block ahead of the rows. Every load of the loop is issued in every round, past
+  // the last block for that again, with dims past the head's at its first: the compiler then
+  // counts the loads that are younger than the one it waits for (behind a branch it waits for all).
   auto position = [&](int blk) { return kBlock * (blk < bl.first_blocks ? blk : blk + bl.jump) + lane % kBlock; };
-  auto page_of = [&](int blk) {
-    const int first = position(blk) & ~7;
-    return first < bl.end ? table[page_index(first)] : -1;
-  };
+  auto eight_of = [&](int blk) { return min(position(blk), bl.end - 1) & ~7; };
+  auto page_of = [&](int blk) { return table[page_index(eight_of(blk))]; };
   auto known = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
   auto seen_of = [&](int blk, int page) {
     const int j = position(blk);
     return (uint32_t)__ballot(known(page) && j < bl.end && (j >= bl.first || j < bl.kept));
   };
   auto row_of = [&](int blk, int page) {  // of the eight's first position (page unknown: any row)
-    const uint32_t first = position(blk) & ~7;
+    const uint32_t first = eight_of(blk);
     return known(page) ? (uint32_t)page * a.page_rows + (first - page_index(first) * page_size) : 0u;
   };
   // Row 4 (l / 16) + i of score tile t is position 8 (l / 16) + 4 t + i: the lane's weights are then
@@ -132,35 +127,32 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
       const uint64_t at = eight + 4 * t + col % 4;
 #pragma unroll
       for (int h = 0; h < S::kParts; ++h) {
-        const bool on = EXACT || mx_k_dim<D>(4 * h, quad) < a.dim;
-        if constexpr (D == 64) {
-          *reinterpret_cast<v2u*>(kw[t]) = mx_load<ONCE, v2u>(kc + at * row_bytes + 8 * quad, on);
-          kse[t][0] = mx_load<false, uint8_t>(ks + at * groups + quad / 2, on);
-        } else {
-          *reinterpret_cast<v4u*>(kw[t] + 4 * h) = mx_load<ONCE, v4u>(kc + at * row_bytes + 64 * h + 16 * quad, on);
-          kse[t][h] = mx_load<false, uint8_t>(ks + at * groups + 4 * h + quad, on);
-        }
+        const int dim = mx_k_dim<D>(4 * h, quad), there = EXACT || dim < a.dim ? dim : 0;
+        const uint8_t* p = kc + at * row_bytes + there / 2;
+        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = mx_load<ONCE, v2u>(p);
+        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = mx_load<ONCE, v4u>(p);
+        kse[t][h] = mx_load<false, uint8_t>(ks + at * groups + there / kMxGroup);
       }
     }
   };
+  // (K's dims past the head's meet zeros of Q: what counts is that they are numbers)
+  auto k_scale = [&](int t, int h) {
+    return u2f(EXACT || mx_k_dim<D>(4 * h, quad) < a.dim ? kse[t][h] << 23 : 0u);
+  };
   constexpr bool kVector = EXACT && D != 256;  // the scales of eight rows as one or two 16-byte loads
-  const bool v_on = EXACT || col * S::kCols < a.dim;
-  const int v_group = col * S::kCols / kMxGroup;
+  const int v_dim = EXACT || col * S::kCols < a.dim ? col * S::kCols : 0, v_group = v_dim / kMxGroup;
   auto issue_v = [&](uint32_t row) {
     const uint64_t eight = (uint32_t)__builtin_amdgcn_ds_bpermute(32 * quad, (int)row);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint8_t* p = vc + (eight + j) * row_bytes + col * S::kCols / 2;
-      if constexpr (D == 64) vw[j][0] = mx_load<ONCE, uint16_t>(p, v_on);
-      else if constexpr (D == 128) vw[j][0] = mx_load<ONCE, uint32_t>(p, v_on);
-      else *reinterpret_cast<v2u*>(vw[j]) = mx_load<ONCE, v2u>(p, v_on);
+      const uint8_t* p = vc + (eight + j) * row_bytes + v_dim / 2;
+      if constexpr (D == 64) vw[j][0] = mx_load<ONCE, uint16_t>(p);
+      else if constexpr (D == 128) vw[j][0] = mx_load<ONCE, uint32_t>(p);
+      else *reinterpret_cast<v2u*>(vw[j]) = mx_load<ONCE, v2u>(p);
       if constexpr (!kVector) {
-        if constexpr (D == 64) {
-          if (j % 2 == 0) vse[j / 2] = 0;
-          vse[j / 2] |= (uint32_t)mx_load<false, uint8_t>(vs + (eight + j) * groups + v_group, v_on) << (16 * (j % 2) + 8 * v_group);
-        } else {
-          vse[j] = mx_load<false, uint8_t>(vs + (eight + j) * groups + v_group, v_on);
-        }
+        const uint32_t code = mx_load<false, uint8_t>(vs + (eight + j) * groups + v_group);
+        if constexpr (D == 64) vse[j / 2] = (j % 2 ? vse[j / 2] : 0) | code << (16 * (j % 2) + 8 * v_group);
+        else vse[j] = code;
       }
     }
     if constexpr (kVector) {
@@ -172,11 +164,12 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
 
   int page = page_of(i);
   uint32_t seen = seen_of(i, page), row = row_of(i, page);
-  page = i + WAVES < most ? page_of(i + WAVES) : -1;
+  auto following = [&](int blk) { return blk + WAVES < most ? blk + WAVES : blk; };
+  page = page_of(following(i));
   issue_k(row);
   issue_v(row);
   while (true) {
-    const bool more = i + WAVES < most;
+    const int next = following(i);
     const uint32_t now = seen;
     v4f s[2];
 #pragma unroll
@@ -185,19 +178,17 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
 #pragma unroll
       for (int d = 0; d < S::kSteps; ++d) {
         const uint32_t w = kw[t][d];
-        const float sc = u2f(kse[t][S::kParts == 2 ? d / 4 : 0] << 23);
+        const float sc = k_scale(t, S::kParts == 2 ? d / 4 : 0);
         const v4u f{mx4_widen2<0>(w, sc), mx4_widen2<1>(w, sc), mx4_widen2<2>(w, sc), mx4_widen2<3>(w, sc)};
         s[t] = mfma16<AYK_BF16>(f, qf[d], s[t]);
         if constexpr (kSplitQ) s[t] = mfma16<AYK_BF16>(f, ql[d], s[t]);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (more) {
-      seen = seen_of(i + WAVES, page);
-      row = row_of(i + WAVES, page);
-      if (i + 2 * WAVES < most) page = page_of(i + 2 * WAVES);
-      issue_k(row);
-    }
+    seen = seen_of(next, page);
+    row = row_of(next, page);
+    page = page_of(following(next));
+    issue_k(row);
     float x[8], vsc[8], top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -266,9 +257,9 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
       product(std::integral_constant<int, 7>{});
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (!more) break;
     issue_v(row);
-    i += WAVES;
+    if (next == i) break;
+    i = next;
   }
 }
 
