@@ -178,7 +178,7 @@ _here = contextlib.nullcontext()
 
 def on_device(t: torch.Tensor) -> Any:
     """Context in which ``t``'s device is the current one (kernels are launched on that)."""
-    index = t.device.index
+    index = t.get_device()
     return _here if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 

@@ -18,6 +18,7 @@ from ayaka.kernel.hip.attention._checks import (
     check_scale,
     check_window,
     new_output,
+    on_device_of,
     rows_of_heads,
 )
 from ayaka.kernel.hip.cache.mxfp4_cache import check_planes
@@ -66,8 +67,9 @@ def paged_decode_attention_mxfp4(
     Lengths and tables are read on the device only: the operator can be captured in a graph
     and replayed with new contents.
     """
-    check_devices(query, "query", key_codes=key_codes, key_scales=key_scales, value_codes=value_codes, value_scales=value_scales,
-                  block_tables=block_tables, seq_lens=seq_lens)
+    if not on_device_of(query, key_codes, key_scales, value_codes, value_scales, block_tables, seq_lens):
+        check_devices(query, "query", key_codes=key_codes, key_scales=key_scales, value_codes=value_codes,
+                      value_scales=value_scales, block_tables=block_tables, seq_lens=seq_lens)
     if query.dtype not in ATTENTION_DTYPES:
         require_dtype(query, "query", ATTENTION_DTYPES)
     if query.ndim != 3:

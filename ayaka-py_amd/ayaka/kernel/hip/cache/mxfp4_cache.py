@@ -18,13 +18,13 @@ import torch
 
 from ayaka.kernel.hip import _lib
 from ayaka.kernel.hip._host import require_dtype
-from ayaka.kernel.hip.attention._checks import MAX_HEAD_DIM, rows_of_heads
+from ayaka.kernel.hip.attention._checks import MAX_HEAD_DIM, on_device_of
 from ayaka.kernel.hip.cache.rope_cache import (
     check_devices,
     check_payload,
     check_result,
     check_rotation,
-    rows_and_strides,
+    packed_rows,
 )
 from ayaka.kernel.ops import custom_op
 
@@ -39,46 +39,56 @@ def check_plane(codes: torch.Tensor, scales: torch.Tensor, name: str) -> tuple[i
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         require_dtype(codes, f"{name}_codes", (torch.uint8,))
         require_dtype(scales, f"{name}_scales", (torch.uint8,))
-    if codes.ndim != 4 or scales.ndim != 4 or codes.shape[:3] != scales.shape[:3]:
+    shape, groups = codes.shape, scales.shape
+    if len(shape) != 4 or len(groups) != 4 or shape[:3] != groups[:3]:
         raise ValueError(f"{name}_codes and {name}_scales must be [pages, kv_heads, page_size, head_dim / 2] and [..., head_dim / 32]")
-    pages, kv_heads, page_size, half = codes.shape
+    pages, kv_heads, page_size, half = shape
     dim = 2 * half
-    if dim % GROUP or not GROUP <= dim <= MAX_HEAD_DIM or scales.shape[3] * GROUP != dim:
+    if dim % GROUP or not GROUP <= dim <= MAX_HEAD_DIM or groups[3] * GROUP != dim:
         raise ValueError(f"the head_dim of a 4-bit cache must be a multiple of {GROUP} up to {MAX_HEAD_DIM}, with a scale for every "
-                         f"{GROUP} dims; got {dim} dims and {scales.shape[3]} scales")
+                         f"{GROUP} dims; got {dim} dims and {groups[3]} scales")
     if kv_heads < 1 or page_size < 8 or page_size % 8:
         raise ValueError(f"a 4-bit cache needs kv_heads and a page_size that is a multiple of 8, got {kv_heads} and {page_size}")
-    if not codes.is_contiguous() or not scales.is_contiguous():
-        raise ValueError("KV cache pages must be contiguous")
-    if codes.data_ptr() % 16 or scales.data_ptr() % 16:
-        raise ValueError(f"{name}_codes and {name}_scales must be 16-byte aligned")
+    _check_memory(codes, scales, name)
     return pages, kv_heads, page_size, dim
 
 
+def _check_memory(codes, scales, name) -> None:
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError("KV cache pages must be contiguous")
+    if (codes.data_ptr() | scales.data_ptr()) & 15:
+        raise ValueError(f"{name}_codes and {name}_scales must be 16-byte aligned")
+
+
 def check_planes(key_codes, key_scales, value_codes, value_scales) -> tuple[int, int, int, int]:
+    """Those of K and V; V's geometry needs no look of its own where it is K's."""
     geometry = check_plane(key_codes, key_scales, "key")
-    if check_plane(value_codes, value_scales, "value") != geometry:
+    same = value_codes.shape == key_codes.shape and value_scales.shape == key_scales.shape
+    if same and value_codes.dtype == value_scales.dtype == torch.uint8:
+        _check_memory(value_codes, value_scales, "value")
+    elif check_plane(value_codes, value_scales, "value") != geometry:
         raise ValueError("KV cache planes must share geometry")
     return geometry
 
 
-def _write(query, key, value, positions, cos_sin, planes, slots, query_out, key_out, interleaved) -> None:
+def _write(query, heads, key, value, rows, positions, cos_sin, planes, slots, query_out, key_out, interleaved) -> None:
     pages, kv_heads, page_size, dim = check_planes(*planes)
-    if key.shape[1:] != (kv_heads, dim):
-        raise ValueError(f"key and value rows {tuple(key.shape[1:])} do not match a cache of {kv_heads} heads of {dim}")
-    tokens = key.shape[0]
+    if rows[1] != kv_heads or rows[2] != dim:
+        raise ValueError(f"key and value rows {tuple(rows[1:])} do not match a cache of {kv_heads} heads of {dim}")
+    tokens = rows[0]
     if tokens == 0:
         return
-    heads = 0 if query is None else query.shape[1]
-    query = None if query is None else rows_of_heads(query)
-    key, value, slots = rows_of_heads(key), rows_of_heads(value), slots.contiguous()
+    # (the tensors stay referenced: a copy's memory must not be handed out before the launch)
+    query, *q = packed_rows(query)
+    key, *k = packed_rows(key)
+    value, *v = packed_rows(value)
+    slots = slots.contiguous()
     positions = None if positions is None else positions.contiguous()
-    table_rows, rotary = (0, 0) if cos_sin is None else cos_sin.shape
     with _lib.on_device(key):
-        _lib.call("ayk_rope_kv_write_mxfp4", *rows_and_strides(query), *rows_and_strides(key), *rows_and_strides(value),
-                  _lib.dtype_code(key.dtype), tokens, heads, kv_heads, dim, _lib.ptr(positions), _lib.ptr(cos_sin), table_rows,
-                  rotary, int(interleaved), *rows_and_strides(query_out), *rows_and_strides(key_out),
-                  *(p.data_ptr() for p in planes), pages, page_size, slots.data_ptr(), _lib.stream_of(key))
+        _lib.call("ayk_rope_kv_write_mxfp4", *q, *k, *v, _lib.dtype_code(key.dtype), tokens, heads, kv_heads, dim,
+                  _lib.ptr(positions), _lib.ptr(cos_sin), *((0, 0) if cos_sin is None else cos_sin.shape), int(interleaved),
+                  *packed_rows(query_out)[1:], *packed_rows(key_out)[1:], *[p.data_ptr() for p in planes], pages, page_size,
+                  slots.data_ptr(), _lib.stream_of(key))
 
 
 def _rope_write_kv_mxfp4_fake(query, key, value, positions, cos_sin, key_codes, key_scales, value_codes, value_scales, slots,
@@ -106,19 +116,18 @@ def rope_write_kv_mxfp4(
     """``rope_write_kv`` into a 4-bit cache: the arguments, and what becomes of padding tokens,
     are that operator's, but for the planes (see the module) and the static scales, which a
     4-bit cache does not have."""
-    others = {"key": key, "value": value, "positions": positions, "cos_sin": cos_sin, "key_codes": key_codes,
-              "key_scales": key_scales, "value_codes": value_codes, "value_scales": value_scales, "slots": slots,
-              "query_out": query_out}
+    if not on_device_of(query, key, value, positions, cos_sin, key_codes, key_scales, value_codes, value_scales, slots,
+                        query_out, query if key_out is None else key_out):
+        check_devices(query, "query", key=key, value=value, positions=positions, cos_sin=cos_sin, key_codes=key_codes,
+                      key_scales=key_scales, value_codes=value_codes, value_scales=value_scales, slots=slots,
+                      query_out=query_out, key_out=query if key_out is None else key_out)
+    rows = check_payload(key, value, slots)
+    shape = check_rotation(query, key, rows, positions, cos_sin)
+    check_result(query_out, "query_out", query, shape)
     if key_out is not None:
-        others["key_out"] = key_out
-    check_devices(query, "query", **others)
-    check_payload(key, value, slots)
-    check_rotation(query, key, positions, cos_sin)
-    check_result(query_out, "query_out", query, "query")
-    if key_out is not None:
-        check_result(key_out, "key_out", key, "key")
-    _write(query, key, value, positions, cos_sin, (key_codes, key_scales, value_codes, value_scales), slots, query_out, key_out,
-           interleaved)
+        check_result(key_out, "key_out", key, rows)
+    _write(query, shape[1], key, value, rows, positions, cos_sin, (key_codes, key_scales, value_codes, value_scales), slots,
+           query_out, key_out, interleaved)
 
 
 def _write_kv_mxfp4_fake(key, value, key_codes, key_scales, value_codes, value_scales, slots) -> None:
@@ -145,8 +154,8 @@ def write_kv_mxfp4(
     """
     check_devices(key, "key", value=value, key_codes=key_codes, key_scales=key_scales, value_codes=value_codes,
                   value_scales=value_scales, slots=slots)
-    check_payload(key, value, slots)
-    _write(None, key, value, None, None, (key_codes, key_scales, value_codes, value_scales), slots, None, None, False)
+    rows = check_payload(key, value, slots)
+    _write(None, 0, key, value, rows, None, None, (key_codes, key_scales, value_codes, value_scales), slots, None, None, False)
 
 
 def _gather_cache_mxfp4_fake(codes, scales, slots, destination) -> None:
@@ -169,13 +178,14 @@ def gather_cache_mxfp4(codes: torch.Tensor, scales: torch.Tensor, slots: torch.T
         raise ValueError("gather slots must be a rank-1 int64 tensor")
     if destination.dtype not in _PAYLOAD_DTYPES:
         require_dtype(destination, "destination", _PAYLOAD_DTYPES)
-    if destination.numel() != slots.numel() * kv_heads * dim:
+    rows = slots.numel()
+    if destination.numel() != rows * kv_heads * dim:
         raise ValueError("gather destination must hold one cache row per slot")
     if not destination.is_contiguous():
         raise ValueError("gather needs a contiguous destination")
-    if slots.numel() == 0:
+    if rows == 0:
         return
     slots = slots.contiguous()
     with _lib.on_device(codes):
         _lib.call("ayk_kv_gather_mxfp4", codes.data_ptr(), scales.data_ptr(), pages, page_size, kv_heads, dim, slots.data_ptr(),
-                  slots.numel(), destination.data_ptr(), _lib.dtype_code(destination.dtype), _lib.stream_of(codes))
+                  rows, destination.data_ptr(), _lib.dtype_code(destination.dtype), _lib.stream_of(codes))

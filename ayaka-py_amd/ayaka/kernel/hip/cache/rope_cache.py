@@ -12,7 +12,7 @@ import torch
 
 from ayaka.kernel.hip import _lib
 from ayaka.kernel.hip._host import require_cuda, require_dtype, require_same_device, require_shape
-from ayaka.kernel.hip.attention._checks import ATTENTION_DTYPES, MAX_HEAD_DIM, check_heads, on_device_of, rows_of_heads
+from ayaka.kernel.hip.attention._checks import ATTENTION_DTYPES, MAX_HEAD_DIM, check_heads, on_device_of
 from ayaka.kernel.hip.cache.cache_ops import _check_scale
 from ayaka.kernel.ops import custom_op
 
@@ -21,16 +21,19 @@ __all__ = ["rope_write_kv"]
 _FP8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 
 
-def check_payload(key, value, slots) -> None:
-    """Keys and values of one step and their slots."""
+def check_payload(key, value, slots) -> torch.Size:
+    """Keys and values of one step and their slots; their shape."""
     if key.dtype not in ATTENTION_DTYPES or value.dtype != key.dtype:
         require_dtype(key, "key", ATTENTION_DTYPES)
         require_dtype(value, "value", (key.dtype,))
-    if key.ndim != 3 or key.shape != value.shape:
+    shape = key.shape
+    if len(shape) != 3 or shape != value.shape:
         raise ValueError("key and value must be [tokens, kv_heads, head_dim] of one shape")
-    if key.shape[1] < 1 or not 1 <= key.shape[2] <= MAX_HEAD_DIM:
+    tokens, kv_heads, dim = shape
+    if kv_heads < 1 or not 1 <= dim <= MAX_HEAD_DIM:
         raise ValueError(f"key and value must have heads, and a head_dim between 1 and {MAX_HEAD_DIM}")
-    check_index(slots, "slots", key.shape[0])
+    check_index(slots, "slots", tokens)
+    return shape
 
 
 def check_index(index, name, tokens) -> None:
@@ -40,33 +43,35 @@ def check_index(index, name, tokens) -> None:
         require_shape(index, name, (tokens,))
 
 
-def check_rotation(query, key, positions, cos_sin) -> None:
-    """Queries beside their keys, and the table that rotates both."""
+def check_rotation(query, key, shape, positions, cos_sin) -> torch.Size:
+    """Queries beside their keys (of that shape), and the table that rotates both; the queries' shape."""
     if query.dtype != key.dtype:
         require_dtype(query, "query", (key.dtype,))
-    if query.ndim != 3 or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
+    queries, (tokens, kv_heads, dim) = query.shape, shape
+    if len(queries) != 3 or queries[0] != tokens or queries[2] != dim:
         raise ValueError("query must be [tokens, heads, head_dim] with the key's tokens and head_dim")
-    check_heads(query.shape[1], key.shape[1], key.shape[2])
-    check_index(positions, "positions", key.shape[0])
+    check_heads(queries[1], kv_heads, dim)
+    check_index(positions, "positions", tokens)
     if cos_sin.dtype != torch.float32:
         require_dtype(cos_sin, "cos_sin", (torch.float32,))
     if cos_sin.ndim != 2 or cos_sin.shape[0] < 1 or not cos_sin.is_contiguous():
         raise ValueError("cos_sin must be a contiguous [positions, rotary_dim] table")
     rotary = cos_sin.shape[1]
-    if rotary < 2 or rotary % 2 or rotary > key.shape[2]:
-        raise ValueError(f"rotary_dim must be even, at least 2 and at most head_dim {key.shape[2]}, got {rotary}")
+    if rotary < 2 or rotary % 2 or rotary > dim:
+        raise ValueError(f"rotary_dim must be even, at least 2 and at most head_dim {dim}, got {rotary}")
+    return queries
 
 
-def check_result(out, name, like, like_name) -> None:
+def check_result(out, name, like, shape) -> None:
     """A caller's buffer for rotated rows: any row and head stride, elements side by side."""
     if out.dtype != like.dtype:
         require_dtype(out, name, (like.dtype,))
-    if out.shape != like.shape:
-        require_shape(out, name, tuple(like.shape))
-    require_same_device(out, name, like, like_name)
-    if out.shape[2] > 1 and out.stride(2) != 1:
+    if out.shape != shape:
+        require_shape(out, name, tuple(shape))
+    row, head, unit = out.stride()
+    if unit != 1 and shape[2] > 1:
         raise ValueError(f"{name} must have stride(2) == 1")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+    if (row == 0 and shape[0] > 1) or (head == 0 and shape[1] > 1):
         raise ValueError(f"{name} must not overlap itself")
 
 
@@ -79,9 +84,16 @@ def check_devices(first, first_name, **others) -> None:
             require_same_device(t, name, first, first_name)
 
 
-def rows_and_strides(t: torch.Tensor | None) -> tuple:
-    """Address and the row and head strides of ``[tokens, heads, dim]`` rows."""
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+def packed_rows(t: torch.Tensor | None) -> tuple:
+    """``[tokens, heads, dim]`` rows with unit stride along ``dim`` (a copy only where it has another): the
+    tensor, its address, its row and head strides."""
+    if t is None:
+        return None, None, 0, 0
+    row, head, unit = t.stride()
+    if unit != 1 and t.shape[2] != 1:
+        t = t.contiguous()
+        row, head, _ = t.stride()
+    return t, t.data_ptr(), row, head
 
 
 def _rope_write_kv_fake(query, key, value, positions, cos_sin, key_cache, value_cache, slots, k_inverse, v_inverse, query_out,
@@ -129,32 +141,34 @@ def rope_write_kv(
 
     A token whose position is outside the table gives zero rows and is not written.
     """
-    others = {"key": key, "value": value, "positions": positions, "cos_sin": cos_sin, "key_cache": key_cache,
-              "value_cache": value_cache, "slots": slots, "query_out": query_out}
-    if key_out is not None:
-        others["key_out"] = key_out
-    check_devices(query, "query", **others)
+    # (a dictionary of names only where an operand is refused)
+    if not on_device_of(query, key, value, positions, cos_sin, key_cache, value_cache, slots, query_out,
+                        query if key_out is None else key_out):
+        check_devices(query, "query", key=key, value=value, positions=positions, cos_sin=cos_sin, key_cache=key_cache,
+                      value_cache=value_cache, slots=slots, query_out=query_out, key_out=query if key_out is None else key_out)
     _check_scale(k_inverse, v_inverse)
-    check_payload(key, value, slots)
-    check_rotation(query, key, positions, cos_sin)
-    tokens, heads, dim = query.shape
-    kv_heads, cache = key.shape[1], key_cache.shape
-    if key_cache.dtype not in _FP8_DTYPES and key_cache.dtype != key.dtype:
+    rows = check_payload(key, value, slots)
+    shape = check_rotation(query, key, rows, positions, cos_sin)
+    tokens, kv_heads, dim = rows
+    cache, kind = key_cache.shape, key_cache.dtype
+    if kind not in _FP8_DTYPES and kind != key.dtype:
         require_dtype(key_cache, "key_cache", (*_FP8_DTYPES, key.dtype))
-    if len(cache) != 4 or cache != value_cache.shape or value_cache.dtype != key_cache.dtype or cache[2:] != key.shape[1:]:
+    if len(cache) != 4 or cache != value_cache.shape or value_cache.dtype != kind or cache[2] != kv_heads or cache[3] != dim:
         raise ValueError("key_cache and value_cache must be [pages, page_size, kv_heads, head_dim] of one dtype, for the key's heads")
     if not key_cache.is_contiguous() or not value_cache.is_contiguous():
         raise ValueError("KV cache pages must be contiguous")
-    check_result(query_out, "query_out", query, "query")
+    check_result(query_out, "query_out", query, shape)
     if key_out is not None:
-        check_result(key_out, "key_out", key, "key")
+        check_result(key_out, "key_out", key, rows)
     if tokens == 0:
         return
-    query, key, value = rows_of_heads(query), rows_of_heads(key), rows_of_heads(value)
+    # (the tensors stay referenced: a copy's memory must not be handed out before the launch)
+    query, *q = packed_rows(query)
+    key, *k = packed_rows(key)
+    value, *v = packed_rows(value)
     positions, slots = positions.contiguous(), slots.contiguous()
     with _lib.on_device(query):
-        _lib.call("ayk_rope_kv_write", *rows_and_strides(query), *rows_and_strides(key), *rows_and_strides(value),
-                  _lib.dtype_code(query.dtype), tokens, heads, kv_heads, dim, positions.data_ptr(), cos_sin.data_ptr(),
-                  cos_sin.shape[0], cos_sin.shape[1], int(interleaved), *rows_and_strides(query_out), *rows_and_strides(key_out),
-                  key_cache.data_ptr(), value_cache.data_ptr(), _lib.dtype_code(key_cache.dtype), cache[0] * cache[1],
-                  slots.data_ptr(), k_inverse, v_inverse, _lib.stream_of(query))
+        _lib.call("ayk_rope_kv_write", *q, *k, *v, _lib.dtype_code(query.dtype), tokens, shape[1], kv_heads, dim,
+                  positions.data_ptr(), cos_sin.data_ptr(), *cos_sin.shape, int(interleaved), *packed_rows(query_out)[1:],
+                  *packed_rows(key_out)[1:], key_cache.data_ptr(), value_cache.data_ptr(), _lib.dtype_code(kind),
+                  cache[0] * cache[1], slots.data_ptr(), k_inverse, v_inverse, _lib.stream_of(query))

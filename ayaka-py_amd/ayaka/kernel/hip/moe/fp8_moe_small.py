@@ -40,11 +40,10 @@ def _check_experts(codes, scale, name, shape) -> None:
 
 
 def _check(x, gate_up, gate_up_scale, down, down_scale, topk_weights, topk_ids) -> None:
-    named = {"gate_up": gate_up, "gate_up_scale": gate_up_scale, "down": down, "down_scale": down_scale,
-             "topk_weights": topk_weights, "topk_ids": topk_ids}
-    if not on_device_of(x, *named.values()):
+    if not on_device_of(x, gate_up, gate_up_scale, down, down_scale, topk_weights, topk_ids):
         require_cuda(x, "x")
-        for name, t in named.items():
+        for name, t in (("gate_up", gate_up), ("gate_up_scale", gate_up_scale), ("down", down), ("down_scale", down_scale),
+                        ("topk_weights", topk_weights), ("topk_ids", topk_ids)):
             require_cuda(t, name)
             require_same_device(t, name, x, "x")
     if x.dtype not in ATTENTION_DTYPES:

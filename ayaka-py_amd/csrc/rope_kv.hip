@@ -270,32 +270,71 @@ __global__ __launch_bounds__(kRopeThreads) void rope_write_rows_kernel(RopeArgs 
   }
 }
 
+struct GatherArgs {
+  const uint8_t *codes, *scales;
+  const int64_t* slots;
+  void* dest;
+  int64_t n, num_slots, page_size;
+  int page_shift, dim, kv_heads, tile;  // tile: slots of a workgroup
+  // j / (dim / 8) = mulhi(j, magic) >> shift for j < 2^31, and j / (kv_heads dim / 8)
+  uint32_t head_magic, head_shift, row_magic, row_shift;
+};
+constexpr int kGatherSpans = 4;  // chunks of a thread whose loads are in flight at once
+
 // Rows of a 4-bit plane by slot, widened: destination [n, kv_heads, dim]. A thread takes 8 codes of
-// one head of one slot, the heads of a slot side by side, so that the stores, two thirds of the
+// one head of one slot at a time, the heads of a slot side by side, so that the stores, two thirds of the
 // bytes and more, are consecutive. Slots outside the plane give zeros.
 template <int DT, bool WIDE>
-__global__ __launch_bounds__(kRopeThreads) void mx4_gather_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                  int64_t num_slots, int64_t page_size, int page_shift, int kv_heads, int dim,
-                                                                  const int64_t* __restrict__ slots, int64_t n,
-                                                                  void* __restrict__ dest) {
-  const uint32_t chunk = blockIdx.x * kRopeThreads + threadIdx.x, per_head = dim / 8, per_row = kv_heads * per_head;
-  const uint32_t i = chunk / per_row, h = (chunk - i * per_row) / per_head, d = (chunk - i * per_row - h * per_head) * 8;
-  if (i >= n) return;
-  const int64_t e = (int64_t)chunk * 8, slot = slots[i];
-  float x[8] = {};
-  if (slot >= 0 && slot < num_slots) {
-    const int64_t row = mx4_row(slot, page_size, page_shift, kv_heads) + h * page_size;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * (dim / 2) + d / 2);
-    mx4_decode8(w, u2f((uint32_t)scales[row * (dim / kMxGroup) + d / kMxGroup] << 23), x);
-  }
-  if constexpr (WIDE && DT == AYK_F32) {
-    reinterpret_cast<float4*>(static_cast<float*>(dest) + e)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(static_cast<float*>(dest) + e)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else if constexpr (WIDE) {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dest) + e) = narrow8<DT>(x);
-  } else {
+__global__ __launch_bounds__(kRopeThreads) void mx4_gather_kernel(GatherArgs a) {
+  const int64_t first = (int64_t)blockIdx.x * a.tile, left = a.n - first;
+  const uint32_t per_head = a.dim / 8, per_row = a.kv_heads * per_head;
+  const uint32_t total = (uint32_t)(left < a.tile ? left : a.tile) * per_row;
+  for (uint32_t base = threadIdx.x; base < total; base += kGatherSpans * kRopeThreads) {
+    int64_t slot[kGatherSpans];
+    uint32_t h[kGatherSpans], c[kGatherSpans], w[kGatherSpans], scale[kGatherSpans];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) store_f32(dest, DT, e + q, x[q]);
+    for (int k = 0; k < kGatherSpans; ++k) {
+      const uint32_t j = min(base + k * kRopeThreads, total - 1), i = __umulhi(j, a.row_magic) >> a.row_shift;
+      h[k] = __umulhi(j - i * per_row, a.head_magic) >> a.head_shift;
+      c[k] = j - i * per_row - h[k] * per_head;
+      slot[k] = a.slots[first + i];
+    }
+#pragma unroll
+    for (int k = 0; k < kGatherSpans; ++k) {
+      // (row 0 for a slot outside: a load under a branch would wait for those before it)
+      const bool known = slot[k] >= 0 && slot[k] < a.num_slots;
+      const int64_t row = known ? mx4_row(slot[k], a.page_size, a.page_shift, a.kv_heads) + h[k] * a.page_size : 0;
+      w[k] = *reinterpret_cast<const uint32_t*>(a.codes + row * (a.dim / 2) + 4 * c[k]);
+      scale[k] = a.scales[row * (a.dim / kMxGroup) + c[k] / 4];
+      if (!known) slot[k] = -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kGatherSpans; ++k) {
+      const uint32_t j = base + k * kRopeThreads;
+      if (j >= total) break;
+      const int64_t e = (first * per_row + j) * 8;
+      const float sc = u2f(scale[k] << 23);
+      const bool known = slot[k] >= 0;
+      if constexpr (WIDE && DT == AYK_BF16) {  // exact in bf16
+        uint4 r = make_uint4(mx4_widen2<0>(w[k], sc), mx4_widen2<1>(w[k], sc), mx4_widen2<2>(w[k], sc), mx4_widen2<3>(w[k], sc));
+        if (!known) r = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dest) + e) = r;
+      } else {
+        float x[8];
+        mx4_decode8(w[k], sc, x);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = known ? x[q] : 0.0f;
+        if constexpr (WIDE && DT == AYK_F32) {
+          reinterpret_cast<float4*>(static_cast<float*>(a.dest) + e)[0] = make_float4(x[0], x[1], x[2], x[3]);
+          reinterpret_cast<float4*>(static_cast<float*>(a.dest) + e)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else if constexpr (WIDE) {
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dest) + e) = narrow8<DT>(x);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) store_f32(a.dest, DT, e + q, x[q]);
+        }
+      }
+    }
   }
 }
 
@@ -440,14 +479,29 @@ int ayk_kv_gather_mxfp4(const void* codes, const void* scales, int64_t num_pages
   if (slots == nullptr || dest == nullptr || (num_pages > 0 && (codes == nullptr || scales == nullptr)))
     return fail(AYK_EINVAL, "%s: missing operand", op);
   if (reinterpret_cast<uintptr_t>(codes) % 4) return fail(AYK_EINVAL, "%s: codes must be 4-byte aligned", op);
-  const int64_t blocks = n <= 0x7FFFFFFF ? cdiv(n * kv_heads * dim / 8, kRopeThreads) : kMostGroups + 1;
-  if (blocks > kMostGroups) return fail(AYK_EINVAL, "%s: too many rows", op);
+  const int64_t per_head = dim / 8, per_row = kv_heads * per_head;
+  GatherArgs a{};
+  // A thread takes its spans where that leaves a workgroup for every CU twice.
+  const int64_t fill = kGatherSpans * kRopeThreads / per_row, spread = n / 512;
+  a.tile = (int)(fill < spread ? fill : spread);
+  if (a.tile < kRopeThreads / per_row) a.tile = (int)(kRopeThreads / per_row);
+  if (a.tile < 1) a.tile = 1;
+  const int64_t blocks = cdiv(n, a.tile);
+  if (n > 0x7FFFFFFF || blocks > kMostGroups) return fail(AYK_EINVAL, "%s: too many rows", op);
   if (int rc = check_device()) return rc;
+  a.slots = slots, a.dest = dest, a.n = n, a.num_slots = num_pages * page_size, a.page_size = page_size;
+  // (a plane without pages has nothing to read: the destination stands in for it, whatever it holds)
+  a.codes = static_cast<const uint8_t*>(a.num_slots > 0 ? codes : dest);
+  a.scales = static_cast<const uint8_t*>(a.num_slots > 0 ? scales : dest);
+  a.page_shift = page_shift_of(page_size), a.dim = (int)dim, a.kv_heads = (int)kv_heads;
+  auto magic = [](int64_t by, uint32_t& m, uint32_t& shift) {  // 2^(31 + s) / by rounded up, by <= 2^s
+    const int bits = 64 - __builtin_clzll((uint64_t)by - 1);
+    m = (uint32_t)cdiv((int64_t)1 << (31 + bits), by), shift = bits - 1;
+  };
+  magic(per_head, a.head_magic, a.head_shift);
+  magic(per_row, a.row_magic, a.row_shift);
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define AYK_MXG(D, W)                                                                                                        \
-  hipLaunchKernelGGL((mx4_gather_kernel<D, W>), dim3((unsigned)blocks), dim3(kRopeThreads), 0, st,                            \
-                     static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), num_pages * page_size, page_size, \
-                     page_shift_of(page_size), (int)kv_heads, (int)dim, slots, n, dest)
+#define AYK_MXG(D, W) hipLaunchKernelGGL((mx4_gather_kernel<D, W>), dim3((unsigned)blocks), dim3(kRopeThreads), 0, st, a)
   const bool wide = aligned16(dest);
   if (dest_dtype == AYK_F32) { if (wide) AYK_MXG(AYK_F32, true); else AYK_MXG(AYK_F32, false); }
   else if (dest_dtype == AYK_F16) { if (wide) AYK_MXG(AYK_F16, true); else AYK_MXG(AYK_F16, false); }
