@@ -24,6 +24,7 @@ namespace {
 struct MxArgs : DecodeArgs {
   const uint8_t *ks, *vs;  // scales
   uint32_t page_rows;      // kv_heads page_size: rows of a page
+  uint32_t q_sign;         // exclusive-or of Q: a negative scale's sign, so that the factor of the scores is not
 };
 
 // What a wave holds of an item: D dims (the next of 64, 128, 256).
@@ -42,13 +43,7 @@ __device__ inline int mx_k_dim(int s, int quad) {
   return D == 64 ? 16 * quad + 8 * s : 128 * (s / 4) + 32 * quad + 8 * (s % 4);
 }
 
-template <bool ONCE, typename T>
-__device__ inline T mx_load(const uint8_t* p) {
-  if constexpr (ONCE && sizeof(T) >= 4) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
-  else return *reinterpret_cast<const T*>(p);
-}
-
-template <int QT, int D, bool EXACT, int WAVES, bool ONCE>
+template <int QT, int D, bool EXACT, int WAVES>
 __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int tile, int from, int to, Running<D>& r) {
   using S = MxShape<D>;
   typedef uint32_t v2u __attribute__((ext_vector_type(2)));
@@ -79,6 +74,7 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
 #pragma unroll
         for (int e = 0; e < 4; ++e) qf[s][e] = (uint32_t)p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
       }
+      qf[s] ^= a.q_sign;
     }
     if constexpr (kSplitQ) {
 #pragma unroll
@@ -129,9 +125,9 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
       for (int h = 0; h < S::kParts; ++h) {
         const int dim = mx_k_dim<D>(4 * h, quad), there = EXACT || dim < a.dim ? dim : 0;
         const uint8_t* p = kc + at * row_bytes + there / 2;
-        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = mx_load<ONCE, v2u>(p);
-        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = mx_load<ONCE, v4u>(p);
-        kse[t][h] = mx_load<false, uint8_t>(ks + at * groups + there / kMxGroup);
+        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = *reinterpret_cast<const v2u*>(p);
+        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = *reinterpret_cast<const v4u*>(p);
+        kse[t][h] = *reinterpret_cast<const uint8_t*>(ks + at * groups + there / kMxGroup);
       }
     }
   };
@@ -146,11 +142,11 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint8_t* p = vc + (eight + j) * row_bytes + v_dim / 2;
-      if constexpr (D == 64) vw[j][0] = mx_load<ONCE, uint16_t>(p);
-      else if constexpr (D == 128) vw[j][0] = mx_load<ONCE, uint32_t>(p);
-      else *reinterpret_cast<v2u*>(vw[j]) = mx_load<ONCE, v2u>(p);
+      if constexpr (D == 64) vw[j][0] = *reinterpret_cast<const uint16_t*>(p);
+      else if constexpr (D == 128) vw[j][0] = *reinterpret_cast<const uint32_t*>(p);
+      else *reinterpret_cast<v2u*>(vw[j]) = *reinterpret_cast<const v2u*>(p);
       if constexpr (!kVector) {
-        const uint32_t code = mx_load<false, uint8_t>(vs + (eight + j) * groups + v_group);
+        const uint32_t code = *reinterpret_cast<const uint8_t*>(vs + (eight + j) * groups + v_group);
         if constexpr (D == 64) vse[j / 2] = (j % 2 ? vse[j / 2] : 0) | code << (16 * (j % 2) + 8 * v_group);
         else vse[j] = code;
       }
@@ -190,16 +186,19 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
     page = page_of(following(next));
     issue_k(row);
     float x[8], vsc[8], top = -INFINITY;
+    uint32_t hidden = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[j] = s[j / 4][j % 4] * a.scale_log2;
-      const uint32_t code = D == 64 ? vse[j / 2] >> (16 * (j % 2) + 8 * v_group) : kVector ? vse[j] >> (8 * v_group) : vse[j];
-      vsc[j] = u2f((code & 0xFFu) << 23);
+      x[j] = s[j / 4][j % 4];
+      // (of a scale the converter takes the exponent's eight bits alone: those around the code may stay)
+      const uint32_t word = D == 64 ? vse[j / 2] : vse[j], low = D == 64 ? 16 * (j % 2) : 0;
+      vsc[j] = u2f(D == 64 || kVector ? __builtin_amdgcn_alignbit(word, word, 8 * v_group + low + 9) : word << 23);
     }
     if (now != 0xFFFFFFFFu) {
+      hidden = ~(now >> 8 * quad);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool on = (now >> (8 * quad + j)) & 1;
+        const bool on = !(hidden >> j & 1);
         x[j] = on ? x[j] : -INFINITY;
         vsc[j] = on ? vsc[j] : 0.0f;  // a weight of 0 times a hidden NaN
 #pragma unroll
@@ -208,8 +207,11 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
-    top = fmaxf(r.m, max_quads(top));
-    if (__ballot(top > r.m)) {  // wave-uniform: some head's maximum grew
+    top = max_quads(top) * a.scale_log2;
+    // The maximum moves only when a score beats it by 2^8: until then weights may reach 256, which no
+    // sum or type minds, and O need not be rescaled (wave-uniform: for some head).
+    if (__ballot(top > r.m + 8.0f)) {
+      top = fmaxf(r.m, top);
       const float keep = r.m == -INFINITY ? 0.0f : exp2_fast(r.m - top);
       r.m = top;
       r.l *= keep;
@@ -217,11 +219,17 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
       for (int t = 0; t < D / 16; ++t) r.acc[t] *= keep;
     }
     const float base = r.m == -INFINITY ? 0.0f : r.m;  // nothing visible so far weighs 0
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __builtin_fmaf(x[j], a.scale_log2, -base);
+    if (now != 0xFFFFFFFFu) {  // (a factor of 0 makes NaN of a hidden score)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = hidden >> j & 1 ? -INFINITY : x[j];
+    }
     v4u p, pl;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      x[j] = exp2_fast(x[j] - base);
-      x[j + 1] = exp2_fast(x[j + 1] - base);
+      x[j] = exp2_fast(x[j]);
+      x[j + 1] = exp2_fast(x[j + 1]);
       r.l += x[j];
       r.l += x[j + 1];
       p[j / 2] = pack2<AYK_BF16>(x[j], x[j + 1]);
@@ -300,7 +308,7 @@ __global__ __launch_bounds__(WAVES * kWave, (MxShape<D>::kWavesPerSimd)) void mx
   __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_mx<QT, D, EXACT, WAVES, false>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
+  attend_mx<QT, D, EXACT, WAVES>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
   join_waves<D, WAVES>(r, lds);
   if (threadIdx.x < kWave) write_mx<QT, D, EXACT>(a, b, g, tile, r, nullptr);
 }
@@ -309,7 +317,7 @@ __global__ __launch_bounds__(WAVES * kWave, (MxShape<D>::kWavesPerSimd)) void mx
 // workgroup, whatever the lengths. A run may end one item, hold some whole and begin another; what
 // it does not hold whole it leaves as a partial result, in slot 0 (the run begins inside the item) or
 // slot 1 (it ends inside).
-template <int QT, int D, bool EXACT, bool ONCE>
+template <int QT, int D, bool EXACT>
 __global__ __launch_bounds__(kDecodeThreads, (MxShape<D>::kWavesPerSimd)) void mx_decode_split_kernel(MxArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
   const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
@@ -333,7 +341,7 @@ __global__ __launch_bounds__(kDecodeThreads, (MxShape<D>::kWavesPerSimd)) void m
       const int last = first + (end - at) < steps ? first + (end - at) : steps;
       Running<D> r;
       const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
-      attend_mx<QT, D, EXACT, 4, ONCE>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
+      attend_mx<QT, D, EXACT, 4>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
       join_waves<D, 4>(r, lds);
       float* partial = nullptr;
       if (first > 0 || last < steps) partial = a.partial + ((int64_t)run * 2 + (first > 0 ? 0 : 1)) * a.rows * (D + 2);
@@ -355,7 +363,7 @@ int launch_mx(const MxArgs& a, bool split, hipStream_t st) {
     note_plan("paged_decode_mxfp4 whole");
   } else {
     constexpr int runs = 256 * MxShape<D>::kWavesPerSimd;
-    hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT, false>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
     launch_join<QT, D, 1>(a, runs, st);
     note_plan("paged_decode_mxfp4 split");
   }
@@ -378,7 +386,7 @@ int64_t mx_longest(int64_t most, int64_t window, int64_t sinks) {
 }
 bool mx_deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest) {
   const int64_t items = batch * cdiv(heads / kv_heads, kHeadTile) * kv_heads;
-  const int64_t limit = (items <= 256 ? 640 : items < 512 ? 400 : 560) * 1024 / mx_width(dim);
+  const int64_t width = mx_width(dim), limit = items <= 256 ? 1300 - 3 * width + 15 * items : (items < 512 ? 400 : 560) * 1024 / width;
   return longest > limit && items * (cdiv(longest, kStep) + 1) < 0x40000000;
 }
 
@@ -451,7 +459,8 @@ int ayk_paged_decode_attention_mxfp4(const void* q, int q_dtype, int64_t q_row_s
   a.tiles = (int)tiles;
   a.rows = (int)(group < kHeadTile ? group : kHeadTile);
   a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctzll((uint64_t)page_size);
-  a.scale_log2 = scale * kLog2e;
+  a.scale_log2 = fabsf(scale) * kLog2e;
+  a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   a.v_scale = 1.0f;
   a.window = (int)(window < 0x7FFFFFFF ? window : 0x7FFFFFFF);
   a.sinks = (int)(sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF);
