@@ -45,7 +45,7 @@ struct MoeArgs {
 // number the rows alike.
 struct MoeList {
   uint64_t tokens[kMoeExperts];
-  uint16_t expert[kMoeExperts], row[kMoeExperts];
+  uint16_t expert[kMoeExperts], row[kMoeExperts + 1];  // row: one more behind the last entry
   int count;
 };
 // masks: room for kMoeExperts in LDS while the list is made.
@@ -76,6 +76,7 @@ __device__ inline void list_experts(const MoeArgs& a, MoeList& l, uint64_t* mask
         l.expert[at] = (uint16_t)mine;
         l.tokens[at] = mask;
         l.row[at] = (uint16_t)rows;
+        if (at + 1 == __popcll(leaders)) l.row[at + 1] = (uint16_t)(rows + count);
       }
       if (lane == 0) l.count = __popcll(leaders);
     }
@@ -105,7 +106,10 @@ __device__ inline void list_experts(const MoeArgs& a, MoeList& l, uint64_t* mask
       count += __popcll(used);
       rows += __builtin_amdgcn_readlane(upto, kWave - 1);
     }
-    if (threadIdx.x == 0) l.count = count;
+    if (threadIdx.x == 0) {
+      l.count = count;
+      l.row[count] = (uint16_t)rows;
+    }
   }
   __syncthreads();
 }
@@ -122,7 +126,8 @@ __device__ inline uint64_t uniform(uint64_t v) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32;
 }
-__device__ inline int power_of_two_from(int n) { return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)); }
+__device__ inline int log2_from(int n) { return n <= 1 ? 0 : 32 - __builtin_clz(n - 1); }  // rounded up
+__device__ inline int power_of_two_from(int n) { return 1 << log2_from(n); }
 
 template <int DT>
 __device__ inline v4u widen8(uint32_t a, uint32_t b) {
@@ -154,6 +159,23 @@ __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"
 // A barrier behind this wave's accesses to LDS; direct loads stay in flight (__syncthreads waits for
 // stores to global memory, and with them for every load).
 __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+// Four floats from one workgroup to another, wherever on the chip it runs: accesses of the agent's scope.
+__device__ inline void store_past_caches(float* to, v4f v) { asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(to), "v"(v) : "memory"); }
+__device__ inline void load_past_caches(const float* const (&from)[8], v4f (&v)[8]) {
+  asm volatile(
+      "global_load_dwordx4 %0, %8, off sc1\n\tglobal_load_dwordx4 %1, %9, off sc1\n\tglobal_load_dwordx4 %2, %10, off sc1\n\t"
+      "global_load_dwordx4 %3, %11, off sc1\n\tglobal_load_dwordx4 %4, %12, off sc1\n\tglobal_load_dwordx4 %5, %13, off sc1\n\t"
+      "global_load_dwordx4 %6, %14, off sc1\n\tglobal_load_dwordx4 %7, %15, off sc1\n\ts_waitcnt vmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3]), "v"(from[4]), "v"(from[5]), "v"(from[6]), "v"(from[7])
+      : "memory");
+}
+// Four values rounded to the output, which need not be aligned.
+template <int DT>
+__device__ inline void store_four(uint16_t* out, int64_t at, v4f v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_f32(out, DT, at + e, v[e]);
+}
 // Sixteen bytes a lane of both loads of a half block of weights; with it the k slots of the four steps
 // of this lane's row. The reads are done when the block ends.
 __device__ inline void read_half(uint32_t weights, v4u (&w)[2]) {
@@ -229,6 +251,20 @@ struct GateWalk {
   }
 };
 
+// Sixty-four entries of the list, one a lane: a look at one costs no trip to LDS.
+struct Entries {
+  int base, packed, first;  // number of lane 0's; expert and rows; first row of h
+  __device__ void hold(const MoeList& l, int from) {
+    base = from;
+    const int e = min(from + (int)(threadIdx.x % kWave), kMoeExperts - 1);  // (those past the list are not asked for)
+    first = l.row[e];
+    // (64 tokens of 1024 experts are 2^16 rows: the difference is taken in 16 bits)
+    packed = l.expert[e] | (uint16_t)(l.row[e + 1] - first) << 16;
+  }
+  __device__ int expert(int u) const { return __builtin_amdgcn_readlane(packed, u - base) & 0xFFFF; }
+  __device__ int rows(int u) const { return (uint32_t)__builtin_amdgcn_readlane(packed, u - base) >> 16; }
+  __device__ int row(int u) const { return __builtin_amdgcn_readlane(first, u - base); }
+};
 template <int DT>
 __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) {
   __shared__ MoeList list;
@@ -259,29 +295,39 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   walk.enter(list);
 
   // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes. A wave's
-  // blocks of a chunk are its number and every eighth from there; past the last the same loads are
-  // issued again, so that the waits count the same throughout.
+  // blocks of an item's pass are its number and every eighth from there, whatever the chunks (all but
+  // a pass's last are whole eights); past the last pass that is loaded again, so that the waits count
+  // the same throughout.
   const uint32_t lane_at = (uint32_t)col * a.hidden + 16 * quad, ring = lds_address(rings[wave]);
-  GateWalk ahead = walk;
-  int at = wave;  // block within ahead's chunk
-  while (ahead.count && at >= ahead.count) ahead.next(list);
+  Entries entries;
+  entries.hold(list, walk.u);
   const int64_t up_bytes = (int64_t)a.inner * a.hidden;
+  int item = walk.item, entry = walk.u, slice = walk.slice, pass = 0, passes = 1, at = wave;
   const uint8_t* from = a.gate_up;
-  auto point = [&]() {
-    if (ahead.count)
-      from = a.gate_up + ((int64_t)ahead.expert * 2 * a.inner + 16 * ahead.slice) * a.hidden + (int64_t)(ahead.b0 + at) * kMoeBlock;
+  auto point = [&]() {  // at this wave's first block (one without any loads the last, and does not read it)
+    passes = (entries.rows(entry) + kGateRows - 1) / kGateRows;
+    from = a.gate_up + ((int64_t)entries.expert(entry) * 2 * a.inner + 16 * slice) * a.hidden + min(wave, blocks - 1) * kMoeBlock;
+    at = wave;
   };
   point();
   auto issue = [&](int to, bool up) {
     load_to_lds(from + (up ? up_bytes : 0), lane_at, ring + 2048 * to);
     load_to_lds(from + (up ? up_bytes : 0) + 64, lane_at, ring + 2048 * to + 1024);
-    if (!up || !ahead.count) return;
+    if (!up) return;
     at += kMoeWaves;
-    if (at >= ahead.count) {
-      do {
-        ahead.next(list);
-        at = wave;
-      } while (ahead.count && at >= ahead.count);
+    if (at < blocks) {
+      from += kMoeWaves * kMoeBlock;
+      return;
+    }
+    if (++pass >= passes) {
+      pass = 0;
+      if (item + 1 < walk.last) {
+        ++item;
+        if (++slice == walk.slices) {
+          slice = 0;
+          ++entry;  // (no run has more than five: 8192 items of 1024 experts over 256 workgroups)
+        }
+      }
     }
     point();
   };
@@ -428,52 +474,52 @@ __device__ inline void read_block(uint32_t weights, uint32_t at, uint32_t scales
       : "memory");
 }
 
-// A walk over the chunks of a workgroup's run, [unit, last) in the list of (expert, block). All but
-// `table` is the same in all lanes. An entry of more than kDownRows rows takes a chunk's blocks in
-// passes, one after the other.
+// A walk over the chunks of a workgroup's run, [unit, last) in the list of (expert, block). All is the
+// same in all lanes. A chunk goes on into the next entries while its rows, as many for every unit, have
+// room: with one entry a chunk, two blocks of 128 k an expert took 1.4 us each, a trip to memory. An
+// entry of more than kDownRows rows takes its units one by one, each in passes.
 constexpr int kDownRows = 32;
 struct DownWalk {
-  int unit, last, blocks;      // the chunk's first unit; the run's end; blocks of an expert
-  int u, b, r0, count;         // entry of the list, first block, first row, blocks of the chunk (0: the run is over)
-  int expert, first_row, all;  // of the entry: expert, first row of h, rows
-  int rows, stride;            // rows of the pass, and rounded up to a power of two
-  int table;                   // the entry's tokens
-  __device__ void enter(const MoeList& l) {  // the entry of `unit`
+  int unit, last, blocks;  // the chunk's first unit; the run's end; blocks of an expert
+  int u, b, r0;            // entry of the list and block of the first unit, first row of the pass
+  int count, shift;        // units of the chunk (0: the run is over), rows of each: 2^shift
+  int all;                 // rows of entry u
+  __device__ void start(const MoeList& l, Entries& e) {
     u = unit / blocks;
     b = unit - u * blocks;
-    expert = __builtin_amdgcn_readfirstlane(l.expert[u]);
-    first_row = __builtin_amdgcn_readfirstlane(l.row[u]);
-    const uint64_t tokens = uniform(l.tokens[u]);
-    table = token_table(tokens);
-    all = __popcll(tokens);
-    pass(0);
-    size();
+    e.hold(l, u);
+    size(l, e);
   }
-  __device__ void pass(int first) {
-    r0 = first;
-    rows = all - r0 < kDownRows ? all - r0 : kDownRows;
-    stride = power_of_two_from(rows);
+  __device__ void size(const MoeList& l, Entries& e) {
+    r0 = 0;
+    if (u + kDownPairs - e.base > kWave) e.hold(l, u);  // the entries of a chunk are held together
+    all = e.rows(u);
+    shift = log2_from(min(all, kDownRows));
+    count = min(min(blocks - b, last - unit), kDownPairs >> shift);
+    if (all > kDownRows) return;
+    for (int v = u + 1; unit + count < last && b + count == (v - u) * blocks; ++v) {
+      const int rows = e.rows(v), wide = max(shift, log2_from(rows)), room = (kDownPairs >> wide) - count;
+      if (rows > kDownRows || room <= 0) break;
+      shift = wide;
+      count += min(min(room, blocks), last - unit - count);
+    }
   }
-  __device__ void size() {  // by the first pass, which has most rows
-    const int most = kDownPairs / stride;
-    count = blocks - b < last - unit ? blocks - b : last - unit;
-    if (count > most) count = most;
-  }
-  __device__ void next(const MoeList& l) {
+  __device__ void next(const MoeList& l, Entries& e) {
     if (r0 + kDownRows < all) {
-      pass(r0 + kDownRows);
+      r0 += kDownRows;
       return;
     }
     unit += count;
     b += count;
     if (unit >= last) {
       count = 0;
-    } else if (b == blocks) {
-      enter(l);
-    } else {
-      if (r0) pass(0);
-      size();
+      return;
     }
+    if (b >= blocks) {
+      u += b / blocks;
+      b %= blocks;
+    }
+    size(l, e);
   }
 };
 
@@ -483,7 +529,7 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   __shared__ alignas(1024) uint8_t stage[2][kDownPairs * kPairBytes];
   __shared__ alignas(1024) uint8_t rings[kMoeWaves][kRingBytes];
   __shared__ float scales[2][kMoeWaves][kWave];  // of a chunk's blocks
-  extern __shared__ float sums[];                // [tokens][kTokenFloats], room for kMoeThreads at least
+  extern __shared__ __attribute__((aligned(16))) float sums[];  // [tokens][kTokenFloats], room for 4 kMoeThreads at least
   list_experts(a, list, reinterpret_cast<uint64_t*>(stage));
   for (int i = threadIdx.x; i < a.tokens * kTokenFloats; i += kMoeThreads) sums[i] = 0.0f;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), col = lane % 16, quad = lane / 16;
@@ -494,40 +540,75 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
   walk.unit = (int)(units * blockIdx.y / gridDim.y);
   walk.last = (int)(units * (blockIdx.y + 1) / gridDim.y);
   if (walk.unit < walk.last) {
-    walk.enter(list);
+    Entries held, held_ahead;
+    walk.start(list, held);
+    held_ahead = held;
     // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes.
     const uint8_t* panel = a.down + (int64_t)(n0 + 16 * wave) * a.inner;
     const uint32_t lane_at = (uint32_t)col * a.inner + 16 * quad, ring = lds_address(rings[wave]);
     const int64_t expert_bytes = (int64_t)a.hidden * a.inner;
-    DownWalk ahead = walk;
-    int at = 0, slot = 0;  // block within ahead's chunk; the ring's place that is read, and then filled, next
-    int64_t offset = ahead.expert * expert_bytes + (int64_t)ahead.b * kMoeBlock;
-    // Past the run's end the last block is loaded again, so that the waits count the same loads throughout.
+    // The unit whose weights are asked for next, and how often it is: in every pass of its entry. Past the
+    // run's end the last is loaded again, so that the waits count the same loads throughout.
+    int unit = walk.unit, entry = walk.u, block = walk.b, pass = 0, passes = 1, slot = 0;  // slot: the ring's place that is read, and then filled, next
+    int64_t offset = 0;
+    auto point = [&]() {
+      if (entry - held_ahead.base >= kWave) held_ahead.hold(list, entry);
+      passes = (held_ahead.rows(entry) + kDownRows - 1) / kDownRows;
+      offset = held_ahead.expert(entry) * expert_bytes + (int64_t)block * kMoeBlock;
+    };
+    point();
     auto issue = [&](int to) {
       load_to_lds(panel + offset, lane_at, ring + 2048 * to);
       load_to_lds(panel + offset + 64, lane_at, ring + 2048 * to + 1024);
-      if (++at < ahead.count) {
+      if (++pass >= passes && unit + 1 < walk.last) {
+        pass = 0;
+        ++unit;
         offset += kMoeBlock;
-      } else if (ahead.count) {
-        at = 0;
-        ahead.next(list);
-        if (ahead.count) offset = ahead.expert * expert_bytes + (int64_t)ahead.b * kMoeBlock;
+        if (++block == blocks) {
+          block = 0;
+          ++entry;
+          point();
+        }
       }
     };
     // Rows: a wave takes four pairs, two a load, and lane l piece l % 32 of its pair. Pieces are
     // exchanged within a pair so that the same piece of sixteen pairs lies in sixteen groups of banks.
     auto fetch = [&](const DownWalk& w, int buffer) {
-      const int shift = __builtin_ctz(w.stride);
+      const bool one = w.b + w.count <= blocks;  // of one entry
+      // expert, first row, rows and block of a unit (past the last: of that)
+      auto locate = [&](int c, int& expert, int& first, int& rows, int& k) {
+        k = w.b + min(c, w.count - 1);
+        expert = held.expert(w.u), first = held.row(w.u), rows = held.rows(w.u);
+        if (!one) {
+          const int past = k / blocks, from = 4 * (w.u + past - held.base);
+          k -= past * blocks;
+          first = __builtin_amdgcn_ds_bpermute(from, held.first);
+          const uint32_t packed = __builtin_amdgcn_ds_bpermute(from, held.packed);
+          expert = packed & 0xFFFF, rows = packed >> 16;
+        }
+      };
+      int expert, first, rows, k;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int pair = 4 * wave + 2 * i + lane / 32, row = pair & (w.stride - 1), block = pair >> shift;
-        const int64_t r = w.first_row + w.r0 + (row < w.rows ? row : 0);
-        const int k = w.b + (block < w.count ? block : 0);
+        const int pair = 4 * wave + 2 * i + lane / 32, row = pair & ((1 << w.shift) - 1);
+        locate(pair >> w.shift, expert, first, rows, k);
+        const int64_t r = first + w.r0 + (w.r0 + row < rows ? row : 0);
         load_to_lds(reinterpret_cast<const uint8_t*>(a.h) + (r * a.inner + k * kMoeBlock) * 4 + 16 * ((lane % 32) ^ (pair & 15)),
                     lds_address(stage[buffer] + (4 * wave + 2 * i) * kPairBytes));
       }
-      word_to_lds(a.down_scale + ((int64_t)w.expert * panels + blockIdx.x) * blocks + w.b + (lane < w.count ? lane : 0),
-                  lds_address(scales[buffer][wave]));
+      locate(lane, expert, first, rows, k);
+      word_to_lds(a.down_scale + ((int64_t)expert * panels + blockIdx.x) * blocks + k, lds_address(scales[buffer][wave]));
+    };
+    v4f total[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // of the entry's pass
+    auto join = [&](int u, int r0) {  // it to its tokens
+      const uint64_t tokens = uniform(list.tokens[u]);
+      const int table = token_table(tokens), rows = __popcll(tokens) - r0;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int t = token_of(table, r0 + 16 * r + col);
+        if (16 * r + col < min(rows, kDownRows)) *reinterpret_cast<v4f*>(sums + t * kTokenFloats + 16 * wave + 4 * quad) += total[r];
+        total[r] = v4f{0, 0, 0, 0};
+      }
     };
     fetch(walk, 0);
 #pragma unroll
@@ -535,14 +616,15 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
     wait_loads<2 * kDownAhead>();
     __builtin_amdgcn_s_barrier();
     int buffer = 0;
-    v4f total[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // of the entry's pass
     while (true) {
       DownWalk following = walk;
-      following.next(list);
-      fetch(following.count ? following : walk, buffer ^ 1);
-      const bool two = walk.rows > 16;
+      following.next(list, held);
+      if (following.count) fetch(following, buffer ^ 1);
+      else fetch(walk, buffer ^ 1);
+      const bool two = walk.all - walk.r0 > 16;  // (then a chunk is one unit)
+      int u = walk.u, b = walk.b;
       for (int c = 0; c < walk.count; ++c) {
-        const int pair = c * walk.stride + (col & (walk.stride - 1));
+        const int pair = (c << walk.shift) + (col & ((1 << walk.shift) - 1));
         const uint32_t rows = lds_address(stage[buffer]) + pair * kPairBytes + 16 * ((4 * quad) ^ (pair & 15));
         float scale;
         v4u w[2], f[4];
@@ -569,13 +651,11 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
           }
           total[1] += (sum[0] + sum[1]) * scale;
         }
-      }
-      if (following.count == 0 || following.u != walk.u || following.r0 != walk.r0) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int t = token_of(walk.table, walk.r0 + 16 * r + col);
-          if (16 * r + col < walk.rows) *reinterpret_cast<v4f*>(sums + t * kTokenFloats + 16 * wave + 4 * quad) += total[r];
-          total[r] = v4f{0, 0, 0, 0};
+        const bool ends = ++b == blocks;
+        if (ends || (c + 1 == walk.count && (following.count == 0 || walk.all > kDownRows))) join(u, walk.r0);
+        if (ends) {
+          ++u;
+          b = 0;
         }
       }
       if (following.count == 0) break;
@@ -598,45 +678,48 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
       store_f32(a.out, DT, i / kMoeBlock * a.ldo + n0 + i % kMoeBlock, sums[i / kMoeBlock * kTokenFloats + i % kMoeBlock]);
     return;
   }
-  // Partial results pass from one chip part's cache to another's as atomics of the agent's scope, which
+  // Partial results pass from one chip part's cache to another's as accesses of the agent's scope, which
   // go to memory and come from there. A fence would do the same for plain ones by writing back the
   // whole cache, once a wave: 35 us of the launch. What orders them is that the stores are done, for all
   // waves, before the count goes up.
   const int64_t plane = (int64_t)tokens * a.hidden;
-  for (int i = threadIdx.x; i < tokens * kMoeBlock; i += kMoeThreads)
-    __hip_atomic_store(a.partial + blockIdx.y * plane + (int64_t)(i / kMoeBlock) * a.hidden + n0 + i % kMoeBlock,
-                       sums[i / kMoeBlock * kTokenFloats + i % kMoeBlock], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int cells = tokens * (kMoeBlock / 4);  // of four channels
+  for (int i = threadIdx.x; i < cells; i += kMoeThreads) {
+    const int t = i / (kMoeBlock / 4), n = i % (kMoeBlock / 4) * 4;
+    store_past_caches(a.partial + blockIdx.y * plane + (int64_t)t * a.hidden + n0 + n, *reinterpret_cast<const v4f*>(sums + t * kTokenFloats + n));
+  }
   wait_loads<0>();  // and stores
   __syncthreads();
   __shared__ int arrived;
   if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(a.arrived + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (arrived != (int)gridDim.y - 1) return;
-  // A few threads a cell where the cells are few; eight loads at a time, as each goes to memory.
-  const int cells = tokens * kMoeBlock, runs = gridDim.y, share = cells < kMoeThreads ? kMoeThreads / cells : 1;
+  // A few threads a cell where the cells are few; eight loads at a time, as each goes to memory (by single
+  // floats this took 20 us of 28 for 38 tokens and 14 runs).
+  const int runs = gridDim.y, share = max(1, min(kMoeThreads / cells, (runs + 7) / 8));
   for (int i = threadIdx.x; i < cells * share; i += kMoeThreads) {
-    const int cell = i % cells, first = i / cells;
-    const float* p = a.partial + (int64_t)(cell / kMoeBlock) * a.hidden + n0 + cell % kMoeBlock;
-    float sum = 0.0f;
+    const int cell = i % cells, first = i / cells, t = cell / (kMoeBlock / 4), n = n0 + cell % (kMoeBlock / 4) * 4;
+    const float* p = a.partial + (int64_t)t * a.hidden + n;
+    v4f sum{0, 0, 0, 0};
     for (int r0 = first; r0 < runs; r0 += 8 * share) {
-      float v[8];
+      const float* from[8];
+      v4f v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = r0 + k * share;
-        v[k] = r < runs ? __hip_atomic_load(p + r * plane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
-      }
+      for (int k = 0; k < 8; ++k) from[k] = p + min(r0 + k * share, runs - 1) * plane;
+      load_past_caches(from, v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += v[k];
+      for (int k = 0; k < 8; ++k)
+        if (r0 + k * share < runs) sum += v[k];
     }
-    if (share == 1) store_f32(a.out, DT, cell / kMoeBlock * a.ldo + n0 + cell % kMoeBlock, sum);
-    else sums[i] = sum;
+    if (share == 1) store_four<DT>(a.out, t * a.ldo + n, sum);
+    else reinterpret_cast<v4f*>(sums)[i] = sum;
   }
   if (share == 1) return;
   __syncthreads();
   for (int i = threadIdx.x; i < cells; i += kMoeThreads) {
-    float sum = 0.0f;
-    for (int k = 0; k < share; ++k) sum += sums[k * cells + i];
-    store_f32(a.out, DT, i / kMoeBlock * a.ldo + n0 + i % kMoeBlock, sum);
+    v4f sum{0, 0, 0, 0};
+    for (int k = 0; k < share; ++k) sum += reinterpret_cast<const v4f*>(sums)[k * cells + i];
+    store_four<DT>(a.out, i / (kMoeBlock / 4) * a.ldo + n0 + i % (kMoeBlock / 4) * 4, sum);
   }
 }
 
@@ -651,6 +734,7 @@ int down_runs(int64_t tokens, int64_t topk, int64_t experts, int64_t hidden, int
 
 // LDS of the second launch: what its declarations take, and the tokens' sums.
 constexpr size_t kDownLds = sizeof(MoeList) + 2 * kDownPairs * kPairBytes + kMoeWaves * (kRingBytes + 2 * 4 * kWave) + 64;
+static_assert(16 * kTokenFloats >= 4 * kMoeThreads, "the join's shares");
 static_assert(kDownLds + kMoeTokens * kTokenFloats * sizeof(float) <= 160 * 1024, "LDS of a CU");
 
 template <int DT>
@@ -659,7 +743,7 @@ int launch_moe(const MoeArgs& a, hipStream_t st) {
   const int64_t items = used * (a.inner / 16);
   hipLaunchKernelGGL((moe_gate_up_kernel<DT>), dim3((unsigned)(items < 256 ? items : 256)), dim3(kMoeThreads), 0, st, a);
   const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner));
-  hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), (a.tokens < 4 ? 4 : a.tokens) * kTokenFloats * sizeof(float), st, a);
+  hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), (a.tokens < 16 ? 16 : a.tokens) * kTokenFloats * sizeof(float), st, a);
   return check_launch("fp8_block_moe_small");
 }
 

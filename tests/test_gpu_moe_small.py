@@ -245,3 +245,44 @@ def test_refusals_on_the_device(gpu):
     refuse(ValueError, "rows that do not overlap", out=torch.empty(4, 512, dtype=BF16, device=gpu)[:, ::2])
     refuse(TypeError, "out must have dtype", out=torch.empty(4, 256, dtype=F16, device=gpu))
     refuse(ValueError, "must be a CUDA tensor|same CUDA device", topk_ids=c["topk_ids"].cpu())
+
+
+@pytest.mark.parametrize("inner", [128, 256, 384])
+def test_chunks_over_several_experts(gpu, inner):
+    """Long runs over experts of few blocks: one row each, some with many, some with more than a pass holds."""
+    c = moe_case(64, 90, 4, 4096, inner, seed=40)
+    ids = c["topk_ids"]
+    ids[:, 0] = torch.where(torch.arange(64) < 50, 11, ids[:, 0])  # 50 rows, behind and before small ones
+    ids[:, 1] = torch.where(torch.arange(64) % 3 == 0, 12, ids[:, 1])
+    ids[:, 2] = torch.where(torch.arange(64) >= 31, 60, ids[:, 2])  # 33 rows
+    ids[:, 3] = torch.where(torch.arange(64) >= 32, 89, ids[:, 3])  # 32 rows, the last entry
+    check(c, gpu, f"chunks over experts, inner={inner}")
+
+
+def test_runs_of_more_experts_than_a_wave_has_lanes(gpu):
+    """Two runs of 70 experts each a channel block; three tokens against their experts in 64 bits."""
+    say("moe long runs")
+    tokens, experts, topk, hidden, inner = 64, 150, 8, 16384, 128
+    g = torch.Generator(device=gpu).manual_seed(41)
+
+    def plane(*shape):
+        codes = torch.randint(0, 256, shape, generator=g, device=gpu, dtype=torch.uint8)
+        return torch.where((codes & 0x7F) == 0x7F, 0, codes).view(torch.float8_e4m3fn)
+
+    def scale(*shape):
+        return (torch.rand(*shape, generator=g, device=gpu) + 0.5) * (0.01 / (shape[-1] * 128) ** 0.5)
+
+    ids = torch.stack([torch.randperm(experts, generator=g, device=gpu)[:topk] for _ in range(tokens)]).to(torch.int32)
+    assert ids.unique().numel() > 130
+    c = {"x": torch.randn(tokens, hidden, generator=g, device=gpu).to(BF16), "gate_up": plane(experts, 2 * inner, hidden),
+         "gate_up_scale": scale(experts, 2 * inner // 128, hidden // 128), "down": plane(experts, hidden, inner),
+         "down_scale": scale(experts, hidden // 128, inner // 128),
+         "topk_weights": torch.rand(tokens, topk, generator=g, device=gpu), "topk_ids": ids}
+    out = run(c)
+    rows = [0, 29, 63]
+    used = ids[rows].unique()
+    part = {n: c[n][used.long()].cpu() for n in ("gate_up", "gate_up_scale", "down", "down_scale")}
+    part |= {n: c[n][rows].cpu() for n in ("x", "topk_weights")}
+    part["topk_ids"] = torch.searchsorted(used, ids[rows]).to(torch.int32).cpu()
+    ref, bound = moe_oracle(part)
+    assert_within(out[rows], ref, bound, "long runs")
