@@ -152,3 +152,37 @@ def test_a_captured_step_replayed(gpu, cache):
 def test_example_runs(gpu, capsys):
     _example().main()
     assert "step 3" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("cache", [None, E4M3])
+def test_a_compiled_step(gpu, cache):
+    """The operators in one graph of the compiler, mutations of cache and queries included."""
+    import ayaka.kernel.hip as H
+
+    ex = _example()
+    layers = [_layer(ex, gpu, cache) for _ in range(2)]
+    gen = torch.Generator().manual_seed(4)
+    tables = torch.arange(30, device=gpu).view(3, 10).to(torch.int32)
+    now = torch.tensor([40, 3, 17], dtype=torch.int32, device=gpu)
+    qkv = torch.randn(3, 12, 64, generator=gen).to(BF16).to(gpu)
+    ids = torch.tensor([[0, 1], [2, 7], [1, 1]], dtype=torch.int32, device=gpu)
+    weights = torch.rand(3, 2, generator=gen).to(gpu)
+
+    def step(layer, qkv, planes):
+        q, k, v = qkv.split((8, 2, 2), dim=1)
+        turned = torch.empty(3, 8, 64, dtype=BF16, device=gpu)
+        slots = ex.slots_of(tables, now - 1, 16)
+        if cache is None:
+            H.rope_write_kv_mxfp4(q, k, v, now.long() - 1, layer.table, *planes, slots, turned)
+            a = H.paged_decode_attention_mxfp4(turned, *planes, tables, now, 0.125)
+        else:
+            H.rope_write_kv(q, k, v, now.long() - 1, layer.table, *planes, slots, 16.0, 16.0, turned)
+            a = H.paged_decode_attention(turned, *planes, tables, now, 0.125, k_scale=1 / 16, v_scale=1 / 16)
+        x = a.flatten(1)
+        return turned, a, H.fp8_block_moe_small(x, layer.gate_up, layer.gate_up_scale, layer.down, layer.down_scale, weights, ids)
+
+    eager = step(layers[0], qkv, layers[0].planes)
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)(layers[1], qkv, layers[1].planes)
+    for got, want in (*zip(compiled, eager), *zip(layers[1].planes, layers[0].planes)):
+        assert torch.equal(bits(got), bits(want))
+    assert layers[1].planes[0].view(torch.uint8).any()

@@ -286,3 +286,16 @@ def test_runs_of_more_experts_than_a_wave_has_lanes(gpu):
     part["topk_ids"] = torch.searchsorted(used, ids[rows]).to(torch.int32).cpu()
     ref, bound = moe_oracle(part)
     assert_within(out[rows], ref, bound, "long runs")
+
+
+@pytest.mark.parametrize("tokens,hidden", [(1, 2048), (5, 512), (40, 1024)])
+def test_partial_results_arrive_whole(gpu, tokens, hidden):
+    """Calls with other inputs in turn, so that a partial result of the call before would show."""
+    say(f"moe in turn, {tokens} tokens")
+    cases = [to(gpu, moe_case(tokens, 16, 2, hidden, 256, seed=50 + i)) for i in range(3)]
+    base = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [run(cases[i % 3]) for i in range(300)]
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, base[i % 3]), f"call {i}"
