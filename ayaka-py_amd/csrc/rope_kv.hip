@@ -37,6 +37,7 @@ struct RopeArgs {
   int64_t num_slots, page_size;
   int page_shift;  // log2 of the page size, or -1
   float k_inv, v_inv;
+  bool past;  // rotated rows are stored past the caches
 };
 
 enum Part { kQuery, kKey, kValue };
@@ -144,6 +145,12 @@ __device__ inline uint32_t group_amax(const float* x) {
   return m;
 }
 
+__device__ inline void store16(void* to, uint4 v, bool past) {
+  typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+  if (past) __builtin_nontemporal_store(v4{v.x, v.y, v.z, v.w}, reinterpret_cast<v4*>(to));
+  else *reinterpret_cast<uint4*>(to) = v;
+}
+
 // One token a workgroup row (blockIdx.x), its groups of rows dealt to the waves of the blockIdx.y
 // workgroups. A row of dim elements takes dim / 8 lanes of one wave, eight elements each, with
 // the partner's eight loaded beside them: all of a row's loads come before its stores, so the
@@ -199,10 +206,10 @@ __global__ __launch_bounds__(kRopeThreads) void rope_write_vec_kernel(RopeArgs a
     if constexpr (CT == kMx4) amax = part == kQuery ? 0 : group_amax(x);
     if (!live) continue;
     if (part == kQuery) {
-      *reinterpret_cast<uint4*>(a.q_out + t * a.qo_row + h * a.qo_head + d) = narrow8<QT>(x);
+      store16(a.q_out + t * a.qo_row + h * a.qo_head + d, narrow8<QT>(x), a.past);
       continue;
     }
-    if (part == kKey && a.k_out) *reinterpret_cast<uint4*>(a.k_out + t * a.ko_row + h * a.ko_head + d) = narrow8<QT>(x);
+    if (part == kKey && a.k_out) store16(a.k_out + t * a.ko_row + h * a.ko_head + d, narrow8<QT>(x), a.past);
     if (at.row >= 0)
       cache_store8<QT, CT>(a, part == kKey ? a.key_cache : a.value_cache, part == kKey ? a.key_scales : a.value_scales,
                            part == kKey ? a.k_inv : a.v_inv, at.row, h, c, x, amax);
@@ -278,6 +285,7 @@ struct GatherArgs {
   int page_shift, dim, kv_heads, tile;  // tile: slots of a workgroup
   // j / (dim / 8) = mulhi(j, magic) >> shift for j < 2^31, and j / (kv_heads dim / 8)
   uint32_t head_magic, head_shift, row_magic, row_shift;
+  bool past;  // stores go past the caches
 };
 constexpr int kGatherSpans = 4;  // chunks of a thread whose loads are in flight at once
 
@@ -318,17 +326,17 @@ __global__ __launch_bounds__(kRopeThreads) void mx4_gather_kernel(GatherArgs a) 
       if constexpr (WIDE && DT == AYK_BF16) {  // exact in bf16
         uint4 r = make_uint4(mx4_widen2<0>(w[k], sc), mx4_widen2<1>(w[k], sc), mx4_widen2<2>(w[k], sc), mx4_widen2<3>(w[k], sc));
         if (!known) r = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dest) + e) = r;
+        store16(static_cast<uint16_t*>(a.dest) + e, r, a.past);
       } else {
         float x[8];
         mx4_decode8(w[k], sc, x);
 #pragma unroll
         for (int q = 0; q < 8; ++q) x[q] = known ? x[q] : 0.0f;
         if constexpr (WIDE && DT == AYK_F32) {
-          reinterpret_cast<float4*>(static_cast<float*>(a.dest) + e)[0] = make_float4(x[0], x[1], x[2], x[3]);
-          reinterpret_cast<float4*>(static_cast<float*>(a.dest) + e)[1] = make_float4(x[4], x[5], x[6], x[7]);
+          store16(static_cast<float*>(a.dest) + e, make_uint4(f2u(x[0]), f2u(x[1]), f2u(x[2]), f2u(x[3])), a.past);
+          store16(static_cast<float*>(a.dest) + e + 4, make_uint4(f2u(x[4]), f2u(x[5]), f2u(x[6]), f2u(x[7])), a.past);
         } else if constexpr (WIDE) {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dest) + e) = narrow8<DT>(x);
+          store16(static_cast<uint16_t*>(a.dest) + e, narrow8<DT>(x), a.past);
         } else {
 #pragma unroll
           for (int q = 0; q < 8; ++q) store_f32(a.dest, DT, e + q, x[q]);
@@ -350,6 +358,10 @@ int launch_rope(const RopeArgs& given, int64_t tokens, bool side, bool vec, hipS
     a.q_groups = (int)cdiv(a.heads, a.rows);
     a.kv_groups = (int)cdiv(a.kv_heads, a.rows);
   }
+  // Rotated queries that the second-level caches (32 MiB in all) cannot keep are not left to push out the rest:
+  // 8192 tokens of 32 heads of 128, 67 MB of them, took 40.5 us through the caches and 37.1 past them; 2048
+  // tokens 17.1 and 16.9, and there attention finds them closer.
+  a.past = tokens * a.heads * a.dim * 2 > (int64_t)32 << 20;
   const int64_t groups = vec ? a.q_groups + 2 * a.kv_groups : a.heads + 2 * a.kv_heads;
   // Few tokens: their rows spread over workgroups, a group a wave; many: a workgroup a token, whose
   // waves keep the angles for all their rows.
@@ -498,6 +510,10 @@ int ayk_kv_gather_mxfp4(const void* codes, const void* scales, int64_t num_pages
     const int bits = 64 - __builtin_clzll((uint64_t)by - 1);
     m = (uint32_t)cdiv((int64_t)1 << (31 + bits), by), shift = bits - 1;
   };
+  // Keys and values that together pass the last-level cache (256 MiB) are stored past the caches: two planes of
+  // 132048 rows of 8 heads of 128, 270 MB each, 113 us through them and 83 past; of 32048 rows, 66 MB each,
+  // 28.3 and 26.8, but attention behind them takes 3 us more.
+  a.past = n * kv_heads * dim * (dest_dtype == AYK_F32 ? 4 : 2) > (int64_t)128 << 20;
   magic(per_head, a.head_magic, a.head_shift);
   magic(per_row, a.row_magic, a.row_shift);
   hipStream_t st = static_cast<hipStream_t>(stream);

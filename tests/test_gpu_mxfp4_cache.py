@@ -242,3 +242,20 @@ def test_refusals_on_the_device(gpu):
     refuse_gather(TypeError, "destination must have dtype", destination=torch.empty(4, 2, 64, dtype=torch.float64, device=gpu))
     refuse_gather(ValueError, "one cache row per slot", destination=torch.empty(3, 2, 64, dtype=BF16, device=gpu))
     refuse_gather(ValueError, "contiguous destination", destination=torch.empty(4, 64, 2, dtype=BF16, device=gpu).transpose(1, 2))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gather_past_the_caches(gpu, dtype):
+    """More than 128 MiB of rows, which are stored past the caches, equal the same rows in two halves."""
+    from ayaka.kernel.hip import gather_cache_mxfp4
+
+    say(f"gather_cache_mxfp4 of many rows {dtype}")
+    codes, scales = (t.to(gpu) for t in mx_planes(40, 8, 64, 256, 7))
+    n = (128 << 20) // (8 * 256 * dtype.itemsize) + 77
+    slots = torch.randint(-5, 40 * 64 + 5, (n,), generator=torch.Generator().manual_seed(8)).to(gpu)
+    whole, parts = (torch.full((n, 8, 256), float("nan"), dtype=dtype, device=gpu) for _ in range(2))
+    gather_cache_mxfp4(codes, scales, slots, whole)
+    for half in (slice(0, n // 2), slice(n // 2, n)):
+        gather_cache_mxfp4(codes, scales, slots[half], parts[half])
+    assert torch.equal(bits(whole), bits(parts))
+    assert not whole.isnan().any()

@@ -288,3 +288,17 @@ def test_refusals_on_the_device(gpu):
     refuse(ValueError, "must be a CUDA tensor|same CUDA device", slots=c["slots"].cpu())
     big = lambda n: torch.zeros(4, n, 264, dtype=BF16, device=gpu)  # noqa: E731
     refuse(ValueError, "head_dim between", query=big(4), key=big(2), value=big(2))
+
+
+def test_rows_past_the_caches(gpu):
+    """Rotated rows of more than 32 MiB, which are stored past the caches; in place as well."""
+    check(make(8200, 16, 2, 128, 64, BF16), gpu, "8200 tokens of 16 heads", "vec")
+    c = make(8200, 16, 2, 128, 128, BF16, interleaved=True)
+    want = expected(c)
+    d = to(gpu, c)
+    d["query_out"] = d["query"]
+    from ayaka.kernel.hip import rope_write_kv
+
+    say("rope_write_kv 8200 tokens in place")
+    rope_write_kv(**d)
+    assert torch.equal(bits(d["query"].cpu()), bits(want["query_out"]))
