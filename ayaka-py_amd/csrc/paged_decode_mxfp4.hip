@@ -13,6 +13,16 @@
 // elements, exactly, whatever the scale: fp16 would overflow or lose groups of small or large scale. An
 // fp16 query is split into two bf16 numbers, exactly (8 + 3 bits), and so are the weights, rounded to
 // 16 bits; the products that this adds hide behind the widening.
+//
+// K and V of the next block come to registers while this one is worked on. Long batches run at the memory's
+// pace: 32 x 4096 of 8 kv heads of 128 in 27 us (143 MB, 5.3 TB/s), 1 x 1048576 in 228 (5.0), 64 x 8192 in 122
+// (4.7). What is short of that: a workgroup's own pace, 4096 positions in 20 us, half of it widening and
+// softmax (32 sequences of 0 to 4096: 25 us for 15.5 of bytes), and starts and the second launch
+// (1 x 131072: 32 + 5.3 us for 27.6 of bytes; 1 x 37: 6.3).
+// Tried and left out: K and V through a ring in LDS by direct loads (1 x 262144 70 -> 60 us, but 32 x 4096
+// 27.1 -> 29.1 and 96 windows of 1028 17.6 -> 19.6); sixteen waves a workgroup (ragged batch the same, 32
+// short sequences 7.8 -> 9.1 us); K as the 4-bit operand of the scaled matrix instruction with Q in 8-bit parts:
+// its sums of 128 products were off by up to 2^-12.6 of their magnitudes.
 #include <type_traits>
 
 #include "mxfp4.h"
@@ -34,8 +44,14 @@ struct MxShape {
   static constexpr int kParts = D == 256 ? 2 : 1;          // 16-byte pieces of a K row in each of its four lanes
   static constexpr int kPartWords = D == 64 ? 2 : 4;
   static constexpr int kCols = D / 16;                     // dims of a V row in each of its sixteen lanes
-  static constexpr int kWavesPerSimd = D == 64 ? 4 : D == 128 ? 3 : 1;
 };
+
+// Waves a SIMD that the registers are shared among. 256 dims: two instead of one, 64 x 4096 121 -> 94 us; dealt
+// out with an fp16 query, whose parts do not fit then, one (1 x 32768 28.5 us, 39.6 with two).
+template <int QT, int D, bool SPLIT>
+constexpr int mx_waves() {
+  return D == 64 ? 4 : D == 128 ? 3 : SPLIT && QT == AYK_F16 ? 1 : 2;
+}
 
 // First dim of lane quad `quad`'s eight k slots at step s of the score product.
 template <int D>
@@ -304,7 +320,7 @@ __device__ inline void write_mx(const MxArgs& a, int b, int g, int tile, const R
 
 // One workgroup per sequence, kv head and head tile, whose waves take its blocks in turn.
 template <int QT, int D, bool EXACT, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, (MxShape<D>::kWavesPerSimd)) void mx_decode_kernel(MxArgs a) {
+__global__ __launch_bounds__(WAVES * kWave, (mx_waves<QT, D, false>())) void mx_decode_kernel(MxArgs a) {
   __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
@@ -318,7 +334,7 @@ __global__ __launch_bounds__(WAVES * kWave, (MxShape<D>::kWavesPerSimd)) void mx
 // it does not hold whole it leaves as a partial result, in slot 0 (the run begins inside the item) or
 // slot 1 (it ends inside).
 template <int QT, int D, bool EXACT>
-__global__ __launch_bounds__(kDecodeThreads, (MxShape<D>::kWavesPerSimd)) void mx_decode_split_kernel(MxArgs a) {
+__global__ __launch_bounds__(kDecodeThreads, (mx_waves<QT, D, true>())) void mx_decode_split_kernel(MxArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
   const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
   const int total = __builtin_amdgcn_readfirstlane(total_steps(a));
@@ -357,12 +373,11 @@ int launch_mx(const MxArgs& a, bool split, hipStream_t st) {
   if (!split) {
     const unsigned items = (unsigned)(a.batch * a.tiles * a.kv_items);
     // Two waves a SIMD where a CU has one workgroup at most.
-    constexpr int kMostWaves = MxShape<D>::kWavesPerSimd >= 2 ? 8 : 4;
-    if (items <= 256) hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, kMostWaves>), dim3(items), dim3(kMostWaves * kWave), 0, st, a);
+    if (items <= 256) hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, 8>), dim3(items), dim3(8 * kWave), 0, st, a);
     else hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, 4>), dim3(items), dim3(4 * kWave), 0, st, a);
     note_plan("paged_decode_mxfp4 whole");
   } else {
-    constexpr int runs = 256 * MxShape<D>::kWavesPerSimd;
+    constexpr int runs = 256 * mx_waves<QT, D, true>();
     hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
     launch_join<QT, D, 1>(a, runs, st);
     note_plan("paged_decode_mxfp4 split");
@@ -386,6 +401,12 @@ int64_t mx_longest(int64_t most, int64_t window, int64_t sinks) {
 }
 bool mx_deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest) {
   const int64_t items = batch * cdiv(heads / kv_heads, kHeadTile) * kv_heads;
+  // Whole items pay for the longest, dealt-out ones for the second launch. Few items leave most of the chip idle:
+  // one sequence of 8 kv heads of 128 takes 10.1 us whole and 9.9 dealt out at 1000 positions, 24.9 and 11.1
+  // at 4000; 8 of them at 4096 26.2 and 19.9, 16 27.4 and 27.1, 32 28.3 and 36.7 (ragged 27.3 and 27.6). With a
+  // second workgroup on some CUs, 48 sequences, 48.5 and 43.2 at 4096; with two on all, 64, 55.5 and 65.3, and
+  // 128 at 8192 228 and 242 (ragged 156 and 156). 64 dims cross later (16 at 2048: 11.9 and 13.7, at 4096 19.7
+  // and 17.2), 256 earlier (1 at 1000: 17.5 and 13.2).
   const int64_t width = mx_width(dim), limit = items <= 256 ? 1300 - 3 * width + 15 * items : (items < 512 ? 400 : 560) * 1024 / width;
   return longest > limit && items * (cdiv(longest, kStep) + 1) < 0x40000000;
 }
