@@ -404,10 +404,13 @@ bool mx_deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, i
   // Whole items pay for the longest, dealt-out ones for the second launch. Few items leave most of the chip idle:
   // one sequence of 8 kv heads of 128 takes 10.1 us whole and 9.9 dealt out at 1000 positions, 24.9 and 11.1
   // at 4000; 8 of them at 4096 26.2 and 19.9, 16 27.4 and 27.1, 32 28.3 and 36.7 (ragged 27.3 and 27.6). With a
-  // second workgroup on some CUs, 48 sequences, 48.5 and 43.2 at 4096; with two on all, 64, 55.5 and 65.3, and
-  // 128 at 8192 228 and 242 (ragged 156 and 156). 64 dims cross later (16 at 2048: 11.9 and 13.7, at 4096 19.7
-  // and 17.2), 256 earlier (1 at 1000: 17.5 and 13.2).
-  const int64_t width = mx_width(dim), limit = items <= 256 ? 1300 - 3 * width + 15 * items : (items < 512 ? 400 : 560) * 1024 / width;
+  // second workgroup on some CUs, 48 sequences, 48.5 and 43.2 at 4096 (ragged 24.1 and 25.2 at 2048); with two
+  // on all, 64, 55.5 and 65.3 at 4096, ragged 58.3 and 51.2 at 6000. 64 dims cross later (16 at 2048 11.9 and
+  // 13.7, at 4096 19.7 and 17.2; 48 ragged at 8192 61 and 37), 256 earlier where items are few (1 at 1000 16.0
+  // and 13.6), else as 128 (48 ragged at 2048 38.6 and 47.0, at 4096 68.1 and 64.5; 64 ragged at 4096 81.8 and
+  // 90.0, at 8192 169 and 160).
+  const int64_t width = mx_width(dim), few = 1300 - 3 * width + 15 * items;
+  const int64_t limit = items <= 256 ? few : (items < 512 ? 400 : 560) * 1024 / (width < 128 ? width : 128);
   return longest > limit && items * (cdiv(longest, kStep) + 1) < 0x40000000;
 }
 
