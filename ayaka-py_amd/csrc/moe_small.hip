@@ -11,6 +11,12 @@
 // activations' type, and the columns are tokens. A block of 128 k is summed on its own and joins the
 // fp32 total under its scale. h is kept as two bf16 numbers (16 significant bits, fp32's range): one
 // would add a rounding as coarse as the output's, and fp16 overflows where gate and up are large.
+//
+// 64 tokens of 256 experts, 8 each, 7168 x 2048: 1150 us for 6.37 GB and 534 for 3.19 (5.5 and 6.0 TB/s; a copy of a
+// GiB runs at 5.16). 21 tokens of 8 experts, 2 each, 4096 x 14336: 174 and 92 us (5.4 and 5.1). One token of
+// 64 experts, 6 each, 2048 x 1408: 15.9 and 12.2 us for 6.7 and 3.4 of bytes: start, ids, first weights and, in
+// the second launch, the count and the partial results are trips to memory one behind the other, and 528
+// items over 256 CUs are three on some.
 #include "attn_frag.h"
 
 namespace ayk {
@@ -198,6 +204,9 @@ __device__ inline void read_rows_and_half(uint32_t weights, uint32_t at, uint32_
 // an item. The waves of a workgroup take blocks of 128 k in turn and join their sums in LDS. A wave's
 // weights run kGateAhead half blocks ahead, across items; the tokens' rows of x come in chunks
 // of up to kGatePairs (row, block) pairs of 256 bytes, a chunk ahead.
+// Tried and left out: weights through registers (1910 us for the second launch of the first case above), six half blocks ahead
+// (nothing), items of eight channels, gate and up rows in one tile (256 experts with 256 inner channels, one
+// token, 26.0 -> 23.4 us for both launches, but the small layer 28.0 -> 31.1 and every larger batch by 10 to 20%).
 constexpr int kGateAhead = 4;  // half blocks: gate or up rows
 constexpr int kGatePairs = 128;
 constexpr int kGatePairBytes = 2 * kMoeBlock;
@@ -439,8 +448,8 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
 // partial results, which the last workgroup to finish adds in the runs' order. Sums of an expert's
 // rows join those of their tokens in LDS, where each lane owns its cells: results do not depend on
 // the order of waves.
-// A wave's weights run kDownAhead blocks ahead; the rows of h, which the waves share, come in chunks of
-// up to kDownPairs (row, block) pairs of 512 bytes, a chunk ahead.
+// A wave's weights run kDownAhead blocks ahead (six: nothing); the rows of h, which the waves share, come in
+// chunks of up to kDownPairs (row, block) pairs of 512 bytes, a chunk ahead.
 constexpr int kDownAhead = 4;
 constexpr int kDownPairs = 32;
 constexpr int kPairBytes = 4 * kMoeBlock;
@@ -476,7 +485,8 @@ __device__ inline void read_block(uint32_t weights, uint32_t at, uint32_t scales
 
 // A walk over the chunks of a workgroup's run, [unit, last) in the list of (expert, block). All is the
 // same in all lanes. A chunk goes on into the next entries while its rows, as many for every unit, have
-// room: with one entry a chunk, two blocks of 128 k an expert took 1.4 us each, a trip to memory. An
+// room: with one entry a chunk, two blocks of 128 k an expert took 1.4 us each, a trip to memory (30 tokens of
+// 256 experts with 256 inner channels 120 us, now 81 for 57 of bytes). An
 // entry of more than kDownRows rows takes its units one by one, each in passes.
 constexpr int kDownRows = 32;
 struct DownWalk {
