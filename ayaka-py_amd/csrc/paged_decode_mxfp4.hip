@@ -409,7 +409,7 @@ bool mx_deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, i
   // 13.7, at 4096 19.7 and 17.2; 48 ragged at 8192 61 and 37), 256 earlier where items are few (1 at 1000 16.0
   // and 13.6), else as 128 (48 ragged at 2048 38.6 and 47.0, at 4096 68.1 and 64.5; 64 ragged at 4096 81.8 and
   // 90.0, at 8192 169 and 160).
-  const int64_t width = mx_width(dim), few = 1300 - 3 * width + 15 * items;
+  const int64_t width = mx_width(dim), few = 1360 - 3 * width + 15 * items;
   const int64_t limit = items <= 256 ? few : (items < 512 ? 400 : 560) * 1024 / (width < 128 ? width : 128);
   return longest > limit && items * (cdiv(longest, kStep) + 1) < 0x40000000;
 }
