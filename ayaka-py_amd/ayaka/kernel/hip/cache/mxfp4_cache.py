@@ -39,14 +39,16 @@ def check_plane(codes: torch.Tensor, scales: torch.Tensor, name: str) -> tuple[i
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         require_dtype(codes, f"{name}_codes", (torch.uint8,))
         require_dtype(scales, f"{name}_scales", (torch.uint8,))
-    shape, groups = codes.shape, scales.shape
-    if len(shape) != 4 or len(groups) != 4 or shape[:3] != groups[:3]:
+    if codes.ndim != 4 or scales.ndim != 4:
         raise ValueError(f"{name}_codes and {name}_scales must be [pages, kv_heads, page_size, head_dim / 2] and [..., head_dim / 32]")
-    pages, kv_heads, page_size, half = shape
+    pages, kv_heads, page_size, half = codes.shape
+    their_pages, their_heads, their_size, groups = scales.shape
+    if their_pages != pages or their_heads != kv_heads or their_size != page_size:
+        raise ValueError(f"{name}_codes and {name}_scales must be [pages, kv_heads, page_size, head_dim / 2] and [..., head_dim / 32]")
     dim = 2 * half
-    if dim % GROUP or not GROUP <= dim <= MAX_HEAD_DIM or groups[3] * GROUP != dim:
+    if dim % GROUP or not GROUP <= dim <= MAX_HEAD_DIM or groups * GROUP != dim:
         raise ValueError(f"the head_dim of a 4-bit cache must be a multiple of {GROUP} up to {MAX_HEAD_DIM}, with a scale for every "
-                         f"{GROUP} dims; got {dim} dims and {groups[3]} scales")
+                         f"{GROUP} dims; got {dim} dims and {groups} scales")
     if kv_heads < 1 or page_size < 8 or page_size % 8:
         raise ValueError(f"a 4-bit cache needs kv_heads and a page_size that is a multiple of 8, got {kv_heads} and {page_size}")
     _check_memory(codes, scales, name)
