@@ -201,7 +201,8 @@ __device__ inline void read_rows_and_half(uint32_t weights, uint32_t at, uint32_
 }
 
 // Gate and up projections of sixteen inner channels for the tokens of one expert, the activation, and h:
-// an item. The waves of a workgroup take blocks of 128 k in turn and join their sums in LDS. A wave's
+// an item. The waves of a group take blocks of 128 k in turn and join their sums in LDS; the groups of a
+// workgroup, one for long rows of weights, up to eight for short ones, take an item each. A wave's
 // weights run kGateAhead half blocks ahead, across items; the tokens' rows of x come in chunks
 // of up to kGatePairs (row, block) pairs of 256 bytes, a chunk ahead.
 // Tried and left out: weights through registers (1910 us for the second launch of the first case above), six half blocks ahead
@@ -212,11 +213,12 @@ constexpr int kGatePairs = 128;
 constexpr int kGatePairBytes = 2 * kMoeBlock;
 constexpr int kGateRows = 16;  // of a pass over an item
 
-// A walk over the chunks of a workgroup's items, a run of consecutive ones. All but `table` is the
-// same in all lanes.
+// A walk over the chunks of a workgroup's steps. A step is up to GROUPS consecutive items of one entry, one
+// for each group of waves. All but `table` is the same in all lanes.
+template <int GROUPS>
 struct GateWalk {
   int item, last, slices, blocks;
-  int u, slice, r0, b0, count;  // list entry, sixteen channels, first row, first block, blocks (0: no more)
+  int u, slice, wide, r0, b0, count;  // list entry, first sixteen channels, items, first row, first block, blocks (0: no more)
   int expert, first_row, all, rows, stride;
   int table;  // the entry's tokens
   __device__ void enter(const MoeList& l) {  // the entry of `item`
@@ -228,17 +230,19 @@ struct GateWalk {
     table = token_table(tokens);
     all = __popcll(tokens);
     r0 = b0 = 0;
+    step();
     size();
   }
+  __device__ void step() { wide = min(GROUPS, min(slices - slice, last - item)); }
   __device__ void size() {
     rows = all - r0 < kGateRows ? all - r0 : kGateRows;
     stride = power_of_two_from(rows);
     const int most = kGatePairs / stride;  // whole eights: every wave's share
     count = blocks - b0 < most ? blocks - b0 : most;
   }
-  __device__ bool ends_item() const { return b0 + count == blocks; }
+  __device__ bool ends_step() const { return b0 + count == blocks; }
   __device__ void next(const MoeList& l) {
-    if (!ends_item()) {
+    if (!ends_step()) {
       b0 += count;
       size();
       return;
@@ -247,14 +251,17 @@ struct GateWalk {
     r0 += kGateRows;
     if (r0 >= all) {
       r0 = 0;
-      if (++item >= last) {
+      item += wide;
+      slice += wide;
+      if (item >= last) {
         count = 0;
         return;
       }
-      if (++slice == slices) {
+      if (slice == slices) {
         enter(l);
         return;
       }
+      step();
     }
     size();
   }
@@ -274,7 +281,7 @@ struct Entries {
   __device__ int rows(int u) const { return (uint32_t)__builtin_amdgcn_readlane(packed, u - base) >> 16; }
   __device__ int row(int u) const { return __builtin_amdgcn_readlane(first, u - base); }
 };
-template <int DT>
+template <int DT, int GROUPS>
 __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) {
   __shared__ MoeList list;
   __shared__ alignas(1024) uint8_t stage[2][kGatePairs * kGatePairBytes];
@@ -294,9 +301,11 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   const int blocks = a.hidden / kMoeBlock, block_rows = a.inner / kMoeBlock;
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < blocks; i += kMoeThreads) a.arrived[i] = 0;
-  GateWalk walk;
+  GateWalk<GROUPS> walk;
   walk.slices = a.inner / 16;
   walk.blocks = blocks;
+  constexpr int per = kMoeWaves / GROUPS;  // waves of a group
+  const int group = wave / per, mate = wave % per;
   const int64_t items = (int64_t)__builtin_amdgcn_readfirstlane(list.count) * walk.slices;
   walk.item = (int)(items * blockIdx.x / gridDim.x);
   walk.last = (int)(items * (blockIdx.x + 1) / gridDim.x);
@@ -304,45 +313,51 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   walk.enter(list);
 
   // Weights: lane l of a load takes sixteen bytes of row l % 16, piece l / 16 of 64 bytes. A wave's
-  // blocks of an item's pass are its number and every eighth from there, whatever the chunks (all but
-  // a pass's last are whole eights); past the last pass that is loaded again, so that the waits count
-  // the same throughout.
+  // blocks of an item's pass are its number in the group and every `per` from there, whatever the chunks
+  // (all but a pass's last are whole eights); past the last pass that is loaded again, so that the waits
+  // count the same throughout.
   const uint32_t lane_at = (uint32_t)col * a.hidden + 16 * quad, ring = lds_address(rings[wave]);
   Entries entries;
   entries.hold(list, walk.u);
   const int64_t up_bytes = (int64_t)a.inner * a.hidden;
-  int item = walk.item, entry = walk.u, slice = walk.slice, pass = 0, passes = 1, at = wave;
+  // This wave's items are its group's of the steps, which begin at the run's first item and at every entry's.
+  int item, begin = walk.item, end = min(walk.last, (walk.u + 1) * walk.slices), entry = walk.u, pass = 0, passes = 1, at = mate;
   const uint8_t* from = a.gate_up;
-  auto point = [&]() {  // at this wave's first block (one without any loads the last, and does not read it)
+  auto point = [&]() {  // at its first block (a wave without any loads the last, and does not read it)
     passes = (entries.rows(entry) + kGateRows - 1) / kGateRows;
-    from = a.gate_up + ((int64_t)entries.expert(entry) * 2 * a.inner + 16 * slice) * a.hidden + min(wave, blocks - 1) * kMoeBlock;
-    at = wave;
+    from = a.gate_up + ((int64_t)entries.expert(entry) * 2 * a.inner + 16 * (item - entry * walk.slices)) * a.hidden +
+           min(mate, blocks - 1) * kMoeBlock;
+    at = mate;
   };
+  auto seek = [&](int next) {  // the next item from `next` on, in this entry or a later one, or the last again
+    while (next >= end && end < walk.last) {
+      ++entry;  // (no run has more than five: 8192 items of 1024 experts over 256 workgroups)
+      begin = end;
+      end = min(walk.last, begin + walk.slices);
+      next = begin + group;
+    }
+    item = min(next, end - 1);
+  };
+  seek(begin + group);
   point();
   auto issue = [&](int to, bool up) {
     load_to_lds(from + (up ? up_bytes : 0), lane_at, ring + 2048 * to);
     load_to_lds(from + (up ? up_bytes : 0) + 64, lane_at, ring + 2048 * to + 1024);
     if (!up) return;
-    at += kMoeWaves;
+    at += per;
     if (at < blocks) {
-      from += kMoeWaves * kMoeBlock;
+      from += per * kMoeBlock;
       return;
     }
     if (++pass >= passes) {
       pass = 0;
-      if (item + 1 < walk.last) {
-        ++item;
-        if (++slice == walk.slices) {
-          slice = 0;
-          ++entry;  // (no run has more than five: 8192 items of 1024 experts over 256 workgroups)
-        }
-      }
+      seek(item + GROUPS);
     }
     point();
   };
   // Rows: a wave takes sixteen pairs, four a load, and lane l piece l % 16 of its pair. Pieces are
   // exchanged within a pair so that the same piece of sixteen rows lies in sixteen groups of banks.
-  auto fetch = [&](const GateWalk& w, int buffer) {
+  auto fetch = [&](const GateWalk<GROUPS>& w, int buffer) {
     const int shift = __builtin_ctz(w.stride);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -353,8 +368,8 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
                   lds_address(stage[buffer] + (16 * wave + 4 * i) * kGatePairBytes));
     }
     // The block scales come with them: read where they are used, they cost a trip to memory an item.
-    const int block = wave + kMoeWaves * (lane % 16);
-    word_to_lds(a.gate_up_scale + ((int64_t)(2 * w.expert + (lane / 16 & 1)) * block_rows + w.slice / 8) * blocks + w.b0 +
+    const int block = mate + per * (lane % 16), slice = w.slice + min(group, w.wide - 1);
+    word_to_lds(a.gate_up_scale + ((int64_t)(2 * w.expert + (lane / 16 & 1)) * block_rows + slice / 8) * blocks + w.b0 +
                     (block < w.count ? block : 0),
                 lds_address(scales[buffer][wave]));
   };
@@ -367,11 +382,11 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
   float weight_table = 0.0f;
   v4f g{0, 0, 0, 0}, w{0, 0, 0, 0};
   while (true) {
-    GateWalk following = walk;
+    GateWalk<GROUPS> following = walk;
     following.next(list);
     fetch(following.count ? following : walk, buffer ^ 1);
     int mine = 0;
-    for (int c = wave; c < walk.count; c += kMoeWaves, ++mine) {
+    for (int c = group < walk.wide ? mate : walk.count; c < walk.count; c += per, ++mine) {
       const int pair = c * walk.stride + (col & (walk.stride - 1));
       const uint32_t rows = lds_address(stage[buffer]) + pair * kGatePairBytes + 16 * ((2 * quad) ^ (pair & 15));
       v4u xs[4], raw[2];
@@ -395,7 +410,7 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
     // past them, of one they are counted.
     if (mine == 1) wait_loads<4>();
     else if (mine == 0) wait_loads<0>();
-    if (walk.ends_item()) {
+    if (walk.ends_step()) {
       auto part = reinterpret_cast<float(*)[2][16][16]>(stage[buffer]);  // [wave]: its rows have all been read
       __builtin_amdgcn_s_barrier();
 #pragma unroll
@@ -405,7 +420,6 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
       }
       g = w = v4f{0, 0, 0, 0};
       lds_barrier();
-      const int r = threadIdx.x / 16, n = threadIdx.x % 16;
       if (walk.u != weighed) {  // the weights of a new entry's rows, row l to lane l
         weighed = walk.u;
         weight_table = 0.0f;
@@ -419,18 +433,20 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
           }
         }
       }
-      const float weight = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(4 * (walk.r0 + r), (int)f2u(weight_table)));
-      if (r < walk.rows) {
+      for (int o = threadIdx.x; o < 256 * walk.wide; o += kMoeThreads) {  // whole waves
+        const int of = o / 256, r = o / 16 % 16, n = o % 16;
+        const float weight = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(4 * (walk.r0 + r), (int)f2u(weight_table)));
+        if (r >= walk.rows) continue;
         float gate_sum = 0.0f, up_sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kMoeWaves; ++v) {
-          gate_sum += part[v][0][r][n];
-          up_sum += part[v][1][r][n];
+        for (int v = 0; v < per; ++v) {
+          gate_sum += part[of * per + v][0][r][n];
+          up_sum += part[of * per + v][1][r][n];
         }
         const float y = weight * (gate_sum / (1.0f + expf(-gate_sum)) * up_sum);
         const uint16_t hi = f32_to_bf16_bits(y);
         const float rest = y - bf16_bits_to_f32(hi);
-        uint16_t* to = a.h + ((int64_t)(walk.first_row + walk.r0 + r) * a.inner + 16 * walk.slice + n / 8 * 8) * 2 + n % 8;
+        uint16_t* to = a.h + ((int64_t)(walk.first_row + walk.r0 + r) * a.inner + 16 * (walk.slice + of) + n / 8 * 8) * 2 + n % 8;
         to[0] = hi;
         to[8] = f32_to_bf16_bits(rest == rest ? rest : 0.0f);  // an infinity has no second part
       }
@@ -751,7 +767,18 @@ template <int DT>
 int launch_moe(const MoeArgs& a, hipStream_t st) {
   const int64_t pairs = (int64_t)a.tokens * a.topk, used = pairs < a.experts ? pairs : a.experts;
   const int64_t items = used * (a.inner / 16);
-  hipLaunchKernelGGL((moe_gate_up_kernel<DT>), dim3((unsigned)(items < 256 ? items : 256)), dim3(kMoeThreads), 0, st, a);
+  // Every item costs a join of its waves, about a microsecond: rows of weights that leave a wave less than four
+  // blocks are shared among fewer waves, several items at once, where a workgroup has that many: 15 tokens of 256
+  // experts, 768 x 5376, 53.6 us with one, 34.1 with eight; 8 tokens of 64, 6 each, 2048 x 1408, 59.2 and 51
+  // with two; where two items a workgroup were shared among four groups, 13.9 became 16.4.
+  const int blocks = a.hidden / kMoeBlock;
+  int groups = blocks >= 32 ? 1 : blocks >= 16 ? 2 : blocks >= 8 ? 4 : 8;
+  while (groups > 1 && items < 256 * groups) groups /= 2;
+  const dim3 first((unsigned)(items < 256 ? items : 256));
+  if (groups == 8) hipLaunchKernelGGL((moe_gate_up_kernel<DT, 8>), first, dim3(kMoeThreads), 0, st, a);
+  else if (groups == 4) hipLaunchKernelGGL((moe_gate_up_kernel<DT, 4>), first, dim3(kMoeThreads), 0, st, a);
+  else if (groups == 2) hipLaunchKernelGGL((moe_gate_up_kernel<DT, 2>), first, dim3(kMoeThreads), 0, st, a);
+  else hipLaunchKernelGGL((moe_gate_up_kernel<DT, 1>), first, dim3(kMoeThreads), 0, st, a);
   const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner));
   hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), (a.tokens < 16 ? 16 : a.tokens) * kTokenFloats * sizeof(float), st, a);
   return check_launch("fp8_block_moe_small");

@@ -299,3 +299,14 @@ def test_partial_results_arrive_whole(gpu, tokens, hidden):
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert torch.equal(g, base[i % 3]), f"call {i}"
+
+
+@pytest.mark.parametrize("tokens,experts,topk,hidden,inner", [
+    (40, 40, 4, 640, 896), (7, 64, 8, 128, 768), (64, 300, 8, 256, 128), (33, 40, 4, 896, 1024), (40, 40, 4, 1024, 512),
+    (20, 60, 6, 1152, 384), (64, 130, 4, 1920, 128), (40, 40, 4, 2048, 256), (12, 50, 6, 2944, 256), (64, 80, 2, 3968, 128)])
+def test_several_items_at_once(gpu, tokens, experts, topk, hidden, inner):
+    """Short rows of weights: groups of waves take an item each, over runs that end anywhere in an entry."""
+    c = moe_case(tokens, experts, topk, hidden, inner, seed=hidden + inner)
+    if tokens > 32:
+        c["topk_ids"][:36, 0] = 3  # more rows than one pass holds
+    check(c, gpu, f"{tokens} tokens, {experts} experts, {hidden} x {inner}")
