@@ -310,3 +310,11 @@ def test_several_items_at_once(gpu, tokens, experts, topk, hidden, inner):
     if tokens > 32:
         c["topk_ids"][:36, 0] = 3  # more rows than one pass holds
     check(c, gpu, f"{tokens} tokens, {experts} experts, {hidden} x {inner}")
+
+
+@pytest.mark.parametrize("tokens,topk", [(64, 20), (33, 32), (64, 40)])
+def test_more_choices_than_lds_holds(gpu, tokens, topk):
+    """More than 1024 (token, choice) pairs: ids and weights are read where they are used."""
+    c = moe_case(tokens, 40, topk, 256, 128, seed=60 + topk, away=0.2)
+    c["topk_ids"][5, 3] = c["topk_ids"][5, 4]
+    check(c, gpu, f"{tokens} tokens of {topk} choices")

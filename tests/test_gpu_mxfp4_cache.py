@@ -259,3 +259,38 @@ def test_gather_past_the_caches(gpu, dtype):
         gather_cache_mxfp4(codes, scales, slots[half], parts[half])
     assert torch.equal(bits(whole), bits(parts))
     assert not whole.isnan().any()
+
+
+def test_a_cache_without_pages(gpu):
+    """Nothing is written, rows read back are zeros, queries are rotated all the same."""
+    from ayaka.kernel.hip import gather_cache_mxfp4, rope_write_kv_mxfp4, write_kv_mxfp4
+
+    c = make(5, 4, 2, 64, 64)
+    want = expected(c)
+    d = to(gpu, c)
+    for n in PLANES:
+        d[n] = d[n][:0].clone()
+    say("mxfp4 cache without pages")
+    rope_write_kv_mxfp4(**d)
+    same(d, {n: want[n] for n in ("query_out", "key_out")}, "no pages")
+    write_kv_mxfp4(d["key"], d["value"], *(d[n] for n in PLANES), d["slots"])
+    for dtype in (F32, F16, BF16):
+        rows = torch.full((5, 2, 64), float("nan"), dtype=dtype, device=gpu)
+        gather_cache_mxfp4(d["key_codes"], d["key_scales"], d["slots"], rows)
+        assert not rows.any()
+
+
+@pytest.mark.parametrize("kv_heads,dim,n", [(1, 32, 70000), (3, 96, 1000), (40, 256, 300), (200, 256, 3), (1, 256, 1)])
+def test_gather_of_any_row_size(gpu, kv_heads, dim, n):
+    """Rows shorter and longer than a workgroup's span, and counts that end inside one."""
+    from ayaka.kernel.hip import gather_cache_mxfp4
+
+    say(f"gather_cache_mxfp4 {n} rows of {kv_heads} x {dim}")
+    codes, scales = mx_planes(5, kv_heads, 24, dim, 9)
+    slots = torch.randint(-3, 5 * 24 + 3, (n,), generator=torch.Generator().manual_seed(n))
+    values = deco.by_position(deco.mx_values(codes, scales)).flatten(0, 1)
+    inside = (slots >= 0) & (slots < 5 * 24)
+    want = torch.where(inside[:, None, None], values[slots.clamp(0, 119)], 0.0).to(BF16)
+    got = torch.full((n, kv_heads, dim), float("nan"), dtype=BF16, device=gpu)
+    gather_cache_mxfp4(codes.to(gpu), scales.to(gpu), slots.to(gpu), got)
+    assert torch.equal(bits(got.cpu()), bits(want))
