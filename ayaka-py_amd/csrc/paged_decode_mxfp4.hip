@@ -132,18 +132,24 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
   // Row 4 (l / 16) + i of score tile t is position 8 (l / 16) + 4 t + i: the lane's weights are then
   // those of eight positions in a row, in the order of V's k slots.
   uint32_t kw[2][S::kParts * S::kPartWords], kse[2][S::kParts], vw[8][D == 256 ? 2 : 1], vse[D == 64 ? 4 : 8];
+  // Addresses are a lane's own part, formed once, the eight's, and what the instruction adds.
+  const uint8_t *k_lane[S::kParts], *ks_lane[S::kParts];
+#pragma unroll
+  for (int h = 0; h < S::kParts; ++h) {
+    const int dim = mx_k_dim<D>(4 * h, quad), there = EXACT || dim < a.dim ? dim : 0;
+    k_lane[h] = kc + col % 4 * row_bytes + there / 2;
+    ks_lane[h] = ks + col % 4 * groups + there / kMxGroup;
+  }
   auto issue_k = [&](uint32_t row) {
-    const uint32_t eight = (uint32_t)__builtin_amdgcn_ds_bpermute(32 * (col / 4), (int)row);
+    const uint64_t eight = (uint32_t)__builtin_amdgcn_ds_bpermute(32 * (col / 4), (int)row);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint64_t at = eight + 4 * t + col % 4;
+    for (int h = 0; h < S::kParts; ++h) {
+      const uint8_t *p = k_lane[h] + eight * row_bytes, *q = ks_lane[h] + eight * groups;
 #pragma unroll
-      for (int h = 0; h < S::kParts; ++h) {
-        const int dim = mx_k_dim<D>(4 * h, quad), there = EXACT || dim < a.dim ? dim : 0;
-        const uint8_t* p = kc + at * row_bytes + there / 2;
-        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = *reinterpret_cast<const v2u*>(p);
-        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = *reinterpret_cast<const v4u*>(p);
-        kse[t][h] = *reinterpret_cast<const uint8_t*>(ks + at * groups + there / kMxGroup);
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = *reinterpret_cast<const v2u*>(p + 4 * t * row_bytes);
+        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = *reinterpret_cast<const v4u*>(p + 4 * t * row_bytes);
+        kse[t][h] = q[4 * t * groups];
       }
     }
   };
