@@ -59,7 +59,14 @@ __device__ inline int mx_k_dim(int s, int quad) {
   return D == 64 ? 16 * quad + 8 * s : 128 * (s / 4) + 32 * quad + 8 * (s % 4);
 }
 
-template <int QT, int D, bool EXACT, int WAVES>
+template <bool PAST, typename T>
+__device__ inline T mx_load(const uint8_t* p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else return *reinterpret_cast<const T*>(p);
+}
+
+// PAST: K and V are read past the caches.
+template <int QT, int D, bool EXACT, int WAVES, bool PAST>
 __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int tile, int from, int to, Running<D>& r) {
   using S = MxShape<D>;
   typedef uint32_t v2u __attribute__((ext_vector_type(2)));
@@ -147,8 +154,8 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
       const uint8_t *p = k_lane[h] + eight * row_bytes, *q = ks_lane[h] + eight * groups;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = *reinterpret_cast<const v2u*>(p + 4 * t * row_bytes);
-        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = *reinterpret_cast<const v4u*>(p + 4 * t * row_bytes);
+        if constexpr (D == 64) *reinterpret_cast<v2u*>(kw[t]) = mx_load<PAST, v2u>(p + 4 * t * row_bytes);
+        else *reinterpret_cast<v4u*>(kw[t] + 4 * h) = mx_load<PAST, v4u>(p + 4 * t * row_bytes);
         kse[t][h] = q[4 * t * groups];
       }
     }
@@ -164,9 +171,9 @@ __device__ inline void attend_mx(const MxArgs& a, int b, int len, int g, int til
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint8_t* p = vc + (eight + j) * row_bytes + v_dim / 2;
-      if constexpr (D == 64) vw[j][0] = *reinterpret_cast<const uint16_t*>(p);
-      else if constexpr (D == 128) vw[j][0] = *reinterpret_cast<const uint32_t*>(p);
-      else *reinterpret_cast<v2u*>(vw[j]) = *reinterpret_cast<const v2u*>(p);
+      if constexpr (D == 64) vw[j][0] = mx_load<PAST, uint16_t>(p);
+      else if constexpr (D == 128) vw[j][0] = mx_load<PAST, uint32_t>(p);
+      else *reinterpret_cast<v2u*>(vw[j]) = mx_load<PAST, v2u>(p);
       if constexpr (!kVector) {
         const uint32_t code = *reinterpret_cast<const uint8_t*>(vs + (eight + j) * groups + v_group);
         if constexpr (D == 64) vse[j / 2] = (j % 2 ? vse[j / 2] : 0) | code << (16 * (j % 2) + 8 * v_group);
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(WAVES * kWave, (mx_waves<QT, D, false>())) void mx_
   __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_mx<QT, D, EXACT, WAVES>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
+  attend_mx<QT, D, EXACT, WAVES, false>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
   join_waves<D, WAVES>(r, lds);
   if (threadIdx.x < kWave) write_mx<QT, D, EXACT>(a, b, g, tile, r, nullptr);
 }
@@ -339,7 +346,7 @@ __global__ __launch_bounds__(WAVES * kWave, (mx_waves<QT, D, false>())) void mx_
 // workgroup, whatever the lengths. A run may end one item, hold some whole and begin another; what
 // it does not hold whole it leaves as a partial result, in slot 0 (the run begins inside the item) or
 // slot 1 (it ends inside).
-template <int QT, int D, bool EXACT>
+template <int QT, int D, bool EXACT, bool PAST>
 __global__ __launch_bounds__(kDecodeThreads, (mx_waves<QT, D, true>())) void mx_decode_split_kernel(MxArgs a) {
   __shared__ float lds[2][D / 4 + 2][kWave];
   const int lane = threadIdx.x % kWave, per = a.tiles * a.kv_items;
@@ -363,7 +370,7 @@ __global__ __launch_bounds__(kDecodeThreads, (mx_waves<QT, D, true>())) void mx_
       const int last = first + (end - at) < steps ? first + (end - at) : steps;
       Running<D> r;
       const int b = chunk + k, g = item % a.kv_items, tile = item / a.kv_items;
-      attend_mx<QT, D, EXACT, 4>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
+      attend_mx<QT, D, EXACT, 4, PAST>(a, b, __builtin_amdgcn_readlane(len, k), g, tile, first, last, r);
       join_waves<D, 4>(r, lds);
       float* partial = nullptr;
       if (first > 0 || last < steps) partial = a.partial + ((int64_t)run * 2 + (first > 0 ? 0 : 1)) * a.rows * (D + 2);
@@ -384,9 +391,11 @@ int launch_mx(const MxArgs& a, bool split, hipStream_t st) {
     note_plan("paged_decode_mxfp4 whole");
   } else {
     constexpr int runs = 256 * mx_waves<QT, D, true>();
-    hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    constexpr bool kLines = EXACT && D >= 128;
+    if (kLines && a.once) hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT, kLines>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
+    else hipLaunchKernelGGL((mx_decode_split_kernel<QT, D, EXACT, false>), dim3(runs), dim3(kDecodeThreads), 0, st, a);
     launch_join<QT, D, 1>(a, runs, st);
-    note_plan("paged_decode_mxfp4 split");
+    note_plan(kLines && a.once ? "paged_decode_mxfp4 split, past the caches" : "paged_decode_mxfp4 split");
   }
   return check_launch("paged_decode_attention_mxfp4");
 }
@@ -457,6 +466,7 @@ int ayk_paged_decode_attention_mxfp4(const void* q, int q_dtype, int64_t q_row_s
     return fail(AYK_EINVAL, "%s: a plane has more than 2^32 rows of a head", op);
   if (batch == 0) return AYK_OK;
   const int64_t most = table_width * page_size, group = heads / kv_heads, tiles = cdiv(group, kHeadTile);
+  const int64_t longest = mx_longest(most, window, sinks);
   if (heads > 65535 || batch > kMostGroups || batch * tiles * kv_heads > kMostGroups)
     return fail(AYK_EINVAL, "%s: batch and heads exceed the grid", op);
   if (q == nullptr || out == nullptr || seq_lens == nullptr || (table_width > 0 && block_tables == nullptr) ||
@@ -491,6 +501,11 @@ int ayk_paged_decode_attention_mxfp4(const void* q, int q_dtype, int64_t q_row_s
   a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctzll((uint64_t)page_size);
   a.scale_log2 = fabsf(scale) * kLog2e;
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
+  // Where the tables can name more than the last-level cache holds, 256 MiB, and one tile of heads reads each row:
+  // 128 x 8192 of 8 kv heads of 128 236 us through the caches, 227 past them, 4 x 262144 239 and 233, 32 x 16384
+  // of 256 dims 221 and 213; where it holds them, 1 x 131072, 36 and 42.
+  const double named = (double)batch * (double)(longest < most ? longest : most) * (double)kv_heads * (double)(dim + dim / 16);
+  a.once = tiles == 1 && named > (double)(256 << 20);
   a.v_scale = 1.0f;
   a.window = (int)(window < 0x7FFFFFFF ? window : 0x7FFFFFFF);
   a.sinks = (int)(sinks < 0x7FFFFFFF ? sinks : 0x7FFFFFFF);

@@ -306,3 +306,15 @@ def test_refusals_on_the_device(gpu):
     refuse(ValueError, "sinks must not be negative", sinks=-1)
     refuse(ValueError, "must be a CUDA tensor|same CUDA device", seq_lens=c["seq_lens"].cpu())
     refuse(ValueError, "out must be contiguous", out=torch.empty(2, 64, 4, dtype=BF16, device=gpu).transpose(1, 2))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim,page", [(128, 16), (128, 40), (256, 16)])
+def test_past_the_caches(gpu, dtype, dim, page):
+    """Tables that name more than 256 MiB: read past the caches, with the same bits."""
+    wide = 2**29 // (2 * 2 * dim * page) + 1
+    c = decode_case([5000, 900], 8, 2, dim, page, dtype, seed=70, spare_width=wide)
+    out = check(c, gpu, f"past the caches, {dim} dims", "split, past the caches")
+    c["block_tables"] = c["block_tables"][:, : -(-5000 // page) + 2].contiguous()
+    say("the same through the caches")
+    assert torch.equal(run(to(gpu, c)).cpu(), out)
