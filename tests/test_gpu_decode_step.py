@@ -186,3 +186,29 @@ def test_a_compiled_step(gpu, cache):
     for got, want in (*zip(compiled, eager), *zip(layers[1].planes, layers[0].planes)):
         assert torch.equal(bits(got), bits(want))
     assert layers[1].planes[0].view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("cache", [None, E4M3])
+def test_a_compiled_rotation_in_place(gpu, cache):
+    """Queries and keys that are their own results, as slices of one projection."""
+    import ayaka.kernel.hip as H
+
+    ex = _example()
+    layers = [_layer(ex, gpu, cache) for _ in range(2)]
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 12, 64, generator=gen).to(BF16).to(gpu)
+    positions, slots = torch.tensor([7, 0, 90], device=gpu), torch.tensor([3, -1, 77], device=gpu)
+
+    def step(x, planes, table):
+        qkv = x * 2
+        q, k, v = qkv.split((8, 2, 2), dim=1)
+        if cache is None:
+            H.rope_write_kv_mxfp4(q, k, v, positions, table, *planes, slots, q, key_out=k)
+        else:
+            H.rope_write_kv(q, k, v, positions, table, *planes, slots, 16.0, 16.0, q, key_out=k)
+        return qkv, q + 1, k + 1
+
+    eager = step(x, layers[0].planes, layers[0].table)
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)(x, layers[1].planes, layers[1].table)
+    for got, want in (*zip(compiled, eager), *zip(layers[1].planes, layers[0].planes)):
+        assert torch.equal(bits(got), bits(want))
