@@ -72,12 +72,14 @@ struct Running {
 // What a result under maximum m counts under a common one.
 __device__ inline float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
 
-// Join the waves' results in wave 0: the upper half hands theirs to the lower, and so on.
+// Join the waves' results in wave 0: the upper half hands theirs to the lower, and so on. Waves from `busy` on
+// (the same for all) have none.
 template <int D, int WAVES>
-__device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave]) {
+__device__ inline void join_waves(Running<D>& r, float (*lds)[D / 4 + 2][kWave], int busy = WAVES) {
   const int lane = item_lane(), wave = threadIdx.x / kWave;
 #pragma unroll
   for (int half = WAVES / 2; half >= 1; half /= 2) {
+    if (half >= busy) continue;
     __syncthreads();  // the slots' last readers are done
     if (wave >= half && wave < 2 * half) {
       float(*to)[kWave] = lds[wave - half];

@@ -18,7 +18,7 @@
 // pace: 32 x 4096 of 8 kv heads of 128 in 27 us (143 MB, 5.3 TB/s), 1 x 1048576 in 228 (5.0), 64 x 8192 in 122
 // (4.7). What is short of that: a workgroup's own pace, 4096 positions in 20 us, half of it widening and
 // softmax (32 sequences of 0 to 4096: 25 us for 15.5 of bytes), and starts and the second launch
-// (1 x 131072: 32 + 5.3 us for 27.6 of bytes; 1 x 37: 6.3).
+// (1 x 131072: 32 + 5.3 us for 27.6 of bytes; 1 x 37: 5.0).
 // Tried and left out: K and V through a ring in LDS by direct loads (1 x 262144 70 -> 60 us, but 32 x 4096
 // 27.1 -> 29.1 and 96 windows of 1028 17.6 -> 19.6); sixteen waves a workgroup (ragged batch the same, 32
 // short sequences 7.8 -> 9.1 us); K as the 4-bit operand of the scaled matrix instruction with Q in 8-bit parts:
@@ -337,8 +337,9 @@ __global__ __launch_bounds__(WAVES * kWave, (mx_waves<QT, D, false>())) void mx_
   __shared__ float lds[WAVES / 2][D / 4 + 2][kWave];
   const int g = blockIdx.x % a.kv_items, tile = blockIdx.x / a.kv_items % a.tiles, b = blockIdx.x / a.kv_items / a.tiles;
   Running<D> r;
-  attend_mx<QT, D, EXACT, WAVES, false>(a, b, a.lens[b], g, tile, 0, 0x1FFFFFF, r);
-  join_waves<D, WAVES>(r, lds);
+  const int len = __builtin_amdgcn_readfirstlane(a.lens[b]);
+  attend_mx<QT, D, EXACT, WAVES, false>(a, b, len, g, tile, 0, 0x1FFFFFF, r);
+  join_waves<D, WAVES>(r, lds, blocks_of(a, len).count);
   if (threadIdx.x < kWave) write_mx<QT, D, EXACT>(a, b, g, tile, r, nullptr);
 }
 
