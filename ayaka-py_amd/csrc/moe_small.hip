@@ -444,11 +444,17 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_gate_up_kernel(MoeArgs a) 
           up_sum += part[of * per + v][1][r][n];
         }
         const float y = weight * (gate_sum / (1.0f + expf(-gate_sum)) * up_sum);
-        const uint16_t hi = f32_to_bf16_bits(y);
+        // A finite y that bf16 would round to infinity has the largest bf16 as its first part, and the rest cut off, not
+        // rounded, in the second: rounded, the two could make 2^128. What is not finite itself has no second
+        // part (asked of y, as the difference may be formed from the unrounded product).
+        const bool finite = fabsf(y) < INFINITY;
+        uint16_t hi = f32_to_bf16_bits(y);
+        const bool past = finite && (hi & 0x7FFF) == 0x7F80;
+        if (past) --hi;
         const float rest = y - bf16_bits_to_f32(hi);
         uint16_t* to = a.h + ((int64_t)(walk.first_row + walk.r0 + r) * a.inner + 16 * (walk.slice + of) + n / 8 * 8) * 2 + n % 8;
         to[0] = hi;
-        to[8] = f32_to_bf16_bits(rest == rest ? rest : 0.0f);  // an infinity has no second part
+        to[8] = !finite ? 0 : past ? (uint16_t)(f2u(rest) >> 16) : f32_to_bf16_bits(rest);
       }
     }
     if (following.count == 0) break;
