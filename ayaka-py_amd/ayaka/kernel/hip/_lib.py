@@ -218,7 +218,7 @@ def call(name: str, *args: Any) -> None:
 
 
 def last_plan() -> str:
-    """The kernels (and K split) of the last GEMM launch on this thread."""
+    """The kernels (and K split) of the last launch on this thread that notes them (``ayk_last_plan``)."""
     return (load_library().ayk_last_plan() or b"").decode("utf-8", "replace")
 
 

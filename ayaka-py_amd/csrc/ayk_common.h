@@ -354,7 +354,7 @@ inline void launch_split_reduce(ScalarKernel scalar, const float* part, int64_t 
 int fail(int status, const char* fmt, ...);
 int check_launch(const char* what);
 int check_device();
-// Records which kernels and split the last GEMM launch on this thread used (read back
+// Records which kernels and split the last launch on this thread used (read back
 // through ayk_last_plan; tests assert that a case reaches the kernel it targets).
 void note_plan(const char* fmt, ...);
 

@@ -785,8 +785,10 @@ int launch_moe(const MoeArgs& a, hipStream_t st) {
   else if (groups == 4) hipLaunchKernelGGL((moe_gate_up_kernel<DT, 4>), first, dim3(kMoeThreads), 0, st, a);
   else if (groups == 2) hipLaunchKernelGGL((moe_gate_up_kernel<DT, 2>), first, dim3(kMoeThreads), 0, st, a);
   else hipLaunchKernelGGL((moe_gate_up_kernel<DT, 1>), first, dim3(kMoeThreads), 0, st, a);
-  const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner));
+  const int runs = down_runs(a.tokens, a.topk, a.experts, a.hidden, a.inner);
+  const dim3 grid((unsigned)(a.hidden / kMoeBlock), (unsigned)runs);
   hipLaunchKernelGGL((moe_down_kernel<DT>), grid, dim3(kMoeThreads), (a.tokens < 16 ? 16 : a.tokens) * kTokenFloats * sizeof(float), st, a);
+  note_plan("moe_small groups=%d runs=%d", groups, runs);
   return check_launch("fp8_block_moe_small");
 }
 
