@@ -387,9 +387,10 @@ int launch_mx(const MxArgs& a, bool split, hipStream_t st) {
   if (!split) {
     const unsigned items = (unsigned)(a.batch * a.tiles * a.kv_items);
     // Two waves a SIMD where a CU has one workgroup at most.
-    if (items <= 256) hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, 8>), dim3(items), dim3(8 * kWave), 0, st, a);
+    const bool eight = items <= 256;
+    if (eight) hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, 8>), dim3(items), dim3(8 * kWave), 0, st, a);
     else hipLaunchKernelGGL((mx_decode_kernel<QT, D, EXACT, 4>), dim3(items), dim3(4 * kWave), 0, st, a);
-    note_plan("paged_decode_mxfp4 whole");
+    note_plan(eight ? "paged_decode_mxfp4 whole" : "paged_decode_mxfp4 whole, four waves");
   } else {
     constexpr int runs = 256 * mx_waves<QT, D, true>();
     constexpr bool kLines = EXACT && D >= 128;
