@@ -646,7 +646,7 @@ __global__ __launch_bounds__(kMoeThreads, 2) void moe_down_kernel(MoeArgs a) {
 #pragma unroll
     for (int s = 0; s < kDownAhead; ++s) issue(s);
     wait_loads<2 * kDownAhead>();
-    __builtin_amdgcn_s_barrier();
+    lds_barrier();  // and the zeros of `sums`, which other waves' lanes add to
     int buffer = 0;
     while (true) {
       DownWalk following = walk;
