@@ -6,7 +6,9 @@ A plane is two uint8 tensors, ``codes [pages, kv_heads, page_size, head_dim / 2]
 of a byte; every 32 dims of a row share one UE8M0 scale, the least power of two under which
 none of them exceeds 6 (as ``per_token_group_quant_mxfp8`` scales its groups, for a largest code
 of 448). So there is no calibrated scale, and a cached element takes 4.25 bits. A group that
-holds an infinity or NaN is NaN as a whole; magnitudes over 1.5 * 2^127 count as that.
+holds an infinity or NaN is NaN as a whole; magnitudes over 1.5 * 2^127 count as that. Scale code
+``s`` stands for 2^(s - 127) from 0 on and 255 for NaN; a group of zeros is written with scale code 0 and
+codes of zero. (The mxfp8 products take scale code 0 for a factor of 0 instead.)
 
 The planes are head-major, unlike the 16-bit and fp8 caches: a head's rows of a page are
 consecutive, as its attention reads them. No counterpart in the reference. There is no CPU path.
@@ -173,6 +175,10 @@ def gather_cache_mxfp4(codes: torch.Tensor, scales: torch.Tensor, slots: torch.T
         slots: int64 ``[n]``, repeats allowed; a slot outside the plane gives a zero row.
         destination: contiguous fp32/fp16/bf16 of ``n * kv_heads * head_dim`` elements, ``[n,
             kv_heads, head_dim]`` as ``varlen_attention`` takes keys and values.
+
+    Every value of a cache is exact in fp32 and bf16. fp16 rounds, and has no value for what is held as 65536 or
+    more: it comes back infinite. Of rows that were fp16 when they were written these are the magnitudes
+    from 57344 on.
     """
     check_devices(codes, "codes", scales=scales, slots=slots, destination=destination)
     pages, kv_heads, page_size, dim = check_plane(codes, scales, "cache")

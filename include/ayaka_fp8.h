@@ -324,7 +324,7 @@ int ayk_rope_kv_write(const void* q, int64_t q_row_stride, int64_t q_head_stride
                       const int64_t* slots, float k_inverse, float v_inverse, ayk_stream_t stream);
 /* The same into a 4-bit cache. A plane is codes [num_pages, kv_heads, page_size, dim / 2] (OCP
  * e2m1, the even dim in the low half of a byte) and scales [num_pages, kv_heads, page_size, dim / 32]
- * (UE8M0: value 2^(code - 127), 0xFF NaN), both contiguous. A group of 32 dims takes the least scale
+ * (UE8M0: 2^(code - 127) from code 0 on, where the mxfp8 products have a factor of 0; 0xFF NaN), both contiguous. A group of 32 dims takes the least scale
  * under which no magnitude exceeds 6, codes are rounded to nearest even; zeros have scale code 0, a
  * group with an infinity or NaN has 0xFF. dim % 32 == 0; slot = page * page_size + offset. */
 int ayk_rope_kv_write_mxfp4(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, int64_t k_row_stride,
@@ -336,7 +336,8 @@ int ayk_rope_kv_write_mxfp4(const void* q, int64_t q_row_stride, int64_t q_head_
                             void* value_scales, int64_t num_pages, int64_t page_size, const int64_t* slots,
                             ayk_stream_t stream);
 /* dest[i] = the values of slot slots[i] of one 4-bit plane, [n, kv_heads, dim] in fp32, fp16 or bf16.
- * A slot outside the plane gives zeros. */
+ * A slot outside the plane gives zeros. fp32 and bf16 hold every value exactly; fp16 rounds, and what is held
+ * as 65536 or more (of fp16 rows the magnitudes from 57344 on) comes back infinite. */
 int ayk_kv_gather_mxfp4(const void* codes, const void* scales, int64_t num_pages, int64_t page_size, int64_t kv_heads,
                         int64_t dim, const int64_t* slots, int64_t n, void* dest, int dest_dtype, ayk_stream_t stream);
 
