@@ -3,8 +3,9 @@
 //   h[t, e] = w_te silu(gate[e] x[t]) * (up[e] x[t]),   out[t] = sum_e down[e] h[t, e]
 //
 // over the experts e that token t names, w_te the sum of the weights it names e with. Weights are e4m3
-// under 128 x 128 block scales, activations 16 bits. HBM-bound: the weights of every expert that
-// some token names are read once, for all its tokens.
+// under 128 x 128 block scales, activations 16 bits. HBM-bound where an expert has few tokens: its weights are
+// read once for up to sixteen of them in the first launch, up to thirty-two in the second, and again for every
+// further sixteen or thirty-two (a pass).
 //
 // Both kernels are matrix products with the weights as the first operand, sixteen rows a tile: a lane's
 // eight k slots of a 16x16x32 step are eight consecutive bytes of a row, widened exactly to the
@@ -12,11 +13,14 @@
 // fp32 total under its scale. h is kept as two bf16 numbers (16 significant bits, fp32's range): one
 // would add a rounding as coarse as the output's, and fp16 overflows where gate and up are large.
 //
-// 64 tokens of 256 experts, 8 each, 7168 x 2048: 1150 us for 6.37 GB and 534 for 3.19 (5.5 and 6.0 TB/s; a copy of a
-// GiB runs at 5.16). 21 tokens of 8 experts, 2 each, 4096 x 14336: 174 and 92 us (5.4 and 5.1). One token of
-// 64 experts, 6 each, 2048 x 1408: 15.9 and 12.2 us for 6.7 and 3.4 of bytes: start, ids, first weights and, in
-// the second launch, the count and the partial results are trips to memory one behind the other, and 528
-// items over 256 CUs are three on some.
+// Medians of a kernel trace: 64 tokens of 256 experts, 8 each, 7168 x 2048: 1171 us for 6.37 GB and 510 for 3.19
+// (5.4 and 6.2 TB/s; a copy of a GiB runs at 5.16). 21 tokens of 8 experts, 2 each, 4096 x 14336: 180 and 95 us
+// (5.2 and 5.0). One token of 64 experts, 6 each, 2048 x 1408: 15.5 and 12.1 us for 6.7 and 3.4 of bytes: start, ids,
+// first weights and, in the second launch, the count and the partial results are trips to memory one behind
+// the other, and 528 items over 256 CUs are three on some.
+// What passes cost, 8 experts of 4096 x 14336 (0.94 and 0.47 GB): 64 tokens of 2 each, 14 to 18 rows an expert, two
+// passes for some of them: 310 us (1.06 GB fetched) and 164 (0.54); of 8 each, 64 rows, four and two passes: 704
+// (3.10 GB) and 362 (0.71). Up to sixteen rows an expert there is one.
 #include "attn_frag.h"
 
 namespace ayk {

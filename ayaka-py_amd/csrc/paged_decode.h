@@ -148,7 +148,9 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_decode_join_kernel(Decode
   const float* p = a.partial + (int64_t)col * (D + 2);
   auto slot = [&](int w) { return p + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * stride; };
   // The first partial results are on their way while the maximum is found (a load past the last is one of
-  // the last again): one trip to memory less, 0.9 us of 6.3.
+  // the last again): one trip to memory less, 0.9 us of 6.3 for 64 rows of 96 partial results. Rows of few pay nothing
+  // for it: 15 calls over 16-bit and fp8 caches, 32 to 12800 rows, took 0.1% longer at most and 1.3% less at best
+  // (64 sequences of 16384 and 128 heads 458.8 us without, 459.0 with; 1 x 16384 and 32 heads 15.1 and 14.9).
   constexpr int kAhead = 6;
   const int mine = w0 + wave % kShare;
   float m[kAhead], sum_of[kAhead], v[kAhead][kPer];

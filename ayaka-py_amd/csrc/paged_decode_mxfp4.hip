@@ -15,10 +15,11 @@
 // 16 bits; the products that this adds hide behind the widening.
 //
 // K and V of the next block come to registers while this one is worked on. Long batches run at the memory's
-// pace: 32 x 4096 of 8 kv heads of 128 in 27 us (143 MB, 5.3 TB/s), 1 x 1048576 in 228 (5.0), 64 x 8192 in 122
-// (4.7). What is short of that: a workgroup's own pace, 4096 positions in 20 us, half of it widening and
-// softmax (32 sequences of 0 to 4096: 25 us for 15.5 of bytes), and starts and the second launch
-// (1 x 131072: 32 + 5.3 us for 27.6 of bytes; 1 x 37: 5.0).
+// pace: 32 x 4096 of 8 kv heads of 128 in 27 us (143 MB, 5.3 TB/s), 1 x 1048576 in 198 (5.8), 64 x 8192 in 124
+// (4.6); of 256 dims 32 x 4096 in 50 to 53 (285 MB, 5.5) and 64 x 4096 in 105 (5.4). What is short of that: a
+// workgroup's own pace, 4096 positions of 128 dims in 20 us, half of it widening and softmax (32 sequences of 0 to
+// 4096: 25 us for 15.5 of bytes), and starts and the second launch (1 x 131072: 31 + 5.7 us for 27.6 of bytes;
+// 1 x 32768 of 256 dims 26 for 13.8; 1 x 37: 5.1).
 // Tried and left out: K and V through a ring in LDS by direct loads (1 x 262144 70 -> 60 us, but 32 x 4096
 // 27.1 -> 29.1 and 96 windows of 1028 17.6 -> 19.6); sixteen waves a workgroup (ragged batch the same, 32
 // short sequences 7.8 -> 9.1 us); K as the 4-bit operand of the scaled matrix instruction with Q in 8-bit parts:
@@ -46,8 +47,13 @@ struct MxShape {
   static constexpr int kCols = D / 16;                     // dims of a V row in each of its sixteen lanes
 };
 
-// Waves a SIMD that the registers are shared among. 256 dims: two instead of one, 64 x 4096 121 -> 94 us; dealt
-// out with an fp16 query, whose parts do not fit then, one (1 x 32768 28.5 us, 39.6 with two).
+// Waves a SIMD that the registers are shared among. 256 dims: two instead of one, 48 ragged sequences of 2048 and
+// 8 kv heads 39.9 -> 37.6 us, 64 x 4096 107.0 -> 105.2; dealt out with an fp16 query, whose parts do not fit then,
+// one (1 x 32768 28.5 us, 39.6 with two). Of the others that are dealt out some spill a few vector registers: fp16
+// at 128 dims three (six where the head is padded to them) and bf16 at 256 one. With a wave less they do not: fp16
+// at 128 dims and two waves, 1 x 131072 35.0 us against 38.6 and 64 x 8192 109 against 120, but 32 ragged
+// sequences of 16384 77.6 against 75.2; bf16 at 256 dims and one, 1 x 32768 25.7 against 26.0 and 32 x 16384 198
+// against 194.
 template <int QT, int D, bool SPLIT>
 constexpr int mx_waves() {
   return D == 64 ? 4 : D == 128 ? 3 : SPLIT && QT == AYK_F16 ? 1 : 2;
@@ -419,13 +425,18 @@ int64_t mx_longest(int64_t most, int64_t window, int64_t sinks) {
 bool mx_deals_out(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest) {
   const int64_t items = batch * cdiv(heads / kv_heads, kHeadTile) * kv_heads;
   // Whole items pay for the longest, dealt-out ones for the second launch. Few items leave most of the chip idle:
-  // one sequence of 8 kv heads of 128 takes 10.1 us whole and 9.9 dealt out at 1000 positions, 24.9 and 11.1
-  // at 4000; 8 of them at 4096 26.2 and 19.9, 16 27.4 and 27.1, 32 28.3 and 36.7 (ragged 27.3 and 27.6). With a
-  // second workgroup on some CUs, 48 sequences, 48.5 and 43.2 at 4096 (ragged 24.1 and 25.2 at 2048); with two
-  // on all, 64, 55.5 and 65.3 at 4096, ragged 58.3 and 51.2 at 6000. 64 dims cross later (16 at 2048 11.9 and
-  // 13.7, at 4096 19.7 and 17.2; 48 ragged at 8192 61 and 37), 256 earlier where items are few (1 at 1000 16.0
-  // and 13.6), else as 128 (48 ragged at 2048 38.6 and 47.0, at 4096 68.1 and 64.5; 64 ragged at 4096 81.8 and
-  // 90.0, at 8192 169 and 160).
+  // one sequence of 8 kv heads of 128 takes 10.0 us whole and 10.6 dealt out at 1000 positions, 10.2 and 10.6 at
+  // 1092 (a window of 1024 with four first tokens 10.1 and 10.6), 11.1 and 10.6 at 1200, 24.9 and 11.1 at 4000
+  // (calls one by one, host included, 12.7 and 16.8 up to 1400); four at 1400 11.6 and 11.7; 8 of them at 4096 26.2
+  // and 19.9, 16 27.4 and 27.1, 32 28.3 and 36.7 (ragged 27.3 and 27.6). With a second workgroup on some CUs, 48
+  // sequences, 48.5 and 43.2 at 4096 (ragged 24.1 and 25.2 at 2048); with two on all, 64, 55.5 and 65.3 at 4096,
+  // ragged 58.3 and 51.2 at 6000. 64 dims cross later (16 at 2048 11.9 and 13.7, at 4096 19.7 and 17.2; 48 ragged at
+  // 8192 61 and 37; one at 1300 8.7 and 9.3, at 1800 10.4 and 9.4), 256 earlier where items are few (1 at 600 13.0
+  // and 13.6, at 700 14.5 and 13.7, at 1100 17.1 and 13.7), else as 128 (48 ragged at 2048 38.6 and 47.0, at 4096
+  // 68.1 and 64.5; 64 ragged at 4096 81.8 and 90.0, at 8192 169 and 160).
+  // The rule goes by what the table can name, as lengths are on the device: a table much wider than its sequences costs
+  // (32 x 1000 with tables of 32768 positions 21.5 us, 11.7 with their own; 32 ragged sequences of 4096 with 131072 28.5
+  // and 25.3; 8 x 1000 12.4 and 10.3).
   const int64_t width = mx_width(dim), few = 1360 - 3 * width + 15 * items;
   const int64_t limit = items <= 256 ? few : (items < 512 ? 400 : 560) * 1024 / (width < 128 ? width : 128);
   return longest > limit && items * (cdiv(longest, kStep) + 1) < 0x40000000;
@@ -505,7 +516,7 @@ int ayk_paged_decode_attention_mxfp4(const void* q, int q_dtype, int64_t q_row_s
   a.q_sign = scale < 0.0f ? 0x80008000u : 0u;
   // Where the tables can name more than the last-level cache holds, 256 MiB, and one tile of heads reads each row:
   // 128 x 8192 of 8 kv heads of 128 236 us through the caches, 227 past them, 4 x 262144 239 and 233, 32 x 16384
-  // of 256 dims 221 and 213; where it holds them, 1 x 131072, 36 and 42.
+  // of 256 dims 221 and 213; where it holds them, 1 x 131072, 36 and 42 (39 by a table of 1048576 positions).
   const double named = (double)batch * (double)(longest < most ? longest : most) * (double)kv_heads * (double)(dim + dim / 16);
   a.once = tiles == 1 && named > (double)(256 << 20);
   a.v_scale = 1.0f;

@@ -11,9 +11,11 @@
 // Bound by HBM for long prompts, by launch and latency for decode steps. Between projection and
 // attention every element is read once and written once; separate kernels for the rotation and the
 // write would read the keys twice and launch twice. One token of 16 + 8 + 8 heads of 128 takes 2.8 us, 64 of
-// 64 + 8 + 8 3.7, 8192 of 32 + 8 + 8 with the rotated keys handed on 37.1 (206 MB, 5.5 TB/s; a copy of a
-// GiB runs at 5.16). 2048 tokens into the 4-bit cache take 16.8 for 43 MB: start, a token's place and its
-// angles are trips to memory one behind the other, about 6 us of it.
+// 64 + 8 + 8 3.8, 8192 of 32 + 8 + 8 with the rotated keys handed on 37.1 (206 MB, 5.5 TB/s; a copy of a
+// GiB runs at 5.16). 2048 tokens into the 4-bit cache take 17.8 for 43 MB that no cache holds (11.5 where they lie in
+// the last-level cache): start, a token's place and its angles are trips to memory one behind the other, about 6
+// us of it, and a row's loads wait for its token's place. Keys and values of 2048 tokens without rotation take 5.5
+// there; one token of 32 + 8 + 8 into the 4-bit cache 2.8, 256 4.1.
 #include "attn_rows.h"
 #include "ayk_common.h"
 #include "mxfp4.h"
@@ -295,7 +297,7 @@ constexpr int kGatherSpans = 4;  // chunks of a thread whose loads are in flight
 // Rows of a 4-bit plane by slot, widened: destination [n, kv_heads, dim]. A thread takes 8 codes of
 // one head of one slot at a time, the heads of a slot side by side, so that the stores, two thirds of the
 // bytes and more, are consecutive. Slots outside the plane give zeros. HBM-bound: 32048 rows of 8 heads of 128
-// in 18.9 us (83 MB, 4.4 TB/s), 26.7 with one chunk a thread and a division for every index.
+// in 18.6 us (83 MB, 4.5 TB/s), 26.7 with one chunk a thread and a division for every index.
 template <int DT, bool WIDE>
 __global__ __launch_bounds__(kRopeThreads) void mx4_gather_kernel(GatherArgs a) {
   const int64_t first = (int64_t)blockIdx.x * a.tile, left = a.n - first;
@@ -369,7 +371,7 @@ int launch_rope(const RopeArgs& given, int64_t tokens, bool side, bool vec, hipS
   const int64_t groups = vec ? a.q_groups + 2 * a.kv_groups : a.heads + 2 * a.kv_heads;
   // Few tokens: their rows spread over workgroups, a group a wave; many: a workgroup a token, whose
   // waves keep the angles for all their rows (a workgroup a group instead: 8192 tokens 40.9 -> 49.7 us; the next
-// rows asked for ahead: 2048 tokens 16.8 -> 16.4, but 8192 45.2).
+  // rows asked for ahead: 2048 tokens 16.8 -> 16.4, but 8192 45.2).
   const int64_t most = cdiv(groups, kRopeWaves), want = cdiv(1024, tokens);
   const dim3 grid((unsigned)tokens, (unsigned)(want < most ? want : most));
   if (!vec) hipLaunchKernelGGL((rope_write_rows_kernel<QT, CT>), grid, dim3(kRopeThreads), 0, st, a, (int)side);
